@@ -10,7 +10,11 @@ The Python functions mirror the reference's host interface (mma_half.cu):
 A, B, C may be integer device addresses or CUDA tensors (their data_ptr() is used). Like the
 reference, `solve` returns nothing and synchronizes the device; its outcome is available from
 last_status(). `launch*` return immediately (asynchronous) and raise HgemmError on a failed
-launch. Everything goes through the C ABI of libhgemm_b200.so; there is no fallback path.
+launch. Next to the projections of an attention layer (no counterpart in the reference):
+    lora(X, W, down, up, scale, seg_start, seg_adapter)    projection with adapters of many requests
+    qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq)     norms and position rotation
+    attn_prompt(q, k, v, cu_q)                             attention over packed sequences
+Everything goes through the C ABI of libhgemm_b200.so; there is no fallback path.
 """
 import ctypes
 
@@ -21,7 +25,19 @@ from ._native import (HGEMM_ERR_DEVICE_TIMEOUT, HGEMM_ERR_INVALID_ARG, HGEMM_OK,
 __all__ = ["solve", "launch", "launch_tuned", "launch_host", "gemm", "plan", "last_status",
            "status_string",
            "device_status", "release", "HgemmError", "set_wait_timeout_ns",
-           "selftest_wait_timeout", "shard_rows"]
+           "selftest_wait_timeout", "shard_rows", "lora", "qk_norm_rope", "attn_prompt"]
+
+_OPERATORS = ("lora", "qk_norm_rope", "attn_prompt")
+
+
+def __getattr__(name):
+    # The operators take torch tensors; torch is imported with the first of them.
+    if name in _OPERATORS:
+        from . import operators
+        for n in _OPERATORS:
+            globals()[n] = getattr(operators, n)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 class HgemmError(RuntimeError):

@@ -37,6 +37,37 @@ class HgemmPlan(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+def _args_struct(name, doc, fields):
+    """A ctypes mirror of one of the header's argument structures."""
+    return type(name, (ctypes.Structure,), {"__doc__": doc, "_fields_": fields})
+
+
+_P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+
+HgemmLora = _args_struct(
+    "HgemmLora", "hgemm_lora_t",
+    [(n, _P) for n in ("X", "W", "Y", "down", "up", "scale", "seg_start", "seg_adapter",
+                       "workspace")] +
+    [("workspace_bytes", ctypes.c_size_t)] +
+    [(n, _I) for n in ("tokens", "N", "K", "rank", "adapters", "segments")])
+
+HgemmQkNormRope = _args_struct(
+    "HgemmQkNormRope", "hgemm_qk_norm_rope_t",
+    [(n, _P) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "positions", "axis_of",
+                       "inv_freq")] +
+    [(n, _L) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride")] +
+    [(n, _I) for n in ("tokens", "heads_q", "heads_kv", "head_dim", "rot_dim", "axes",
+                       "interleaved")] + [("eps", ctypes.c_float)])
+
+HgemmAttnPrompt = _args_struct(
+    "HgemmAttnPrompt", "hgemm_attn_prompt_t",
+    [(n, _P) for n in ("q", "k", "v", "out", "lse", "cu_q", "cu_k")] +
+    [(n, _L) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] +
+    [("workspace", _P), ("workspace_bytes", ctypes.c_size_t)] +
+    [(n, _I) for n in ("total_q", "total_k", "batch", "heads_q", "heads_kv", "head_dim",
+                       "causal")] + [("scale", ctypes.c_float)])
+
+
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
@@ -63,6 +94,11 @@ SIGNATURES = {
     "hgemm_selftest_peer_entry": (_i, [_i, ctypes.c_ulonglong]),
     "hgemm_release": (None, []),
     "hgemm_plan": (_i, [_i, _i, _i, _f, _i, _i, _i, _i, _i, _i, ctypes.POINTER(HgemmPlan)]),
+    "hgemm_lora": (_i, [ctypes.POINTER(HgemmLora), _vp]),
+    "hgemm_lora_workspace_bytes": (ctypes.c_size_t, [_i] * 6),
+    "hgemm_qk_norm_rope": (_i, [ctypes.POINTER(HgemmQkNormRope), _vp]),
+    "hgemm_attn_prompt": (_i, [ctypes.POINTER(HgemmAttnPrompt), _vp]),
+    "hgemm_attn_prompt_workspace_bytes": (ctypes.c_size_t, [_i] * 6),
     "hgemm_comm_unique_id": (_i, [_vp, ctypes.c_size_t]),
     "hgemm_comm_init": (_i, [ctypes.POINTER(_vp), _i, _vp, ctypes.c_size_t, _i]),
     "hgemm_comm_destroy": (_i, [_vp]),

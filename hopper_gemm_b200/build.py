@@ -2,7 +2,7 @@
 
 Produces, next to this file:
   libhgemm_b200.so       the GEMM product: tcgen05 kernel, dispatcher, C ABI, NCCL row shards,
-                         host-buffer pipeline
+                         host-buffer pipeline, and the operators of a served attention layer
   libhgemm_cublas_ref.so the cuBLAS comparator used by bench.py and the GPU tests
   libhgemm_cutlass_ref.so the CUTLASS SM100 comparator (third grid column, cross-check tests),
                          built when CUTLASS's headers are found (the copies vendored in the
@@ -67,9 +67,12 @@ def _run(cmd, verbose):
 def build(force=False, verbose=True, extra_flags=()):
     nvcc = _nvcc()
     common = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I" + INCLUDE,
-                     "-I" + CSRC] + list(extra_flags)
-    srcs = [os.path.join(CSRC, f) for f in ("hgemm_sm100.cu", "hgemm_sharded.cpp", "hgemm_host.cpp")]
-    deps = srcs + [os.path.join(CSRC, "ptx_sm100.cuh"), os.path.join(INCLUDE, "hgemm_b200.h")]
+                     "-I" + CSRC, "--threads", "0"] + list(extra_flags)
+    srcs = [os.path.join(CSRC, f) for f in ("hgemm_sm100.cu", "lora.cu", "qk_norm_rope.cu",
+                                             "attn_prompt.cu", "hgemm_sharded.cpp",
+                                             "hgemm_host.cpp")]
+    deps = srcs + [os.path.join(CSRC, "ptx_sm100.cuh"),
+                   os.path.join(CSRC, "ops_sm100.cuh"), os.path.join(INCLUDE, "hgemm_b200.h")]
     if force or _stale(LIB, deps):
         _run([nvcc] + common + ["-shared", "-o", LIB] + srcs + ["-ldl"], verbose)
     csrc = [os.path.join(CSRC, "cublas_ref.cu")]

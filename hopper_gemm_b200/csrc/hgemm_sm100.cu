@@ -45,6 +45,7 @@
 #include <vector>
 
 #include "hgemm_b200.h"
+#include "ops_sm100.cuh"
 #include "ptx_sm100.cuh"
 
 namespace hgemm {
@@ -1711,6 +1712,7 @@ struct DevState {
   bool attr_done[kNumTiles][kNumFlavors] = {};
   void *scratch = nullptr;
   size_t scratch_bytes = 0;
+  unsigned *status_word = nullptr;  // device address of g_dev_status
 };
 std::mutex g_mu;
 DevState g_dev[64];
@@ -2230,6 +2232,66 @@ void noalloc_forget_addresses();
 }  // namespace
 }  // namespace hgemm
 
+// ============================================================================ operators
+// What the operators in lora.cu, qk_norm_rope.cu and attn_prompt.cu take from this file.
+namespace hgemm {
+
+int op_device(OpDevice *out) {
+  int dev;
+  if (current_device(&dev) != HGEMM_OK) return HGEMM_ERR_CUDA;
+  std::lock_guard<std::mutex> lock(g_mu);
+  DevState *d = nullptr;
+  const int st = ensure_device(dev, &d);
+  if (st != HGEMM_OK) return st;
+  if (!d->status_word) {
+    void *p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_dev_status) != cudaSuccess) {
+      cudaGetLastError();
+      return HGEMM_ERR_CUDA;
+    }
+    d->status_word = static_cast<unsigned *>(p);
+  }
+  out->dev = dev;
+  out->sm_count = d->sm_count;
+  out->status_word = d->status_word;
+  out->timeout_ns = g_timeout_ns.load();
+  return HGEMM_OK;
+}
+
+int op_status(int status) { return set_status(status); }
+
+bool op_encode(CUtensorMap *map, const void *ptr, int rank, const unsigned long long *dims,
+               const unsigned long long *strides, const unsigned *box) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t gdim[5], gstride[4];
+  cuuint32_t bx[5], estride[5];
+  for (int i = 0; i < rank; ++i) {
+    gdim[i] = dims[i];
+    bx[i] = box[i];
+    estride[i] = 1;
+    if (i > 0) gstride[i - 1] = strides[i - 1];
+  }
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank),
+             const_cast<void *>(ptr), gdim, gstride, bx, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int op_smem(const void *kernel, int smem, int dev, bool *done) {
+  std::lock_guard<std::mutex> lock(g_mu);
+  if (done[dev]) return HGEMM_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+      cudaSuccess) {
+    cudaGetLastError();
+    return HGEMM_ERR_CUDA;
+  }
+  done[dev] = true;
+  return HGEMM_OK;
+}
+
+}  // namespace hgemm
+
 // ============================================================================ C ABI
 using namespace hgemm;
 
@@ -2571,6 +2633,7 @@ void hgemm_release(void) {
       g_dev[i].scratch = nullptr;
       g_dev[i].scratch_bytes = 0;
     }
+    g_dev[i].status_word = nullptr;
   }
   cudaSetDevice(cur);
   g_tune.clear();

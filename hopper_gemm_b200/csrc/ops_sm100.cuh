@@ -1,0 +1,79 @@
+// Shared by the operators that run next to the GEMM (lora.cu, qk_norm_rope.cu, attn_prompt.cu):
+// what they take from hgemm_sm100.cu (device check, status word, tensor maps) and the bounded
+// mbarrier wait of their kernels.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "hgemm_b200.h"
+#include "ptx_sm100.cuh"
+
+namespace hgemm {
+
+// The current device as an operator's launcher needs it.
+struct OpDevice {
+  int dev;
+  int sm_count;
+  unsigned *status_word;          // device status word (see hgemm_device_status)
+  unsigned long long timeout_ns;  // bound of one wait in a kernel
+};
+// Checks that the current device is an sm_100 and fills `out`; returns a status code.
+int op_device(OpDevice *out);
+// Keeps a call's status for hgemm_last_status() and returns it.
+int op_status(int status);
+// Tensor map of binary16 elements, 128-byte swizzle, zero fill outside: `rank` dimensions,
+// innermost first, byte strides of dimensions 1.. .
+bool op_encode(CUtensorMap *map, const void *ptr, int rank, const unsigned long long *dims,
+               const unsigned long long *strides, const unsigned *box);
+// Opts `kernel` in to `smem` bytes of dynamic shared memory on device `dev`, once per process
+// and device (`done` is the caller's per-kernel array of 64 flags).
+int op_smem(const void *kernel, int smem, int dev, bool *done);
+
+inline bool op_aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Wait sites of the operators' kernels in the device status word (the GEMM uses 1..12).
+enum OpWaitSite : unsigned {
+  kSiteAttnQ = 32,
+  kSiteAttnKvFull = 33,
+  kSiteAttnKvEmpty = 34,
+  kSiteAttnScores = 35,
+  kSiteAttnWeights = 36,
+  kSiteAttnOut = 37,
+  kSiteLoraEmpty = 40,
+  kSiteLoraFull = 41,
+  kSiteLoraAcc = 42,
+  kSiteOpDrain = 63,
+};
+
+// Bounded wait of one thread; false when the CTA is unwinding or the wait ran out (recorded in
+// the device status word, and the CTA's abort flag raised so that every role unwinds).
+struct OpWait {
+  volatile int *abort_flag;  // shared memory
+  unsigned *status_word;
+  unsigned long long timeout_ns;
+};
+__device__ __forceinline__ bool op_wait(uint32_t bar, uint32_t parity, const OpWait &w,
+                                        unsigned site) {
+  if (ptx::mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = ptx::globaltimer();
+  for (uint32_t n = 1;; ++n) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    if ((n & 15u) == 0) {
+      if (*w.abort_flag) return false;
+      if (ptx::globaltimer() - t0 > w.timeout_ns) {
+        atomicCAS(w.status_word, 0u, 0x100u | site);
+        *w.abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+// Teardown form: ignores the abort flag and records nothing.
+__device__ __forceinline__ void op_drain(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = ptx::globaltimer();
+  while (!ptx::mbar_try_wait(bar, parity))
+    if (ptx::globaltimer() - t0 > 50000000ull) return;
+}
+
+}  // namespace hgemm

@@ -219,6 +219,97 @@ typedef struct {
 int hgemm_plan(int M, int N, int K, float beta, int aligned16, int force_bm, int force_bn,
                int group_m, int sm_count, int pair_slots, hgemm_plan_t *out);
 
+/* ---------------------------------------------------------------- the served attention layer
+ * Operators that run next to the projections of an attention layer: the projection itself with
+ * low-rank adapters of many requests, the norms and position rotation of its queries and keys,
+ * and the attention over packed sequences. Binary16 matrices, fp32 sums, asynchronous on
+ * `stream`, on the current device (which must hold every pointer). Everything that depends on
+ * the batch (segments, sequence starts, positions) is read on the device, so a captured call
+ * follows what its tensors hold at replay. The library keeps nothing between calls: scratch
+ * comes from the caller's `workspace` (16-byte aligned, at least the number of bytes that the
+ * matching _workspace_bytes function returns; two calls that can overlap on the GPU need one
+ * each). A NULL args pointer, a size or alignment outside the stated ranges, a NULL pointer to
+ * an operand that is read or written, or a workspace that is too small returns
+ * HGEMM_ERR_INVALID_ARG before any work. No counterpart in the reference. */
+
+/* Shared projection with low-rank adapters:
+ *   Y[t,:] = X[t,:] W + scale[a] * (X[t,:] Down[a]) Up[a],   a = seg_adapter[s], t in segment s
+ * Segment s holds the tokens seg_start[s] <= t < seg_start[s+1]; a token of no segment, or of
+ * one whose adapter is outside [0, adapters), gets X W alone. X W is summed in fp32 and the
+ * adapter's part is added before the one rounding to binary16; X Down is rounded to binary16
+ * (after the scale), as an operand of the second product, so |scale * X Down| must stay below
+ * 65504. K, N and rank are multiples of 8, 8 <= rank <= 256; matrices are row-major, contiguous
+ * and start on 16-byte boundaries. Y must not overlap the inputs. */
+typedef struct {
+  const hgemm_half_t *X;    /* tokens x K */
+  const hgemm_half_t *W;    /* K x N */
+  hgemm_half_t *Y;          /* tokens x N */
+  const hgemm_half_t *down; /* adapters x K x rank */
+  const hgemm_half_t *up;   /* adapters x rank x N */
+  const float *scale;       /* adapters */
+  const int *seg_start;     /* segments + 1, ascending */
+  const int *seg_adapter;   /* segments */
+  void *workspace;
+  size_t workspace_bytes;
+  int tokens, N, K, rank, adapters, segments;
+} hgemm_lora_t;
+int hgemm_lora(const hgemm_lora_t *args, hgemm_stream_t stream);
+/* Workspace of one call: depends on the sizes alone. 0 for sizes that hgemm_lora refuses. */
+size_t hgemm_lora_workspace_bytes(int tokens, int N, int K, int rank, int adapters, int segments);
+
+/* Root-mean-square norm of every query and key head, then the position rotation, in one pass:
+ *   n = x * rsqrt(mean(x^2) + eps) * weight                     (over head_dim, in fp32)
+ *   pair (n1, n2) i of the first rot_dim elements turns by positions[axis_of[i]][t]*inv_freq[i]:
+ *     (n1 cos - n2 sin, n2 cos + n1 sin); elements from rot_dim on are the norm alone.
+ * Pairs are (i, i + rot_dim/2), or (2i, 2i+1) when interleaved != 0. Angles are formed and
+ * reduced in fp64, so any int32 position is exact to fp32. axes > 1 gives every pair the position of one
+ * axis (time, height, width); axis_of may be NULL when axes == 1, and values above axes - 1
+ * count as axes - 1. head_dim is a multiple of 8 up to 256, rot_dim a multiple of 16 up to
+ * head_dim (0: the norm alone). Strides are halves between tokens, multiples of 8 and at least
+ * heads * head_dim; heads of a token are adjacent; every half pointer starts on a 16-byte boundary.
+ * An output is either its input (same pointer and stride) or does not overlap it. */
+typedef struct {
+  const hgemm_half_t *q, *k; /* tokens x heads_q x head_dim, tokens x heads_kv x head_dim */
+  hgemm_half_t *q_out, *k_out;
+  const hgemm_half_t *q_weight, *k_weight; /* head_dim */
+  const int *positions;                    /* axes x tokens */
+  const unsigned char *axis_of;            /* rot_dim / 2, or NULL */
+  const float *inv_freq;                   /* rot_dim / 2 */
+  long long q_stride, k_stride, q_out_stride, k_out_stride;
+  int tokens, heads_q, heads_kv, head_dim, rot_dim, axes, interleaved;
+  float eps;
+} hgemm_qk_norm_rope_t;
+int hgemm_qk_norm_rope(const hgemm_qk_norm_rope_t *args, hgemm_stream_t stream);
+
+/* Attention over packed sequences with grouped heads:
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / group]) v[j, h / group]
+ * Sequence s holds the queries cu_q[s] <= i < cu_q[s+1] and the keys cu_k[s] <= j < cu_k[s+1]
+ * (cu_k NULL: the same as cu_q). With causal != 0 the last query of a sequence sees all of its
+ * keys, the one before it all but the last, and so on (a whole prompt, one appended to earlier
+ * keys, or a single token); a query without any key gets zeros and an lse of -infinity. Queries
+ * behind cu_q[batch] are not touched. Scores, the running maximum and sum are fp32; the
+ * weights of a row, relative to its running maximum, are rounded to binary16 as an operand of the
+ * second product. lse (fp32, total_q x heads_q, natural logarithm of the row's sum) may be NULL.
+ * scale is finite and not negative; heads_q is a multiple of heads_kv, at most 128 times it; head_dim is a multiple of 8 up to 128.
+ * Strides are halves between tokens, multiples of 8 and at least heads * head_dim; heads of a
+ * token are adjacent; q, k, v and out start on 16-byte boundaries. total_q and total_k are the
+ * rows that the tensors hold; starts that point behind them are cut off there. */
+typedef struct {
+  const hgemm_half_t *q, *k, *v;
+  hgemm_half_t *out;
+  float *lse;
+  const int *cu_q, *cu_k; /* batch + 1 */
+  long long q_stride, k_stride, v_stride, out_stride;
+  void *workspace;
+  size_t workspace_bytes;
+  int total_q, total_k, batch, heads_q, heads_kv, head_dim, causal;
+  float scale;
+} hgemm_attn_prompt_t;
+int hgemm_attn_prompt(const hgemm_attn_prompt_t *args, hgemm_stream_t stream);
+/* Workspace of one call: depends on the sizes alone (0 when none is needed). */
+size_t hgemm_attn_prompt_workspace_bytes(int total_q, int total_k, int batch, int heads_q,
+                                         int heads_kv, int head_dim);
+
 /* ---------------------------------------------------------------- multi-GPU (row shards)
  * One process per GPU. Rank r owns rows [row_begin(r), row_begin(r+1)) of A and C, with
  * row_begin(r) = (M * r) / nranks; B is replicated. hgemm_sharded_rank computes the local
