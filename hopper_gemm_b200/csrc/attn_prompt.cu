@@ -19,7 +19,15 @@ struct AttnParams {
   const int *cu_q, *cu_k;
   long long q_stride, k_stride, v_stride, out_stride;
   int total_q, total_k, batch, heads_q, heads_kv, group, head_dim, causal;
-  float scale;
+  float scale2;      // scale * log2(e): scores are kept in log2 units
+  int dim16;         // head_dim rounded up to 16
+  int tile_q;        // queries of a row tile (each with the group's heads)
+  int q_box_bytes;   // bytes of one 64-element block of a tile's queries
+  int nsplit;        // key ranges of a row tile, joined by attn_join_kernel when there are several
+  float *part_o;     // nsplit x total_q x heads_q x dim16, each range's own weighted mean
+  float *part_lse;   // nsplit x total_q x heads_q, log2 of each range's sum
+  unsigned *status_word;
+  unsigned long long timeout_ns;
 };
 
 // Rows [begin, end) of sequence s, cut off at the rows that the tensor holds.
@@ -34,7 +42,6 @@ __device__ void attn_row(const AttnParams &p, const __half *qrow, const __half *
                          int j0, int j1, float (&o)[4], float &m, float &l) {
   const int e0 = 4 * (threadIdx.x & 31);
   const bool live = e0 < p.head_dim;  // head_dim is a multiple of 8
-  const float scale2 = p.scale * 1.44269504088896340736f;
   auto load4 = [&](const __half *src, float (&f)[4]) {
     uint2 u = make_uint2(0u, 0u);
     if (live) u = *reinterpret_cast<const uint2 *>(src + e0);
@@ -57,7 +64,7 @@ __device__ void attn_row(const AttnParams &p, const __half *qrow, const __half *
     float s = q[0] * kk[0] + q[1] * kk[1] + q[2] * kk[2] + q[3] * kk[3];
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= scale2;
+    s *= p.scale2;
     if (s > m) {
       const float f = exp2f(m - s);
       l *= f;
@@ -72,41 +79,526 @@ __device__ void attn_row(const AttnParams &p, const __half *qrow, const __half *
   }
 }
 
-// One warp for each (query, head).
-__global__ void __launch_bounds__(256) attn_rows_kernel(const AttnParams p) {
-  const long long row = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5;
+// ------------------------------------------------------------------------------ the kernel
+constexpr int kRows = 128;  // (query, head of the group) rows of a tile = TMEM lanes
+constexpr int kKeys = 128;  // keys of a block
+constexpr int kSmemLimit = 232448;
+// A row's weights are relative to a maximum that may lag the true one by this factor (log2): its
+// output is rescaled only when the maximum has grown past it. 2^8 times a weight below 1 stays far
+// inside binary16, and the fp32 sums do not care.
+constexpr float kLag = 8.0f;
+
+// DB: 64-element blocks of head_dim in shared memory (head_dim <= 64 DB); TILES: row tiles of a CTA,
+// each with its own four softmax warps.
+template <int DB, int TILES>
+struct AttnCfg {
+  static constexpr int TILE_BYTES = DB * kRows * 128;  // queries of a tile, or keys / values of a block
+  static constexpr int CTAS = TILES == 1 ? 2 : 1;      // per SM
+  // One warpgroup loads and issues; its registers go to the softmax warps, which hold a row of
+  // scores each (LAUNCH_REGS x the warpgroups is what the shares add up to).
+  static constexpr int THREADS = (TILES + 1) * 128;
+  static constexpr int LAUNCH_REGS = TILES == 2 ? 168 : 128;
+  static constexpr int ISSUE_REGS = 56;
+  static constexpr int SOFTMAX_REGS = TILES == 2 ? 224 : 200;
+  static_assert(TILES * SOFTMAX_REGS + ISSUE_REGS == (TILES + 1) * LAUNCH_REGS, "register shares");
+  static constexpr int BUDGET = (kSmemLimit - (CTAS - 1) * 1024) / CTAS - 1024 - 256;
+  static constexpr int STAGES_FIT = (BUDGET - TILES * TILE_BYTES) / TILE_BYTES;
+  static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
+  static constexpr int SMEM = 1024 + (TILES + STAGES) * TILE_BYTES + 256;
+  // TMEM columns: scores of each tile (the weights take the place of their first half), then the
+  // outputs.
+  static constexpr int O_COL = TILES * kKeys;
+  static constexpr int TMEM_COLS = TILES == 2 ? 512 : 256;
+  static_assert(STAGES >= 2, "a stage for keys and one for values");
+  static_assert(O_COL + TILES * DB * 64 <= TMEM_COLS, "TMEM");
+};
+
+// Sequence of tile w (tiles of `span` queries, whole sequences one after the other, longest row range
+// first inside a sequence), by one warp. Returns the sequence or -1, and the tile inside it.
+__device__ __forceinline__ int find_tile(const AttnParams &p, int w, int span, int &tile) {
   const int lane = threadIdx.x & 31;
-  if (row >= static_cast<long long>(p.total_q) * p.heads_q) return;
-  const int i = static_cast<int>(row / p.heads_q), h = static_cast<int>(row % p.heads_q);
-  int s = -1, q0 = 0, q1 = 0;
-  for (int b = 0; b < p.batch; ++b) {
-    seq_range(p.cu_q, b, p.total_q, q0, q1);
-    if (i >= q0 && i < q1) {
-      s = b;
-      break;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    int n = 0;
+    if (b0 + lane < p.batch) {
+      int q0, q1;
+      seq_range(p.cu_q, b0 + lane, p.total_q, q0, q1);
+      n = (q1 - q0 + span - 1) / span;
+    }
+    int sum = n;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, sum, x);
+      if (lane >= x) sum += y;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, w < sum);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int end = __shfl_sync(0xffffffffu, sum, src);
+      tile = end - 1 - w;
+      return b0 + src;
+    }
+    w -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return -1;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int DB, int TILES>
+__global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES>::CTAS)
+    attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                const __grid_constant__ CUtensorMap tmV, const AttnParams p) {
+  using Cfg = AttnCfg<DB, TILES>;
+  constexpr int S = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t *smem = smem_raw + (base - raw);
+  const uint32_t sQ = base, sKV = base + TILES * Cfg::TILE_BYTES;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (TILES + S) * Cfg::TILE_BYTES);
+  const uint32_t full = ptx::smem_u32(bars);          // [S] keys or values landed
+  const uint32_t empty = full + 8 * S;                // [S] the products that read them are done
+  const uint32_t qfull = empty + 8 * S;               // [1] queries landed
+  const uint32_t sfull = qfull + 8;                   // [TILES] scores ready (and the last O product done)
+  const uint32_t pfull = sfull + 8 * TILES;           // [TILES] weights ready (and O rescaled)
+  const uint32_t ofull = pfull + 8 * TILES;           // [TILES] output ready
+  int *misc = reinterpret_cast<int *>(bars + 2 * S + 1 + 3 * TILES);
+  volatile int *abort_flag = misc;
+  volatile int *found = misc + 1;  // sequence, tile
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(misc + 3);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kLoadWarp = TILES * 4, kMmaWarp = TILES * 4 + 1;
+  const int h = blockIdx.x % p.heads_kv;
+  const int split = (blockIdx.x / p.heads_kv) % p.nsplit;
+  const int w = blockIdx.x / p.heads_kv / p.nsplit;
+  const int span = TILES * p.tile_q;  // queries of this CTA
+
+  if (warp == 0) {
+    int tile = 0;
+    const int s = find_tile(p, w, span, tile);
+    if (lane == 0) {
+      found[0] = s;
+      found[1] = tile;
+      *abort_flag = 0;
+      for (int i = 0; i < S; ++i) {
+        ptx::mbar_init(full + 8 * i, 1);
+        ptx::mbar_init(empty + 8 * i, 1);
+      }
+      ptx::mbar_init(qfull, 1);
+      for (int i = 0; i < TILES; ++i) {
+        ptx::mbar_init(sfull + 8 * i, 1);
+        ptx::mbar_init(pfull + 8 * i, 4);
+        ptx::mbar_init(ofull + 8 * i, 1);
+      }
+      ptx::fence_mbar_init_cluster();
+    }
+  } else if (warp == kLoadWarp && lane == 0) {
+    ptx::prefetch_tmap(&tmQ);
+    ptx::prefetch_tmap(&tmK);
+    ptx::prefetch_tmap(&tmV);
+  }
+  __syncthreads();
+  const int s = found[0], qt = found[1];
+  if (s < 0) return;  // behind the last tile (the grid is an upper bound)
+
+  int q0, q1, k0, k1;
+  seq_range(p.cu_q, s, p.total_q, q0, q1);
+  seq_range(p.cu_k, s, p.total_k, k0, k1);
+  const int qlen = q1 - q0, klen = k1 - k0;
+  // Blocks of keys that tile i needs: [0, need_i); this CTA's share is [b0, b0 + count_i).
+  auto need_of = [&](int i) {
+    const int first = qt * span + i * p.tile_q;
+    if (first >= qlen) return 0;
+    const int last = min(first + p.tile_q, qlen) - 1;
+    const int seen = p.causal ? max(0, min(klen, last + 1 + klen - qlen)) : klen;
+    return (seen + kKeys - 1) / kKeys;
+  };
+  const int need = need_of(TILES - 1) > need_of(0) ? need_of(TILES - 1) : need_of(0);
+  const int per = (need + p.nsplit - 1) / p.nsplit;
+  const int b0 = split * per;
+  auto count_of = [&](int i) { return max(0, min(need_of(i) - b0, per)); };
+  const int count0 = count_of(0), count1 = TILES == 2 ? count_of(1) : 0;
+  const int count = max(count0, count1);
+
+  if (count > 0 && warp == kMmaWarp) {
+    ptx::tmem_alloc<1>(ptx::smem_u32(tmem_holder), Cfg::TMEM_COLS);
+    ptx::tmem_relinquish<1>();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = count > 0 ? *reinterpret_cast<volatile uint32_t *>(tmem_holder) : 0u;
+  OpWait wc{abort_flag, p.status_word, p.timeout_ns};
+
+  if (warp >= TILES * 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::ISSUE_REGS));
+    if (warp == kLoadWarp && lane == 0 && count > 0) {
+      // Both tiles' queries in one transaction (a tile without blocks is not read).
+      ptx::mbar_arrive_expect_tx(qfull, ((count0 > 0) + (count1 > 0)) * DB * p.q_box_bytes);
+      for (int i = 0; i < TILES; ++i)
+        if ((i == 0 ? count0 : count1) > 0)
+          for (int x = 0; x < DB; ++x)
+            ptx::tma_load_3d(&tmQ, sQ + i * Cfg::TILE_BYTES + x * (kRows * 128), qfull, 64 * x,
+                             h * p.group, q0 + qt * span + i * p.tile_q);
+      bool ok = true;
+      int it = 0;
+      for (; it < 2 * count; ++it) {
+        const int st = it % S;
+        if (it >= S && !op_wait(empty + 8 * st, (it / S - 1) & 1, wc, kSiteAttnKvEmpty)) {
+          ok = false;
+          break;
+        }
+        ptx::mbar_arrive_expect_tx(full + 8 * st, Cfg::TILE_BYTES);
+        const int row = k0 + (b0 + (it >> 1)) * kKeys;
+        for (int x = 0; x < DB; ++x)
+          ptx::tma_load_3d((it & 1) ? &tmV : &tmK, sKV + st * Cfg::TILE_BYTES + x * (kKeys * 128),
+                           full + 8 * st, 64 * x, h, row);
+      }
+      if (!ok) {
+        // Unwinding: the loads in flight land before the CTA may exit.
+        op_drain(qfull, 0);
+        for (int j = max(0, it - S); j < it; ++j) op_drain(full + 8 * (j % S), (j / S) & 1);
+      }
+    }
+    if (warp == kMmaWarp && lane == 0 && count > 0) {
+      const uint32_t idesc_s = ptx::umma_idesc_f16_f32(kRows, kKeys, true);
+      const uint32_t idesc_o = ptx::umma_idesc_f16_f32(kRows, p.dim16, false);
+      const int ksteps = p.dim16 / 16;
+      bool ok = op_wait(qfull, 0, wc, kSiteAttnQ);
+      auto scores = [&](int i, int stage) {
+        const uint64_t qd = ptx::umma_desc_sw128(sQ + i * Cfg::TILE_BYTES, 16, 1024);
+        const uint64_t kd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES, 16, 1024);
+        for (int k = 0; k < ksteps; ++k) {
+          // 16 elements are 32 bytes of a 128-byte row; the next 64 lie one block of 16 KB on.
+          const uint64_t off = static_cast<uint64_t>((k >> 2) * (kRows * 128 / 16) + (k & 3) * 2);
+          ptx::umma_f16<1>(tmem + i * kKeys, qd + off, kd + off, idesc_s, k > 0);
+        }
+        ptx::umma_commit<1>(sfull + 8 * i);
+      };
+      auto output = [&](int i, int stage, bool first) {
+        const uint64_t vd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES, kKeys * 128, 1024);
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+          ptx::umma_f16_ts(tmem + Cfg::O_COL + i * (DB * 64), tmem + i * kKeys + 8 * k, vd + 128 * k,
+                           idesc_o, !(first && k == 0));
+      };
+      auto cnt = [&](int i) { return i == 0 ? count0 : count1; };
+      if (ok) ok = op_wait(full, 0, wc, kSiteAttnKvFull);
+      if (ok) {
+        ptx::tc_fence_after();
+        for (int i = 0; i < TILES; ++i)
+          if (cnt(i) > 0) scores(i, 0);
+        if (S < 2 * count) ptx::umma_commit<1>(empty);
+      }
+      for (int j = 0; ok && j < count; ++j) {
+        const int vs = 2 * j + 1, ks = 2 * j + 2;
+        const int vst = vs % S, kst = ks % S;
+        if (!(ok = op_wait(full + 8 * vst, (vs / S) & 1, wc, kSiteAttnKvFull))) break;
+        bool k_here = false;
+        for (int i = 0; i < TILES; ++i) {
+          if (j >= cnt(i)) continue;
+          if (!(ok = op_wait(pfull + 8 * i, j & 1, wc, kSiteAttnWeights))) break;
+          ptx::tc_fence_after();
+          output(i, vst, j == 0);
+          if (j + 1 == cnt(i)) {
+            ptx::umma_commit<1>(ofull + 8 * i);
+          } else {
+            if (!k_here && !(ok = op_wait(full + 8 * kst, (ks / S) & 1, wc, kSiteAttnKvFull))) break;
+            k_here = true;
+            ptx::tc_fence_after();
+            // Issued behind the product that reads this tile's weights, whose columns it overwrites;
+            // the tensor core works in issue order.
+            scores(i, kst);
+          }
+        }
+        if (!ok) break;
+        // A stage that nothing is loaded into any more is not announced: no arrival outlives the CTA.
+        if (vs + S < 2 * count) ptx::umma_commit<1>(empty + 8 * vst);
+        if (ks + S < 2 * count) ptx::umma_commit<1>(empty + 8 * kst);
+      }
+      if (!ok) {
+        // Unwinding: every product retires before TMEM is freed.
+        ptx::umma_commit<1>(qfull);
+        op_drain(qfull, 1);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax warps
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::SOFTMAX_REGS));
+    const int i = warp >> 2;
+    const int row = threadIdx.x & 127;
+    const int first = qt * span + i * p.tile_q;
+    const int n = i == 0 ? count0 : count1;
+    const int qi = first + row / p.group;  // query of this row, inside the sequence
+    const bool live = row < p.tile_q * p.group && qi < qlen;
+    const int limit = p.causal ? max(0, min(klen, qi + 1 + klen - qlen)) : klen;
+    const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp, lane << 16
+    const uint32_t tS = tmem + lane_base + i * kKeys;
+    const uint32_t tO = tmem + lane_base + Cfg::O_COL + i * (DB * 64);
+    float m = -INFINITY, l = 0.0f;  // maximum that the weights are relative to (scaled), their sum
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      int okw = 1;
+      if (lane == 0) okw = op_wait(sfull + 8 * i, j & 1, wc, kSiteAttnScores);
+      ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
+      if (!ok) break;
+      ptx::tc_fence_after();
+      uint32_t sr[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(tS + 32 * c, sr[c]);
+      ptx::tmem_ld_wait();
+      const int left = limit - (b0 + j) * kKeys;  // keys of this block that the row sees
+      if (__any_sync(0xffffffffu, left < kKeys)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (32 * c + e >= left) sr[c][e] = 0xff800000u;  // -infinity
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = __uint_as_float(sr[c][0]);
+#pragma unroll
+        for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(sr[c][e]));
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2;
+      const bool grow = top > m + kLag;  // true of the first key, from -infinity
+      const float m_old = m;
+      if (grow) m = top;
+      if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        // The scores of block j were committed behind block j - 1's product, so O is at rest.
+        const float f = (grow && m_old != -INFINITY) ? ex2(m_old - m) : 1.0f;
+        l *= f;
+        for (int c = 0; c < DB * 2; ++c) {
+          uint32_t o[32];
+          ptx::tmem_ld_32x32b_x32(tO + 32 * c, o);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          ptx::tmem_st_32x32b_x32(tO + 32 * c, o);
+        }
+      }
+      const float neg = m == -INFINITY ? 0.0f : -m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 4; c += 2) {
+        uint32_t w2[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const int cc = c + (e >> 4), ee = (e & 15) * 2;
+          const float a = ex2(fmaf(__uint_as_float(sr[cc][ee]), p.scale2, neg));
+          const float b = ex2(fmaf(__uint_as_float(sr[cc][ee + 1]), p.scale2, neg));
+          sum[(e & 1) * 2] += a;
+          sum[(e & 1) * 2 + 1] += b;
+          const __half2 ab = __floats2half2_rn(a, b);
+          w2[e] = *reinterpret_cast<const uint32_t *>(&ab);
+        }
+        ptx::tmem_st_32x32b_x32(tS + 16 * c, w2);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(pfull + 8 * i);
+    }
+    if (ok && n > 0) {
+      int okw = 1;
+      if (lane == 0) okw = op_wait(ofull + 8 * i, 0, wc, kSiteAttnOut);
+      ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
+      ptx::tc_fence_after();
+    }
+    if (ok) {
+      const int kb = b0 * kKeys;                                   // first key of this CTA
+      const int ke = min(limit, kb + n * kKeys);                   // behind the last that the row sees
+      const bool any = ke > kb;
+      const long long orow =
+          static_cast<long long>(q0 + qi) * p.heads_q + h * p.group + row % p.group;
+      const float inv = any ? 1.0f / l : 0.0f;
+      bool odd = any && !(l > 0.0f && l < INFINITY);  // a sum that no finite scores give
+      uint8_t *stage = smem + i * Cfg::TILE_BYTES;
+      float *part = p.part_o + (static_cast<long long>(split) * p.total_q * p.heads_q + orow) * p.dim16;
+      for (int c = 0; c < DB * 2; ++c) {
+        uint32_t o[32];
+        if (n > 0) {
+          ptx::tmem_ld_32x32b_x32(tO + 32 * c, o);
+          ptx::tmem_ld_wait();
+        }
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          f[e] = any ? __uint_as_float(o[e]) * inv : 0.0f;
+          if (32 * c + e < p.head_dim) odd |= !(fabsf(f[e]) < INFINITY);
+        }
+        if (p.nsplit == 1) {
+          // Through the tile's own query buffer (its last product has retired), so that rows leave
+          // in whole 16-byte groups next to each other.
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint32_t u[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const __half2 ab = __floats2half2_rn(f[8 * g + 2 * x], f[8 * g + 2 * x + 1]);
+              u[x] = *reinterpret_cast<const uint32_t *>(&ab);
+            }
+            const int grp = (4 * c + g) & 7;
+            *reinterpret_cast<uint4 *>(stage + (c >> 1) * (kRows * 128) + row * 128 +
+                                       ((grp ^ (row & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+        } else if (live && any) {
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            if (32 * c + 4 * g < p.dim16)
+              *reinterpret_cast<float4 *>(part + 32 * c + 4 * g) =
+                  make_float4(f[4 * g], f[4 * g + 1], f[4 * g + 2], f[4 * g + 3]);
+        }
+      }
+      float lse2 = any ? m + log2f(l) : -INFINITY;
+      if (p.nsplit == 1) {
+        __syncwarp();
+        const int groups = p.head_dim / 8;
+        for (int x = lane; x < 32 * groups; x += 32) {
+          const int r = (row & ~31) + x / groups, grp = x % groups;
+          const int q = first + r / p.group;
+          if (r < p.tile_q * p.group && q < qlen)
+            *reinterpret_cast<uint4 *>(p.out + (q0 + q) * p.out_stride +
+                                       static_cast<long long>(h * p.group + r % p.group) * p.head_dim +
+                                       8 * grp) =
+                *reinterpret_cast<const uint4 *>(stage + (grp >> 3) * (kRows * 128) + r * 128 +
+                                                 (((grp & 7) ^ (r & 7)) << 4));
+        }
+      }
+      __syncwarp();
+      // Infinities or NaN: a masked place of the block may have reached the row (0 times infinity
+      // is NaN in the second product), or the row sees one. Done again over the keys it sees alone.
+      for (unsigned todo = __ballot_sync(0xffffffffu, live && odd); todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        const int r = (row & ~31) + src, q = first + r / p.group;
+        const int end = __shfl_sync(0xffffffffu, ke, src);
+        const int head = h * p.group + r % p.group;
+        float o[4], mr, lr;
+        attn_row(p, p.q + (q0 + q) * p.q_stride + static_cast<long long>(head) * p.head_dim,
+                 p.k + k0 * p.k_stride + static_cast<long long>(h) * p.head_dim,
+                 p.v + k0 * p.v_stride + static_cast<long long>(h) * p.head_dim, kb, end, o, mr, lr);
+        const float ir = 1.0f / lr;
+        if (4 * lane < p.head_dim) {
+          if (p.nsplit == 1) {
+            const __half2 a = __floats2half2_rn(o[0] * ir, o[1] * ir);
+            const __half2 b = __floats2half2_rn(o[2] * ir, o[3] * ir);
+            *reinterpret_cast<uint2 *>(p.out + (q0 + q) * p.out_stride +
+                                       static_cast<long long>(head) * p.head_dim + 4 * lane) =
+                make_uint2(*reinterpret_cast<const uint32_t *>(&a),
+                           *reinterpret_cast<const uint32_t *>(&b));
+          } else {
+            float *dst = p.part_o + (static_cast<long long>(split) * p.total_q * p.heads_q +
+                                     static_cast<long long>(q0 + q) * p.heads_q + head) * p.dim16;
+            *reinterpret_cast<float4 *>(dst + 4 * lane) =
+                make_float4(o[0] * ir, o[1] * ir, o[2] * ir, o[3] * ir);
+          }
+        }
+        if (lane == src) lse2 = mr + log2f(lr);
+      }
+      if (live) {
+        if (p.nsplit > 1)
+          p.part_lse[static_cast<long long>(split) * p.total_q * p.heads_q + orow] = lse2;
+        else if (p.lse)
+          p.lse[orow] = lse2 * 0.69314718055994530942f;
+      }
     }
   }
-  if (s < 0) return;
-  int k0, k1;
-  seq_range(p.cu_k, s, p.total_k, k0, k1);
-  const int klen = k1 - k0;
-  const int seen = p.causal ? max(0, min(klen, i - q0 + 1 + klen - (q1 - q0))) : klen;
-  float o[4], m, l;
-  const long long hk = static_cast<long long>(h / p.group) * p.head_dim;
-  attn_row(p, p.q + i * p.q_stride + static_cast<long long>(h) * p.head_dim,
-           p.k + k0 * p.k_stride + hk, p.v + k0 * p.v_stride + hk, 0, seen, o, m, l);
-  const float inv = seen > 0 ? 1.0f / l : 0.0f;
+  __syncthreads();
+  if (count > 0 && warp == kMmaWarp) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<1>(tmem, Cfg::TMEM_COLS);
+  }
+}
+
+// Joins the key ranges of a row: one warp for each (query, head).
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
+  const long long rows = static_cast<long long>(p.total_q) * p.heads_q;
+  const long long row = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int i = static_cast<int>(row / p.heads_q), h = static_cast<int>(row % p.heads_q);
+  // Rows of no sequence hold nothing and are left as they were.
+  int in = 0;
+  for (int b = lane; b < p.batch; b += 32) {
+    int q0, q1;
+    seq_range(p.cu_q, b, p.total_q, q0, q1);
+    in |= i >= q0 && i < q1;
+  }
+  if (!__any_sync(0xffffffffu, in)) return;
+  float top = -INFINITY;
+  for (int c = 0; c < p.nsplit; ++c) {
+    const float z = p.part_lse[c * rows + row];
+    top = z != z ? z : fmaxf(top, z);  // a NaN stays
+    if (z != z) break;
+  }
+  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
+  if (top != -INFINITY) {
+    for (int c = 0; c < p.nsplit; ++c) {
+      const float z = p.part_lse[c * rows + row];
+      if (z == -INFINITY) continue;
+      const float f = z == top ? 1.0f : exp2f(z - top);
+      l += f;
+      if (4 * lane < p.head_dim) {
+        const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (c * rows + row) * p.dim16 + 4 * lane);
+        o[0] = fmaf(f, v.x, o[0]);
+        o[1] = fmaf(f, v.y, o[1]);
+        o[2] = fmaf(f, v.z, o[2]);
+        o[3] = fmaf(f, v.w, o[3]);
+      }
+    }
+  }
+  const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
   if (4 * lane < p.head_dim) {
-    uint2 u;
     const __half2 a = __floats2half2_rn(o[0] * inv, o[1] * inv);
     const __half2 b = __floats2half2_rn(o[2] * inv, o[3] * inv);
-    u.x = *reinterpret_cast<const uint32_t *>(&a);
-    u.y = *reinterpret_cast<const uint32_t *>(&b);
     *reinterpret_cast<uint2 *>(p.out + i * p.out_stride + static_cast<long long>(h) * p.head_dim +
-                               4 * lane) = u;
+                               4 * lane) = make_uint2(*reinterpret_cast<const uint32_t *>(&a),
+                                                      *reinterpret_cast<const uint32_t *>(&b));
   }
-  if (lane == 0 && p.lse)
-    p.lse[row] = seen > 0 ? (m + log2f(l)) * 0.69314718055994530942f : -INFINITY;
+  if (lane == 0 && p.lse) p.lse[row] = (top + log2f(l)) * 0.69314718055994530942f;
+}
+
+// ------------------------------------------------------------------------------ host side
+// How a call is run: depends on the sizes alone, so that the workspace does.
+struct AttnPlan {
+  int tiles;       // row tiles of a CTA
+  int tile_q;      // queries of a row tile
+  int max_tiles;   // upper bound of the CTAs' query ranges
+  int nsplit;      // key ranges
+  size_t workspace;
+};
+
+AttnPlan make_plan(int total_q, int total_k, int batch, int heads_q, int heads_kv, int head_dim) {
+  AttnPlan pl;
+  const int group = heads_q / heads_kv;
+  pl.tile_q = kRows / group;
+  const int avg_q = (total_q + batch - 1) / batch;
+  pl.tiles = avg_q <= pl.tile_q ? 1 : 2;
+  const int span = pl.tiles * pl.tile_q;
+  pl.max_tiles = static_cast<int>(
+      std::min<long long>(total_q, total_q / span + static_cast<long long>(batch)));
+  const long long units = static_cast<long long>(pl.max_tiles) * heads_kv;
+  const int slots = 148 * (pl.tiles == 1 ? 2 : 1);
+  const int blocks = (static_cast<int>((static_cast<long long>(total_k) + batch - 1) / batch) + kKeys - 1) / kKeys;
+  pl.nsplit = 1;
+  if (units < slots) {
+    pl.nsplit = static_cast<int>(std::min<long long>((2 * slots + units - 1) / units, blocks / 4));
+    pl.nsplit = std::max(1, std::min(pl.nsplit, 64));
+  }
+  pl.workspace = 0;
+  if (pl.nsplit > 1) {
+    const size_t rows = static_cast<size_t>(pl.nsplit) * total_q * heads_q;
+    pl.workspace = rows * ((head_dim + 15) / 16 * 16) * sizeof(float) + rows * sizeof(float);
+  }
+  return pl;
 }
 
 int check(const hgemm_attn_prompt_t *a) {
@@ -129,7 +621,23 @@ int check(const hgemm_attn_prompt_t *a) {
     return HGEMM_ERR_INVALID_ARG;
   if (a->q_stride % 8 || a->out_stride % 8 || a->k_stride % 8 || a->v_stride % 8)
     return HGEMM_ERR_INVALID_ARG;
+  const size_t need = hgemm_attn_prompt_workspace_bytes(a->total_q, a->total_k, a->batch, a->heads_q,
+                                                        a->heads_kv, a->head_dim);
+  if (need > 0 && (!a->workspace || !op_aligned16(a->workspace) || a->workspace_bytes < need))
+    return HGEMM_ERR_INVALID_ARG;
   return HGEMM_OK;
+}
+
+template <int DB, int TILES>
+int launch(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const AttnParams &p,
+           const OpDevice &d, long long ctas, cudaStream_t stream) {
+  using Cfg = AttnCfg<DB, TILES>;
+  static bool done[64];
+  const int st = op_smem(reinterpret_cast<const void *>(attn_kernel<DB, TILES>), Cfg::SMEM, d.dev, done);
+  if (st != HGEMM_OK) return st;
+  attn_kernel<DB, TILES>
+      <<<static_cast<unsigned>(ctas), Cfg::THREADS, Cfg::SMEM, stream>>>(tq, tk, tv, p);
+  return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_LAUNCH;
 }
 
 int run(const hgemm_attn_prompt_t *a, cudaStream_t stream) {
@@ -158,10 +666,47 @@ int run(const hgemm_attn_prompt_t *a, cudaStream_t stream) {
   p.group = a->heads_q / a->heads_kv;
   p.head_dim = a->head_dim;
   p.causal = a->causal != 0;
-  p.scale = a->scale;
-  const long long blocks = (static_cast<long long>(a->total_q) * a->heads_q + 7) / 8;
-  if (blocks > 0x7fffffffll) return HGEMM_ERR_TOO_LARGE;
-  attn_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
+  // scale 0 is a plain mean: any tiny factor gives it without 0 times the masked -infinity.
+  p.scale2 = std::max(a->scale * 1.44269504088896340736f, 1e-37f);
+  p.dim16 = (a->head_dim + 15) / 16 * 16;
+  p.status_word = d.status_word;
+  p.timeout_ns = d.timeout_ns;
+  const AttnPlan pl = make_plan(a->total_q, a->total_k, a->batch, a->heads_q, a->heads_kv, a->head_dim);
+  p.tile_q = pl.tile_q;
+  p.q_box_bytes = pl.tile_q * p.group * 128;
+  p.nsplit = pl.nsplit;
+  p.part_o = static_cast<float *>(a->workspace);
+  p.part_lse = p.part_o + static_cast<size_t>(pl.nsplit) * a->total_q * a->heads_q * p.dim16;
+
+  CUtensorMap tq, tk, tv;
+  auto encode = [&](CUtensorMap *map, const void *ptr, int heads, int rows, long long stride,
+                    int box_heads, int box_rows) {
+    const unsigned long long dims[3] = {static_cast<unsigned long long>(a->head_dim),
+                                        static_cast<unsigned long long>(heads),
+                                        static_cast<unsigned long long>(rows)};
+    const unsigned long long strides[2] = {static_cast<unsigned long long>(a->head_dim) * 2,
+                                           static_cast<unsigned long long>(stride) * 2};
+    const unsigned box[3] = {64, static_cast<unsigned>(box_heads), static_cast<unsigned>(box_rows)};
+    return op_encode(map, ptr, 3, dims, strides, box);
+  };
+  if (!encode(&tq, a->q, a->heads_q, a->total_q, a->q_stride, p.group, pl.tile_q))
+    return HGEMM_ERR_TENSOR_MAP;
+  if (a->total_k > 0) {
+    if (!encode(&tk, a->k, a->heads_kv, a->total_k, a->k_stride, 1, kKeys) ||
+        !encode(&tv, a->v, a->heads_kv, a->total_k, a->v_stride, 1, kKeys))
+      return HGEMM_ERR_TENSOR_MAP;
+  } else {
+    tk = tv = tq;  // no key: never loaded from
+  }
+  const long long ctas = static_cast<long long>(pl.max_tiles) * a->heads_kv * pl.nsplit;
+  const long long joins = (static_cast<long long>(a->total_q) * a->heads_q + 7) / 8;
+  if (ctas > 0x7fffffffll || joins > 0x7fffffffll) return HGEMM_ERR_TOO_LARGE;
+  st = a->head_dim <= 64 ? (pl.tiles == 1 ? launch<1, 1>(tq, tk, tv, p, d, ctas, stream)
+                                          : launch<1, 2>(tq, tk, tv, p, d, ctas, stream))
+                         : (pl.tiles == 1 ? launch<2, 1>(tq, tk, tv, p, d, ctas, stream)
+                                          : launch<2, 2>(tq, tk, tv, p, d, ctas, stream));
+  if (st != HGEMM_OK || pl.nsplit == 1) return st;
+  attn_join_kernel<<<static_cast<unsigned>(joins), 256, 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_LAUNCH;
 }
 
@@ -176,8 +721,11 @@ int hgemm_attn_prompt(const hgemm_attn_prompt_t *args, hgemm_stream_t stream) {
 
 size_t hgemm_attn_prompt_workspace_bytes(int total_q, int total_k, int batch, int heads_q,
                                          int heads_kv, int head_dim) {
-  (void)total_q, (void)total_k, (void)batch, (void)heads_q, (void)heads_kv, (void)head_dim;
-  return 0;
+  if (total_q <= 0 || total_k < 0 || batch <= 0 || heads_kv < 1 || heads_q < heads_kv ||
+      heads_q % heads_kv != 0 || heads_q / heads_kv > hgemm::kRows || head_dim < 8 ||
+      head_dim > hgemm::kMaxDim || head_dim % 8 != 0)
+    return 0;
+  return hgemm::make_plan(total_q, total_k, batch, heads_q, heads_kv, head_dim).workspace;
 }
 
 }  // extern "C"
