@@ -161,6 +161,23 @@ struct PeerMaps {
   unsigned long long epoch;                   // 0: no gate (the caller orders the readers)
   int n;
 };
+// Additional k-blocks of a row tile (see LoraExt in ops_sm100.cuh), as the kernel takes them.
+struct alignas(64) ExtArgs : PeerMaps {
+  CUtensorMap tmLow;  // rows of `low`, 64 columns
+  CUtensorMap tmUp;   // N, rank, adapters
+  const int *base, *count, *adapter;
+  int chunks;
+  unsigned *odd_count;
+  unsigned long long *odd_list;
+};
+template <bool EXT>
+struct TailArgs {
+  using type = PeerMaps;
+};
+template <>
+struct TailArgs<true> {
+  using type = ExtArgs;
+};
 // C stores carry an L2 evict-first policy from this K on: with long main loops the A and B
 // tiles are re-read from L2 many times and the streamed C should not displace them
 // (8192^3: +1.4%); with short K the whole C fits in L2 and is written back after the
@@ -247,17 +264,22 @@ __device__ __forceinline__ uint32_t sw128_off(int r, int j) {
 // one clock under the power cap). The leader CTA's producer thread owns that sequence and
 // publishes every tile index through a small shared-memory ring that the other roles of
 // both CTAs read; -1 ends the sequence.
-template <int PAIR, int BN, bool TMA_EPI, int EPIW, bool SPLITK, bool PEERS>
+//
+// EXT instances walk additional k-blocks behind those of A and B: the same stages and UMMAs on
+// other tensor maps, so that the second product of low-rank adapters lands in the same fp32
+// accumulator and C is written once.
+template <int PAIR, int BN, bool TMA_EPI, int EPIW, bool SPLITK, bool PEERS, bool EXT = false>
 __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
     hgemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, const KParams p,
-                    const __grid_constant__ PeerMaps peers) {
+                    const __grid_constant__ typename TailArgs<EXT>::type peers) {
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
   using Cfg = TileCfg<PAIR, BN, EPIW>;
   // Peer copies of every tile (fused multi-GPU path) exist only in the PEERS instances: the
   // code alone cost the plain GEMM 1-6% (register pressure in the epilogue).
   const int npeer = PEERS ? peers.n : 0;
   static_assert(!SPLITK || (PAIR == 1 && TMA_EPI), "split-K: one-CTA tiles with TMA stores");
+  static_assert(!EXT || (TMA_EPI && !SPLITK && !PEERS), "additional k-blocks: plain TMA-store tiles");
   constexpr int S = Cfg::STAGES;
   constexpr int NSL = Cfg::SCHED_SLOTS;
   constexpr int ACC_BUFS = Cfg::ACC_BUFS;
@@ -408,13 +430,50 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
         decode_tile(tile, p, tm, tn);
         const int arow = tm * Cfg::UMMA_M + static_cast<int>(rank) * CTA_M;
         const int bcol = tn * BN + static_cast<int>(rank) * Cfg::SUB_COLS;
-        for (int kb = kb_begin; kb < kb_end; ++kb) {
+        int ext_base = 0, ext_blocks = 0;
+        if constexpr (EXT) {
+          ext_base = peers.base[tm];
+          ext_blocks = peers.count[tm] * peers.chunks;
+        }
+        // (the count is looked at only behind the tile's own k-blocks, so its load hides)
+        for (int kb = kb_begin; kb < kb_end || (EXT && kb < kb_end + ext_blocks); ++kb) {
           if (!wait_bar<false>(ptx::smem_u32(&empty[s]), ph ^ 1u, wctx, kSiteProducerEmpty))
             return false;
           const uint32_t fbar = full_leader0 + static_cast<uint32_t>(s) * 8u;
           if (rank == 0) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&full[s]), Cfg::TX_BYTES);
           const uint32_t dA = sA0 + static_cast<uint32_t>(s) * Cfg::A_BYTES;
           const uint32_t dB = sB0 + static_cast<uint32_t>(s) * Cfg::B_BYTES;
+          if constexpr (EXT) {
+            if (kb >= kb_end) {
+              const int x = kb - kb_end;
+              const int entry = ext_base + x / peers.chunks, chunk = x % peers.chunks;
+              const int lrow = (entry * peers.chunks + chunk) * Cfg::UMMA_M +
+                               static_cast<int>(rank) * CTA_M;
+              const int adapter = peers.adapter[entry];
+              if (PAIR == 2)
+                ptx::tma_load_2d_pair(&peers.tmLow, dA, fbar, 0, lrow);
+              else
+                ptx::tma_load_2d(&peers.tmLow, dA, fbar, 0, lrow);
+#pragma unroll
+              for (int j = 0; j < Cfg::N_SUB; ++j) {
+#pragma unroll
+                for (int b = 0; b < Cfg::SUB_BOXES; ++b) {
+                  const uint32_t dst = dB + static_cast<uint32_t>(j * Cfg::SUB_BOXES + b) * (BK * 128);
+                  const int col = bcol + j * Cfg::UMMA_N + 64 * b;
+                  if (PAIR == 2)
+                    ptx::tma_load_3d_pair(&peers.tmUp, dst, fbar, col, chunk * BK, adapter);
+                  else
+                    ptx::tma_load_3d(&peers.tmUp, dst, fbar, col, chunk * BK, adapter);
+                }
+              }
+              ++issued;
+              if (++s == S) {
+                s = 0;
+                ph ^= 1u;
+              }
+              continue;
+            }
+          }
           if (PAIR == 2)
             ptx::tma_load_2d_pair(&tmA, dA, fbar, kb * BK, arow);
           else
@@ -582,8 +641,14 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
       while (ok && tile >= 0) {
         int next = -1;
         bool have_next = false;
+        int kb_stop = kb_end;  // behind this tile's last k-block
+        if constexpr (EXT) {
+          int tm, tn;
+          decode_tile(tile, p, tm, tn);
+          kb_stop += peers.count[tm] * peers.chunks;
+        }
         auto poll_next = [&](int kb) {
-          if (!have_next && kb >= kb_end - S && sched_try_read(sslot, sph, next)) have_next = true;
+          if (!have_next && kb >= kb_stop - S && sched_try_read(sslot, sph, next)) have_next = true;
         };
         const int acc = it % ACC_BUFS;
         const uint32_t aph = static_cast<uint32_t>(it / ACC_BUFS) & 1u;
@@ -611,7 +676,7 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
             return true;
           };
           for (int kb = kb_begin; kb < main_kb && ok; ++kb) ok = kblock(kb);
-          for (int kb = main_kb; kb < kb_end && ok; ++kb) {
+          for (int kb = main_kb; kb < kb_stop && ok; ++kb) {
             ok = kblock(kb);
             poll_next(kb);
           }
@@ -650,7 +715,7 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
             return true;
           };
           const int tail_from = p.num_kb - S;  // k-blocks at or past this one are skewed
-          for (int kb = 0; kb < p.num_kb; ++kb) {
+          for (int kb = 0; kb < p.num_kb || (EXT && kb < kb_stop); ++kb) {
             if (!wait_bar<false>(ptx::smem_u32(&full[s]), ph, wctx, kSiteMmaFull)) {
               ok = false;
               break;
@@ -661,7 +726,7 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
               ptx::tc_fence_after();
               h1 = true;
             }
-            if (h1 && kb < tail_from) {
+            if (h1 && (kb < tail_from || (EXT && kb < kb_stop - S))) {
               flush();
               issue_sub(s, kb, 1);
               release_stage(s);
@@ -814,6 +879,17 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
         if (pcol < p.N) ptx::tma_prefetch_l2_2d(&tmC, pcol, prow);
       }
     };
+    // EXT: lists a 32 x 64 block with an infinity or NaN (`odd`: odd_bits of this lane's row).
+    auto note_odd = [&](uint32_t odd, int brow, int bcol) {
+      if constexpr (EXT) {
+        const bool mine = (odd & 0x80008000u) != 0 && brow + lane < p.M && bcol < p.N;
+        if (__any_sync(0xffffffffu, mine) && lane == 0)
+          peers.odd_list[atomicAdd(peers.odd_count, 1u)] =
+              static_cast<unsigned long long>(brow) | (static_cast<unsigned long long>(bcol) << 32);
+      }
+    };
+    // Bit 15 of each half is set when it is an infinity or NaN (exponent field all ones).
+    auto odd_bits = [](uint32_t w) { return (w & 0x7fff7fffu) + 0x04000400u; };
     for (;;) {
       // One lane takes the tile index and waits for the accumulator; the results are
       // broadcast so the warp stays converged for the .sync.aligned TMEM loads below.
@@ -1040,6 +1116,12 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
               ptx::fence_proxy_async_smem();
               __syncwarp();
               const int ccol = col0 + h * (BN / 2) + g * 128 + ch * EPI_COLS;
+              if constexpr (EXT) {
+                uint32_t odd = 0;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) odd |= odd_bits(P[32 * ch + j]);
+                note_odd(odd, row0, ccol);
+              }
               if (lane == 0) {
                 if (row0 < p.M && ccol < p.N) store_c(&tmC, ptx::smem_u32(stg0), ccol, row0);
                 ptx::bulk_commit_group();
@@ -1244,6 +1326,7 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
               }
             }
           }
+          uint32_t odd = 0;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             uint4 w;
@@ -1251,8 +1334,10 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
             w.y = pack_half2(f[8 * j + 2], f[8 * j + 3]);
             w.z = pack_half2(f[8 * j + 4], f[8 * j + 5]);
             w.w = pack_half2(f[8 * j + 6], f[8 * j + 7]);
+            if constexpr (EXT) odd |= odd_bits(w.x) | odd_bits(w.y) | odd_bits(w.z) | odd_bits(w.w);
             *reinterpret_cast<uint4 *>(stg + sw128_off(lane, j)) = w;
           }
+          note_odd(odd, row0, ccol);
           ptx::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -1710,6 +1795,7 @@ struct DevState {
   int cc_major = 0, cc_minor = 0;
   int pair_slots = 74;        // co-resident 2-CTA clusters at our shared-memory size
   bool attr_done[kNumTiles][kNumFlavors] = {};
+  bool ext_attr_done[kNumTiles] = {};
   void *scratch = nullptr;
   size_t scratch_bytes = 0;
   unsigned *status_word = nullptr;  // device address of g_dev_status
@@ -2276,6 +2362,131 @@ bool op_encode(CUtensorMap *map, const void *ptr, int rank, const unsigned long 
              const_cast<void *>(ptr), gdim, gstride, bx, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+namespace {
+
+using ExtKernelFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, KParams, ExtArgs);
+
+// One flavour of each tile: 8 epilogue warps for the one-accumulator 256x512 tile (wide_drain), 4
+// otherwise (adapters stand beside projections, whose K is far above the 128 where 8 pay).
+int ext_epi_warps(int tile) { return tile == kT256x512 ? 8 : 4; }
+ExtKernelFn ext_kernel_for(int tile) {
+  switch (tile) {
+    case kT256x512: return hgemm_tc_kernel<2, 512, true, 8, false, false, true>;
+    case kT256x256: return hgemm_tc_kernel<2, 256, true, 4, false, false, true>;
+    case kT256x128: return hgemm_tc_kernel<2, 128, true, 4, false, false, true>;
+    case kT128x256: return hgemm_tc_kernel<1, 256, true, 4, false, false, true>;
+    case kT128x128: return hgemm_tc_kernel<1, 128, true, 4, false, false, true>;
+    default: return hgemm_tc_kernel<1, 64, true, 4, false, false, true>;
+  }
+}
+
+int ext_plan(int M, int N, int K, const DevState &d, hgemm_plan_t *pl, int *tile) {
+  const int st = make_plan(M, N, K, 0.0f, kAllAligned, 0, 0, 0, d.sm_count, d.pair_slots, pl, false, 1);
+  if (st != HGEMM_OK) return st;
+  if (pl->path != 1 || pl->pad_a || pl->pad_b || !pl->tma_store) return HGEMM_ERR_INVALID_ARG;
+  for (int t = 0; t < kNumTiles; ++t)
+    if (kTiles[t].pair == pl->pair && kTiles[t].bn == pl->tile_n) *tile = t;
+  return HGEMM_OK;
+}
+
+}  // namespace
+
+int lora_gemm_tile_rows(int M, int N, int K, int *rows) {
+  int dev;
+  if (current_device(&dev) != HGEMM_OK) return HGEMM_ERR_CUDA;
+  std::lock_guard<std::mutex> lock(g_mu);
+  DevState *d = nullptr;
+  int st = ensure_device(dev, &d);
+  if (st != HGEMM_OK) return st;
+  hgemm_plan_t pl;
+  int tile = -1;
+  st = ext_plan(M, N, K, *d, &pl, &tile);
+  if (st == HGEMM_OK) *rows = pl.tile_m;
+  return st;
+}
+
+int lora_gemm(const __half *A, const __half *B, __half *C, int M, int N, int K, const LoraExt &ext,
+              cudaStream_t stream) {
+  int dev;
+  if (current_device(&dev) != HGEMM_OK) return HGEMM_ERR_CUDA;
+  std::lock_guard<std::mutex> lock(g_mu);
+  DevState *d = nullptr;
+  int st = ensure_device(dev, &d);
+  if (st != HGEMM_OK) return st;
+  hgemm_plan_t pl;
+  int tile = -1;
+  st = ext_plan(M, N, K, *d, &pl, &tile);
+  if (st != HGEMM_OK) return st;
+  const TileInfo &ti = kTiles[tile];
+  const FlavorInfo &fi = ti.flav[ext_epi_warps(tile) == 8 ? kFlavE8 : kFlavE4];
+  ExtKernelFn k = ext_kernel_for(tile);
+  if (!d->ext_attr_done[tile]) {
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, fi.smem) != cudaSuccess) {
+      cudaGetLastError();
+      return HGEMM_ERR_CUDA;
+    }
+    d->ext_attr_done[tile] = true;
+  }
+  CUtensorMap ta, tb, tc;
+  ExtArgs ea;
+  std::memset(static_cast<void *>(&ea), 0, sizeof(ea));
+  const int umma_n = ti.bn < 256 ? ti.bn : 256;
+  const int sub_boxes = umma_n / ti.pair / 64, n_sub = ti.bn / umma_n;
+  const bool b4 = (N % ti.bn == 0) && sub_boxes * n_sub > 1 &&
+                  encode_b4(&tb, B, K, N, N, umma_n, sub_boxes, n_sub);
+  const unsigned long long up_dims[3] = {static_cast<unsigned long long>(N),
+                                         static_cast<unsigned long long>(ext.rank),
+                                         static_cast<unsigned long long>(ext.adapters)};
+  const unsigned long long up_strides[2] = {2ull * N, 2ull * N * ext.rank};
+  const unsigned up_box[3] = {64, BK, 1};
+  if (!encode_2d(&ta, A, M, K, K, CTA_M, BK) || (!b4 && !encode_2d(&tb, B, K, N, N, BK, 64)) ||
+      !encode_2d(&tc, C, M, N, N, EPI_ROWS, EPI_COLS) ||
+      !encode_2d(&ea.tmLow, ext.low, ext.entries * ext.chunks * pl.tile_m, BK, BK, CTA_M, BK) ||
+      !op_encode(&ea.tmUp, ext.up, 3, up_dims, up_strides, up_box))
+    return HGEMM_ERR_TENSOR_MAP;
+  ea.base = ext.base;
+  ea.count = ext.count;
+  ea.adapter = ext.adapter;
+  ea.chunks = ext.chunks;
+  ea.odd_count = ext.odd_count;
+  ea.odd_list = ext.odd_list;
+  KParams kp;
+  kp.M = M;
+  kp.N = N;
+  kp.K = K;
+  kp.tiles_m = pl.tiles_m;
+  kp.tiles_n = pl.tiles_n;
+  kp.num_tiles = pl.tiles_m * pl.tiles_n;
+  kp.num_kb = ceil_div(K, BK);
+  kp.group_m = pl.group_m;
+  kp.alpha = 1.0f;
+  kp.beta = 0.0f;
+  kp.C = C;
+  kp.ldc = N;
+  kp.timeout_ns = g_timeout_ns.load();
+  kp.sched_static = pl.sched_static;
+  kp.ksplit = 1;
+  kp.b4 = b4 ? 1 : 0;
+  kp.c_evict_first = K >= kCEvictFirstMinK ? 1 : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.grid_ctas, 1, 1);
+  cfg.blockDim = dim3(fi.threads, 1, 1);
+  cfg.dynamicSmemBytes = fi.smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ti.pair == 2 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, k, ta, tb, tc, kp, ea) != cudaSuccess) {
+    cudaGetLastError();
+    return HGEMM_ERR_LAUNCH;
+  }
+  return HGEMM_OK;
 }
 
 int op_smem(const void *kernel, int smem, int dev, bool *done) {

@@ -30,6 +30,23 @@ bool op_encode(CUtensorMap *map, const void *ptr, int rank, const unsigned long 
 // and device (`done` is the caller's per-kernel array of 64 flags).
 int op_smem(const void *kernel, int smem, int dev, bool *done);
 
+// The GEMM with additional k-blocks (the second product of low-rank adapters): row tile i of C gets,
+// after the k-blocks of A and B, count[i] entries e = base[i].. of `chunks` k-blocks each, whose A
+// rows are low[e][chunk][row of the tile][64] and whose B rows are up[adapter[e]][64 chunk ..].
+// A 32 x 64 block of C that leaves with an infinity or NaN is listed (row | column << 32).
+struct LoraExt {
+  const __half *low;
+  const __half *up;       // adapters x rank x N
+  int entries, chunks, rank, adapters;
+  const int *base, *count, *adapter;
+  unsigned *odd_count;
+  unsigned long long *odd_list;
+};
+// Rows of a tile that lora_gemm uses for these sizes (128 or 256).
+int lora_gemm_tile_rows(int M, int N, int K, int *rows);
+int lora_gemm(const __half *A, const __half *B, __half *C, int M, int N, int K, const LoraExt &ext,
+              cudaStream_t stream);
+
 inline bool op_aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Wait sites of the operators' kernels in the device status word (the GEMM uses 1..12).
