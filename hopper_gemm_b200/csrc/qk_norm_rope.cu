@@ -3,13 +3,14 @@
 //   n = x * rsqrt(mean(x^2) + eps) * w;   (n1, n2) -> (n1 cos a - n2 sin a, n2 cos a + n1 sin a)
 //
 // Bound: HBM. Every half is read once and written once (4 bytes of traffic an element), against
-// about ten fp32 operations, so all that matters is wide loads in flight and no second pass: a
-// head lives in the registers of 8, 16 or 32 lanes (8 halves, one 16-byte load, each), the mean
-// square is a butterfly over those lanes and the rotation's partner element comes by a shuffle.
-// The angles of a token serve all of its heads: one thread per pair forms
-// position * inv_freq in fp64 (exact: 31 + 24 bits), reduces it to a turn fraction there and takes sincospi in
-// fp32, once per token and CTA, so a far position loses nothing and the fp64 work is 1 / heads of
-// what it would be inside the loop.
+// about ten fp32 operations, so what matters is loads in flight and few instructions beside them. A
+// head lives in the registers of 8, 16 or 32 lanes, 8 halves each: four consecutive ones and the four
+// that they turn with (half a rotation away, or next to them when pairs are adjacent), so that the
+// rotation needs no other lane and the mean square is the only exchange. Two heads of a lane group are
+// loaded while the two before them are worked on.
+// The angles of a token serve all of its heads: one thread for each pair forms position * inv_freq in
+// fp64 (exact: 31 + 24 bits), reduces it to a turn there and takes sincospi in fp32, once per
+// token and CTA, while the first heads are on their way.
 //
 // No counterpart in the reference.
 
@@ -22,52 +23,137 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHalfRot = 128;
-constexpr int kMaxTokensPerCta = 4;
+constexpr int kMaxTokensPerCta = 2;
+constexpr int kMaxHeads = 1 << 14;  // on each side: item / heads by a 32-bit multiplication is exact
 
 struct NormRopeParams {
   const __half *x[2];  // queries, keys
   __half *y[2];
   const __half *w[2];
   long long xs[2], ys[2];
+  int heads[2];
+  unsigned magic[2];  // ceil(2^32 / heads): item -> token of this CTA
   const int *positions;
   const unsigned char *axis_of;
   const float *inv_freq;
-  int tokens, heads_q, heads, head_dim, half_rot, axes;
+  int tokens, head_dim, half_rot, axes;
   float eps, inv_dim;
-  int tokens_per_cta, heads_per_cta;
+  int tokens_per_cta, parts;  // a token's heads are spread over `parts` CTAs
 };
 
-__device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-    f[2 * i] = v.x;
-    f[2 * i + 1] = v.y;
-  }
+struct Item {
+  uint2 a, b;
+  __half *y;  // null: nothing to do
+  int tt;
+};
+
+__device__ __forceinline__ float4 unpack4(const uint2 &u) {
+  const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+  return make_float4(a.x, a.y, b.x, b.y);
 }
 
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t *>(&h);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
+  const __half2 u = __floats2half2_rn(a, b), v = __floats2half2_rn(c, d);
+  return make_uint2(*reinterpret_cast<const uint32_t *>(&u), *reinterpret_cast<const uint32_t *>(&v));
 }
 
-// LANES lanes hold one head, 8 halves each (lanes behind head_dim / 8 hold zeros).
+// LANES lanes hold one head (lanes behind head_dim / 8 hold zeros).
 template <int LANES, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const NormRopeParams p) {
+__global__ void __launch_bounds__(kThreads, 4) qk_norm_rope_kernel(const NormRopeParams p) {
   constexpr int kGroups = kThreads / LANES;  // heads in flight in this CTA
-  __shared__ float s_cos[kMaxTokensPerCta][kMaxHalfRot];
-  __shared__ float s_sin[kMaxTokensPerCta][kMaxHalfRot];
+  __shared__ __align__(16) float s_cos[kMaxTokensPerCta][kMaxHalfRot];
+  __shared__ __align__(16) float s_sin[kMaxTokensPerCta][kMaxHalfRot];
 
-  const int t0 = blockIdx.x * p.tokens_per_cta;
+  const int part = blockIdx.x % p.parts;
+  const int t0 = blockIdx.x / p.parts * p.tokens_per_cta;
   const int nt = min(p.tokens_per_cta, p.tokens - t0);
+  const int sub = threadIdx.x % LANES;
+  const bool live = 8 * sub < p.head_dim;
+  // This lane's two groups of four elements, and its first angle.
+  const bool turns = INTERLEAVED ? 8 * sub < 2 * p.half_rot : 4 * sub < p.half_rot;
+  int oa = 8 * sub, ob = 8 * sub + 4;
+  if (!INTERLEAVED) {
+    // Lanes behind the rotation hold eight elements in a row: 2 half_rot + 8 (sub - half_rot / 4).
+    if (turns) {
+      oa = 4 * sub;
+      ob = p.half_rot + 4 * sub;
+    }
+  }
+  const int first = part * kGroups + static_cast<int>(threadIdx.x) / LANES;
+  const int step = kGroups * p.parts;
+
+  auto load = [&](int side, int i) {
+    Item it;
+    it.a = it.b = make_uint2(0u, 0u);
+    it.y = nullptr;
+    it.tt = 0;
+    if (live && i < nt * p.heads[side]) {
+      const int tt = static_cast<int>(__umulhi(static_cast<unsigned>(i), p.magic[side]));
+      const int tk = p.heads[side] == 1 ? i : tt;
+      const long long col = static_cast<long long>(i - tk * p.heads[side]) * p.head_dim;
+      const __half *x = p.x[side] + (t0 + tk) * p.xs[side] + col;
+      it.a = *reinterpret_cast<const uint2 *>(x + oa);
+      it.b = *reinterpret_cast<const uint2 *>(x + ob);
+      it.y = p.y[side] + (t0 + tk) * p.ys[side] + col;
+      it.tt = tk;
+    }
+    return it;
+  };
+  auto work = [&](const Item &it, const float4 &wa, const float4 &wb) {
+    float4 xa = unpack4(it.a), xb = unpack4(it.b);
+    float sq = xa.x * xa.x;
+    sq = fmaf(xa.y, xa.y, sq);
+    sq = fmaf(xa.z, xa.z, sq);
+    sq = fmaf(xa.w, xa.w, sq);
+    sq = fmaf(xb.x, xb.x, sq);
+    sq = fmaf(xb.y, xb.y, sq);
+    sq = fmaf(xb.z, xb.z, sq);
+    sq = fmaf(xb.w, xb.w, sq);
+#pragma unroll
+    for (int m = LANES / 2; m > 0; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m, LANES);
+    if (!it.y) return;
+    const float r = rsqrtf(fmaf(sq, p.inv_dim, p.eps));
+    xa.x *= wa.x * r;
+    xa.y *= wa.y * r;
+    xa.z *= wa.z * r;
+    xa.w *= wa.w * r;
+    xb.x *= wb.x * r;
+    xb.y *= wb.y * r;
+    xb.z *= wb.z * r;
+    xb.w *= wb.w * r;
+    if (turns) {
+      const float4 c = *reinterpret_cast<const float4 *>(&s_cos[it.tt][4 * sub]);
+      const float4 s = *reinterpret_cast<const float4 *>(&s_sin[it.tt][4 * sub]);
+      if (INTERLEAVED) {
+        const float4 ya = xa, yb = xb;
+        xa.x = fmaf(ya.x, c.x, -ya.y * s.x);
+        xa.y = fmaf(ya.y, c.x, ya.x * s.x);
+        xa.z = fmaf(ya.z, c.y, -ya.w * s.y);
+        xa.w = fmaf(ya.w, c.y, ya.z * s.y);
+        xb.x = fmaf(yb.x, c.z, -yb.y * s.z);
+        xb.y = fmaf(yb.y, c.z, yb.x * s.z);
+        xb.z = fmaf(yb.z, c.w, -yb.w * s.w);
+        xb.w = fmaf(yb.w, c.w, yb.z * s.w);
+      } else {
+        const float4 ya = xa;
+        xa.x = fmaf(ya.x, c.x, -xb.x * s.x);
+        xa.y = fmaf(ya.y, c.y, -xb.y * s.y);
+        xa.z = fmaf(ya.z, c.z, -xb.z * s.z);
+        xa.w = fmaf(ya.w, c.w, -xb.w * s.w);
+        xb.x = fmaf(xb.x, c.x, ya.x * s.x);
+        xb.y = fmaf(xb.y, c.y, ya.y * s.y);
+        xb.z = fmaf(xb.z, c.z, ya.z * s.z);
+        xb.w = fmaf(xb.w, c.w, ya.w * s.w);
+      }
+    }
+    *reinterpret_cast<uint2 *>(it.y + oa) = pack4(xa.x, xa.y, xa.z, xa.w);
+    *reinterpret_cast<uint2 *>(it.y + ob) = pack4(xb.x, xb.y, xb.z, xb.w);
+  };
+
+  Item next[2] = {load(0, first), load(0, first + step)};
   for (int i = threadIdx.x; i < nt * p.half_rot; i += kThreads) {
-    const int tt = i / p.half_rot, pair = i - tt * p.half_rot;
+    const int tt = i >= p.half_rot, pair = i - tt * p.half_rot;
     const int axis = p.axis_of ? min(static_cast<int>(p.axis_of[pair]), p.axes - 1) : 0;
     const int pos = p.positions[static_cast<long long>(axis) * p.tokens + t0 + tt];
     // angle / pi, reduced to [-1, 1] in fp64.
@@ -81,94 +167,37 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const NormRopePa
   }
   __syncthreads();
 
-  const int sub = threadIdx.x % LANES;
-  const int e0 = sub * 8;
-  const bool live = e0 < p.head_dim;
-  const int h0 = blockIdx.y * p.heads_per_cta;
-  const int h1 = min(h0 + p.heads_per_cta, p.heads);
-  float w[2][8] = {};
-  if (live) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      unpack8(__ldg(reinterpret_cast<const uint4 *>(p.w[j] + e0)), w[j]);
-  }
-  // The rotation of this lane's 8 elements: which angles, and (pairs half a rotation apart) the
-  // lane that holds the partners. rot_dim / 2 is a multiple of 8, so a lane's elements are all first
-  // halves, all second halves, or all behind the rotation.
-  const int rot = 2 * p.half_rot;
-  const bool turns = e0 < rot;
-  const bool second = !INTERLEAVED && turns && e0 >= p.half_rot;
-  const int partner = !turns ? sub : second ? sub - p.half_rot / 8 : sub + p.half_rot / 8;
-
-  for (int tt = 0; tt < nt; ++tt) {
-    float c[8], s[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      c[j] = 1.0f;
-      s[j] = 0.0f;
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    float4 wa = make_float4(0.0f, 0.0f, 0.0f, 0.0f), wb = wa;
+    if (live && p.heads[side] > 0) {
+      wa = unpack4(__ldg(reinterpret_cast<const uint2 *>(p.w[side] + oa)));
+      wb = unpack4(__ldg(reinterpret_cast<const uint2 *>(p.w[side] + ob)));
     }
-    if (turns) {
-      const int a0 = INTERLEAVED ? e0 / 2 : (second ? e0 - p.half_rot : e0);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int a = INTERLEAVED ? a0 + j / 2 : a0 + j;
-        c[j] = s_cos[tt][a];
-        s[j] = s_sin[tt][a];
-        // second element of a pair: n2 cos + n1 sin; first: n1 cos - n2 sin
-        const bool sec = INTERLEAVED ? (j & 1) : second;
-        if (!sec) s[j] = -s[j];
+    // Whole passes, so that every lane of a warp takes part in the exchange.
+    const int n = nt * p.heads[side];
+#pragma unroll 1
+    for (int i = first; i - first + part * kGroups < n; i += 2 * step) {
+      const Item now[2] = {next[0], next[1]};
+      const int j = i + 2 * step;
+      const bool more = j - first + part * kGroups < n;
+      const int side2 = more ? side : 1, at = more ? j : first;
+      if (more || side == 0) {
+        next[0] = load(side2, at);
+        next[1] = load(side2, at + step);
       }
+      work(now[0], wa, wb);
+      work(now[1], wa, wb);
     }
-    const long long token = t0 + tt;
-    // Whole passes, so that every lane of a warp takes part in the shuffles. Two heads of a lane
-    // group are loaded before either is used.
-    for (int hb = h0; hb < h1; hb += 2 * kGroups) {
-      uint4 raw[2];
-      int head[2];
-      bool on[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        head[u] = hb + u * kGroups + static_cast<int>(threadIdx.x) / LANES;
-        on[u] = live && head[u] < h1;
-        raw[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (on[u]) {
-          const int j = head[u] >= p.heads_q;
-          const int h = head[u] - (j ? p.heads_q : 0);
-          raw[u] = *reinterpret_cast<const uint4 *>(
-              p.x[j] + token * p.xs[j] + static_cast<long long>(h) * p.head_dim + e0);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float x[8], o[8];
-        unpack8(raw[u], x);
-        float sq = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sq = fmaf(x[j], x[j], sq);
-#pragma unroll
-        for (int m = LANES / 2; m > 0; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m, LANES);
-        const float r = rsqrtf(fmaf(sq, p.inv_dim, p.eps));
-        const int jw = head[u] >= p.heads_q;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= r * (jw ? w[1][j] : w[0][j]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float y =
-              INTERLEAVED ? x[j ^ 1] : __shfl_sync(0xffffffffu, x[j], partner, LANES);
-          o[j] = fmaf(x[j], c[j], y * s[j]);
-        }
-        if (on[u]) {
-          const int h = head[u] - (jw ? p.heads_q : 0);
-          *reinterpret_cast<uint4 *>(p.y[jw] + token * p.ys[jw] +
-                                     static_cast<long long>(h) * p.head_dim + e0) = pack8(o);
-        }
-      }
+    if (side == 0 && part * kGroups >= n) {
+      next[0] = load(1, first);  // no queries here: the keys were not yet asked for
+      next[1] = load(1, first + step);
     }
   }
 }
 
 template <int LANES>
-void launch(const NormRopeParams &p, bool interleaved, dim3 grid, cudaStream_t stream) {
+void launch(const NormRopeParams &p, bool interleaved, unsigned grid, cudaStream_t stream) {
   if (interleaved)
     qk_norm_rope_kernel<LANES, true><<<grid, kThreads, 0, stream>>>(p);
   else
@@ -182,7 +211,7 @@ int check(const hgemm_qk_norm_rope_t *a) {
     return HGEMM_ERR_INVALID_ARG;
   if (a->axes < 1 || (a->axes > 1 && a->rot_dim > 0 && !a->axis_of)) return HGEMM_ERR_INVALID_ARG;
   if (!(a->eps >= 0.0f)) return HGEMM_ERR_INVALID_ARG;
-  if (static_cast<long long>(a->heads_q) + a->heads_kv > (1 << 20)) return HGEMM_ERR_TOO_LARGE;
+  if (a->heads_q > kMaxHeads || a->heads_kv > kMaxHeads) return HGEMM_ERR_TOO_LARGE;
   if (a->tokens == 0 || a->heads_q + a->heads_kv == 0) return HGEMM_OK;
   if (a->rot_dim > 0 && (!a->positions || !a->inv_freq)) return HGEMM_ERR_INVALID_ARG;
   auto operand = [&](const void *in, const void *out, const void *w, long long is, long long os,
@@ -209,33 +238,36 @@ int run(const hgemm_qk_norm_rope_t *a, cudaStream_t stream) {
   p.x[1] = a->k;
   p.y[0] = a->q_out;
   p.y[1] = a->k_out;
-  // A side without heads is never indexed by a head, but its weights are loaded.
-  p.w[0] = a->heads_q ? a->q_weight : a->k_weight;
-  p.w[1] = a->heads_kv ? a->k_weight : a->q_weight;
+  p.w[0] = a->q_weight;
+  p.w[1] = a->k_weight;
   p.xs[0] = a->q_stride;
   p.xs[1] = a->k_stride;
   p.ys[0] = a->q_out_stride;
   p.ys[1] = a->k_out_stride;
+  p.heads[0] = a->heads_q;
+  p.heads[1] = a->heads_kv;
+  for (int j = 0; j < 2; ++j)
+    p.magic[j] = p.heads[j] > 1 ? static_cast<unsigned>((0x100000000ull + p.heads[j] - 1) / p.heads[j]) : 0u;
   p.positions = a->positions;
   p.axis_of = a->axes > 1 ? a->axis_of : nullptr;
   p.inv_freq = a->inv_freq;
   p.tokens = a->tokens;
-  p.heads_q = a->heads_q;
-  p.heads = a->heads_q + a->heads_kv;
   p.head_dim = a->head_dim;
   p.half_rot = a->rot_dim / 2;
   p.axes = a->axes;
   p.eps = a->eps;
   p.inv_dim = 1.0f / static_cast<float>(a->head_dim);
   const int lanes = a->head_dim <= 64 ? 8 : a->head_dim <= 128 ? 16 : 32;
-  const int groups = 2 * kThreads / lanes;
-  // A CTA takes whole tokens where there are enough of them to fill the SMs, so that one set of
-  // angles serves all heads; with few tokens the heads of one are spread over CTAs (one pass each).
-  p.tokens_per_cta =
-      std::max(1, std::min(kMaxTokensPerCta, a->tokens / std::max(1, 8 * d.sm_count)));
-  p.heads_per_cta = a->tokens >= 2 * d.sm_count ? p.heads : std::min(p.heads, groups);
-  const dim3 grid((a->tokens + p.tokens_per_cta - 1) / p.tokens_per_cta,
-                  (p.heads + p.heads_per_cta - 1) / p.heads_per_cta);
+  const int groups = kThreads / lanes;
+  // Two tokens to a CTA where that still fills the SMs several times over; with few tokens the heads
+  // of one are spread over CTAs (one head to a lane group).
+  p.tokens_per_cta = a->tokens >= 16 * d.sm_count ? 2 : 1;
+  const int most = std::max(a->heads_q, a->heads_kv);
+  p.parts = a->tokens >= 2 * d.sm_count ? 1 : (most + groups - 1) / groups;
+  const long long ctas =
+      static_cast<long long>((a->tokens + p.tokens_per_cta - 1) / p.tokens_per_cta) * p.parts;
+  if (ctas > 0x7fffffffll) return HGEMM_ERR_TOO_LARGE;
+  const unsigned grid = static_cast<unsigned>(ctas);
   if (lanes == 8)
     launch<8>(p, a->interleaved != 0, grid, stream);
   else if (lanes == 16)
