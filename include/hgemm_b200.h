@@ -265,7 +265,7 @@ size_t hgemm_lora_workspace_bytes(int tokens, int N, int K, int rank, int adapte
  * reduced in fp64, so any int32 position is exact to fp32. axes > 1 gives every pair the position of one
  * axis (time, height, width); axis_of may be NULL when axes == 1, and values above axes - 1
  * count as axes - 1. head_dim is a multiple of 8 up to 256, rot_dim a multiple of 16 up to
- * head_dim (0: the norm alone), at most 16384 heads on a side (HGEMM_ERR_TOO_LARGE). Strides are halves between tokens, multiples of 8 and at least
+ * head_dim (0: the norm alone), at most 2^20 heads on a side (HGEMM_ERR_TOO_LARGE). Strides are halves between tokens, multiples of 8 and at least
  * heads * head_dim; heads of a token are adjacent; every half pointer starts on a 16-byte boundary.
  * An output is either its input (same pointer and stride) or does not overlap it. */
 typedef struct {
