@@ -60,8 +60,6 @@ enum OpWaitSite : unsigned {
   kSiteLoraEmpty = 40,
   kSiteLoraFull = 41,
   kSiteLoraAcc = 42,
-  kSiteNormFull = 43,
-  kSiteNormEmpty = 44,
   kSiteOpDrain = 63,
 };
 

@@ -181,15 +181,6 @@ __device__ __forceinline__ void prefetch_tmap(const CUtensorMap *m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
 }
 
-// Untiled copy of `bytes` (a multiple of 16, both ends 16-byte aligned) into this CTA's shared memory.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
 // 2-D tiled load into this CTA's shared memory, completion counted on `bar` (this CTA).
 __device__ __forceinline__ void tma_load_2d(const CUtensorMap *m, uint32_t dst, uint32_t bar,
                                             int32_t c0, int32_t c1) {

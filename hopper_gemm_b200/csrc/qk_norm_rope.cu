@@ -3,18 +3,19 @@
 //   n = x * rsqrt(mean(x^2) + eps) * w;   (n1, n2) -> (n1 cos a - n2 sin a, n2 cos a + n1 sin a)
 //
 // Bound: HBM. Every half is read once and written once (4 bytes of traffic an element), against
-// about ten fp32 operations. Loads through registers held too few bytes in flight (two heads to a
-// lane group: 37 us for 8191 tokens of 40 heads of 128), so the heads of a token, which are adjacent,
-// come by bulk copies into a ring of slots, issued by a warp of their own; the other warps pass
-// over the slots each at its own pace, and results leave with 16-byte stores. A CTA takes a range of
-// tokens, all CTAs the same number to within one.
-// A head then lives in the registers of few lanes, 16 halves each: eight consecutive ones and the
-// eight that they turn with (half a rotation away, or next to them when pairs are adjacent), so that the
-// rotation needs no other lane and the mean square is the only exchange.
-// The angles of a token serve all of its heads: one lane for each pair forms position * inv_freq in
-// fp64 (exact: 31 + 24 bits), reduces it to a turn there and takes sincospi in fp32. The copying warp
-// does that while the copies are under way, so that a slot is full with its angles and the other
-// warps never meet (formed by all of them behind a barrier, they cost 10 us of the 38).
+// about ten fp32 operations, so what matters is loads in flight and few instructions beside them.
+// Norm weight and rotation are one: element e becomes r (x_e A_e + x_partner B_e), with A and B (weight
+// times cos, weight times sin) formed once for a token and side, and two elements go into an
+// instruction (fma.rn.f32x2). A warp takes a token: its lane groups of a few lanes hold a head each, 16
+// halves a lane: eight consecutive ones and the eight that they turn with (half a rotation away, or
+// next to them when pairs are adjacent), so that the rotation needs no other lane, the mean square is
+// the only exchange, and A and B stay in registers over all heads of a side. The heads of the next two
+// passes are on their way while one is worked on.
+// The angles: one lane for each pair forms position * inv_freq in fp64 (exact: 31 + 24 bits), reduces it
+// to a turn there and takes sincospi in fp32, while the token's first heads are loaded.
+// Forms in which a CTA's warps shared a token (through registers, or a ring of bulk copies) took 37 us
+// for 8191 tokens of 40 heads of 128: A and B came from shared memory for every head, whose bandwidth
+// was then the bound.
 //
 // No counterpart in the reference.
 
@@ -25,11 +26,8 @@
 namespace hgemm {
 namespace {
 
-constexpr int kThreads = 256;  // that pass over the heads; one more warp fills the slots
-constexpr int kCtasPerSm = 4;
-constexpr int kSlots = 4;
-constexpr int kMaxHalfRot = 128;
-constexpr int kMaxSlotBytes = 10752;  // kCtasPerSm rings fit an SM
+constexpr int kWarps = 4;  // of a CTA
+constexpr int kCtasPerSm = 5;
 constexpr int kMaxHeads = 1 << 20;
 
 struct NormRopeParams {
@@ -40,227 +38,186 @@ struct NormRopeParams {
   const int *positions;
   const unsigned char *axis_of;
   const float *inv_freq;
-  int tokens, heads_q, heads, head_dim, half_rot, axes;
+  int tokens, heads[2], head_dim, half_rot, axes;
   float eps, inv_dim;
-  // A CTA takes `part_heads` adjacent heads (queries, then keys) of each of its tokens.
-  int part_heads, parts, slot_bytes;
-  unsigned *status_word;
-  unsigned long long timeout_ns;
+  // A warp passes over the heads in steps of one head to a lane group: `passes[0]` over the queries,
+  // then those over the keys. A token's passes are shared by `parts` warps.
+  int passes[2], parts;
 };
 
-__device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
+__device__ __forceinline__ void unpack8(const uint4 &u, float2 (&f)[4]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-    f[2 * i] = v.x;
-    f[2 * i + 1] = v.y;
-  }
+  for (int i = 0; i < 4; ++i) f[i] = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
 }
 
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+__device__ __forceinline__ uint4 pack8(const float2 (&f)[4]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    const __half2 h = __float22half2_rn(f[i]);
     w[i] = *reinterpret_cast<const uint32_t *>(&h);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ void load8(const float *src, float (&f)[8]) {
+// r (x A + y B) for eight elements x with their partners y.
+__device__ __forceinline__ uint4 turn8(const float2 (&x)[4], const float2 (&y)[4],
+                                       const float2 (&A)[4], const float2 (&B)[4], float2 r) {
+  float2 o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    o[i] = __fmul2_rn(__ffma2_rn(x[i], A[i], __fmul2_rn(y[i], B[i])), r);
+  return pack8(o);
+}
+
+__device__ __forceinline__ void load8(const float *src, float2 (&f)[4]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const float4 v = reinterpret_cast<const float4 *>(src)[h];
-    f[4 * h] = v.x;
-    f[4 * h + 1] = v.y;
-    f[4 * h + 2] = v.z;
-    f[4 * h + 3] = v.w;
+    f[2 * h] = make_float2(v.x, v.y);
+    f[2 * h + 1] = make_float2(v.z, v.w);
   }
 }
 
 // LANES lanes hold one head (groups of eight behind head_dim hold zeros).
 template <int LANES, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads + 32, kCtasPerSm)
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     qk_norm_rope_kernel(const NormRopeParams p) {
-  constexpr int kGroups = kThreads / LANES;  // heads in flight in this CTA
-  extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ __align__(16) float s_cos[kSlots][kMaxHalfRot];
-  __shared__ __align__(16) float s_sin[kSlots][kMaxHalfRot];
-  __shared__ __align__(16) float s_w[2][256];
-  __shared__ __align__(8) uint64_t s_full[kSlots], s_empty[kSlots];
-  __shared__ int s_abort;
+  constexpr int kGroups = 32 / LANES;  // heads of a pass
+  constexpr int kDim = LANES * 16;     // head_dim is at most this
+  __shared__ float s_w[2][kDim];
+  // A of the queries, B, A of the keys, B of this warp's token.
+  __shared__ __align__(16) float s_tab[kWarps][2][2][kDim];
 
-  const int part = blockIdx.x % p.parts, cta = blockIdx.x / p.parts, ctas = gridDim.x / p.parts;
-  const int t0 = static_cast<int>(static_cast<long long>(p.tokens) * cta / ctas);
-  const int t1 = static_cast<int>(static_cast<long long>(p.tokens) * (cta + 1) / ctas);
-  const int h0 = part * p.part_heads, n = min(p.part_heads, p.heads - h0);
-  if (threadIdx.x == 0) {
-    s_abort = 0;
-    for (int i = 0; i < kSlots; ++i) {
-      ptx::mbar_init(ptx::smem_u32(&s_full[i]), 2);  // the copies; the angles
-      ptx::mbar_init(ptx::smem_u32(&s_empty[i]), kThreads / 32);
-    }
-    ptx::fence_mbar_init_cluster();
-  }
-  for (int i = threadIdx.x; i < 2 * 256; i += kThreads + 32) {
-    const int j = i >> 8, e = i & 255;
-    s_w[j][e] = p.w[j] && e < p.head_dim ? __half2float(p.w[j][e]) : 0.0f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < 2 * kDim; i += kWarps * 32) {
+    const int j = i / kDim, e = i % kDim;
+    const float w = p.heads[j] > 0 && e < p.head_dim ? __half2float(p.w[j][e]) : 0.0f;
+    s_w[j][e] = w;
+    if (e >= 2 * p.half_rot)  // behind the rotation: the weight alone, for every token
+      for (int x = 0; x < kWarps; ++x) {
+        s_tab[x][j][0][e] = w;
+        s_tab[x][j][1][e] = 0.0f;
+      }
   }
   __syncthreads();
-  const OpWait wc{&s_abort, p.status_word, p.timeout_ns};
-  const int lane = threadIdx.x & 31;
 
-  if (threadIdx.x >= kThreads) {
-    // ---------------------------------------------------------------- copies and angles
-    // This part's queries, its keys, or some of both.
-    const int split = min(max(p.heads_q, h0), h0 + n);
-    const int qbytes = (split - h0) * p.head_dim * 2, kbytes = (h0 + n - split) * p.head_dim * 2;
-    const __half *q = p.x[0] + t0 * p.xs[0] + static_cast<long long>(h0) * p.head_dim;
-    const __half *k = p.x[1] + t0 * p.xs[1] + static_cast<long long>(split - p.heads_q) * p.head_dim;
-    constexpr int kPairs = kMaxHalfRot / 32;  // of a lane: lane, lane + 32, ..
-    const int *place[kPairs];                 // positions of the pair's axis
-    double freq[kPairs];                      // inv_freq / pi
-    int pos[kPairs];
-#pragma unroll
-    for (int j = 0; j < kPairs; ++j) {
-      const int pair = lane + 32 * j;
-      if (pair >= p.half_rot) continue;
-      const int axis = p.axis_of ? min(static_cast<int>(p.axis_of[pair]), p.axes - 1) : 0;
-      place[j] = p.positions + static_cast<long long>(axis) * p.tokens + t0;
-      freq[j] = static_cast<double>(p.inv_freq[pair]);
-      pos[j] = place[j][0];
-    }
-    int i = 0;
-    bool ok = true;
-    for (; i < t1 - t0; ++i) {
-      const int slot = i % kSlots;
-      const uint32_t bar = ptx::smem_u32(&s_full[slot]);
-      int okw = 1;
-      if (lane == 0) {
-        if (i >= kSlots)
-          okw = op_wait(ptx::smem_u32(&s_empty[slot]), (i / kSlots - 1) & 1, wc, kSiteNormEmpty);
-        if (okw) {
-          const uint32_t dst = ptx::smem_u32(ring) + slot * p.slot_bytes;
-          ptx::mbar_arrive_expect_tx(bar, qbytes + kbytes);
-          if (qbytes) ptx::bulk_load(dst, q + i * p.xs[0], qbytes, bar);
-          if (kbytes) ptx::bulk_load(dst + qbytes, k + i * p.xs[1], kbytes, bar);
-        }
-      }
-      ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
-      if (!ok) break;
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        const int pair = lane + 32 * j;
-        if (pair >= p.half_rot) continue;
-        // angle / pi, reduced to [-1, 1] in fp64.
-        const double half_turns = static_cast<double>(pos[j]) * freq[j] * 0.31830988618379067154;
-        if (i + 1 < t1 - t0) pos[j] = place[j][i + 1];
-        const double r = half_turns - 2.0 * rint(half_turns * 0.5);
-        float s, c;
-        sincospif(static_cast<float>(r), &s, &c);
-        s_cos[slot][pair] = c;
-        s_sin[slot][pair] = s;
-      }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar);
-    }
-    if (!ok && lane == 0)  // unwinding: the copies in flight land before the CTA may exit
-      for (int j = max(0, i - kSlots); j < i; ++j)
-        op_drain(ptx::smem_u32(&s_full[j % kSlots]), (j / kSlots) & 1);
-    return;
-  }
-
-  // ------------------------------------------------------------------ norms and rotation
-  const int sub = threadIdx.x % LANES;
+  const int sub = lane % LANES;
   // This lane's two groups of eight: elements oa.. and ob.. .
-  const bool turns = (INTERLEAVED ? 16 : 8) * sub < (INTERLEAVED ? 2 : 1) * p.half_rot;
   int oa = 16 * sub;  // (behind the rotation: 2 half_rot + 16 (sub - half_rot / 8))
   int ob = oa + 8;
-  if (!INTERLEAVED && turns) {
+  if (!INTERLEAVED && 8 * sub < p.half_rot) {
     oa = 8 * sub;
     ob = p.half_rot + 8 * sub;
   }
   const bool live_a = oa < p.head_dim, live_b = ob < p.head_dim;
+  const int gw = blockIdx.x * kWarps + warp, warps = gridDim.x * kWarps;
+  const int part = gw % p.parts;
+  const int all = p.passes[0] + p.passes[1];
+  const int p0 = static_cast<int>(static_cast<long long>(all) * part / p.parts);
+  const int p1 = static_cast<int>(static_cast<long long>(all) * (part + 1) / p.parts);
 
+  // Heads [begin, end) of each side are this warp's; its lane groups take them in turn.
+  const int group = lane / LANES;
+  const int bq = min(p0, p.passes[0]) * kGroups, eq = min(p.heads[0], p1 * kGroups);
+  const int bk = max(p0 - p.passes[0], 0) * kGroups;
+  const int ek = min(p.heads[1], (p1 - p.passes[0]) * kGroups);
+  const int step = kGroups * p.head_dim;
+  // Offsets inside a token's row: heads of a token stay below 2^28 halves.
+  const int cq = (bq + group) * p.head_dim, ck = (bk + group) * p.head_dim;
+
+  auto load = [&](const __half *x, bool on, uint4 &a, uint4 &b) {
+    a = b = make_uint4(0u, 0u, 0u, 0u);
+    if (on && live_a) a = *reinterpret_cast<const uint4 *>(x + oa);
+    if (on && live_b) b = *reinterpret_cast<const uint4 *>(x + ob);
+  };
+  // The heads of one side, the first two passes of which are in (a0, b0) and (a1, b1).
+  auto walk = [&](int side, const __half *x, __half *y, int begin, int end, uint4 a0, uint4 b0,
+                  uint4 a1, uint4 b1) {
+    float2 Aa[4], Ba[4], Ab[4], Bb[4];
+    load8(&s_tab[warp][side][0][oa], Aa);
+    load8(&s_tab[warp][side][1][oa], Ba);
+    load8(&s_tab[warp][side][0][ob], Ab);
+    load8(&s_tab[warp][side][1][ob], Bb);
+    x += 2 * step;
 #pragma unroll 1
-  for (int t = t0; t < t1; ++t) {
-    const int k = t - t0, slot = k % kSlots;
-    // (a wait that ran out leaves the slot's contents unspecified; the status word tells)
-    op_wait(ptx::smem_u32(&s_full[slot]), (k / kSlots) & 1, wc, kSiteNormFull);
-    const __half *stage = reinterpret_cast<const __half *>(ring + slot * p.slot_bytes);
-    // Whole warps, so that every lane takes part in the exchange.
-#pragma unroll 1
-    for (int i = static_cast<int>(threadIdx.x) / LANES; i - lane / LANES < n; i += kGroups) {
-      const bool on = i < n;
-      uint4 ra = make_uint4(0u, 0u, 0u, 0u), rb = ra;
-      if (on && live_a) ra = *reinterpret_cast<const uint4 *>(stage + i * p.head_dim + oa);
-      if (on && live_b) rb = *reinterpret_cast<const uint4 *>(stage + i * p.head_dim + ob);
-      float xa[8], xb[8];
+    for (int left = end - begin - group; left + group > 0; left -= kGroups) {
+      const uint4 ra = a0, rb = b0;
+      a0 = a1;
+      b0 = b1;
+      load(x, left > 2 * kGroups, a1, b1);
+      x += step;
+      float2 xa[4], xb[4];
       unpack8(ra, xa);
       unpack8(rb, xb);
-      float sa = 0.0f, sb = 0.0f;
+      float2 sa = __fmul2_rn(xa[0], xa[0]), sb = __fmul2_rn(xb[0], xb[0]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        sa = fmaf(xa[e], xa[e], sa);
-        sb = fmaf(xb[e], xb[e], sb);
+      for (int e = 1; e < 4; ++e) {
+        sa = __ffma2_rn(xa[e], xa[e], sa);
+        sb = __ffma2_rn(xb[e], xb[e], sb);
       }
-      float sq = sa + sb;
+      sa = __fadd2_rn(sa, sb);
+      float sq = sa.x + sa.y;
 #pragma unroll
       for (int m = LANES / 2; m > 0; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m, LANES);
-      if (!on) continue;
-      const int head = h0 + i, side = head >= p.heads_q;
-      const float r = rsqrtf(fmaf(sq, p.inv_dim, p.eps));
-      float wa[8], wb[8];
-      load8(&s_w[side][oa], wa);
-      load8(&s_w[side][ob], wb);
+      const float r1 = rsqrtf(fmaf(sq, p.inv_dim, p.eps));
+      const float2 r = make_float2(r1, r1);
+      float2 ya[4], yb[4];  // partners
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        xa[e] *= wa[e] * r;
-        xb[e] *= wb[e] * r;
+      for (int e = 0; e < 4; ++e) {
+        ya[e] = INTERLEAVED ? make_float2(xa[e].y, xa[e].x) : xb[e];
+        yb[e] = INTERLEAVED ? make_float2(xb[e].y, xb[e].x) : xa[e];
       }
-      if (turns) {
-        float c[8], s[8];
-        load8(&s_cos[slot][8 * sub], c);
-        load8(&s_sin[slot][8 * sub], s);
-        if (INTERLEAVED) {
+      if (left > 0 && live_a) *reinterpret_cast<uint4 *>(y + oa) = turn8(xa, ya, Aa, Ba, r);
+      if (left > 0 && live_b) *reinterpret_cast<uint4 *>(y + ob) = turn8(xb, yb, Ab, Bb, r);
+      y += step;
+    }
+  };
+
+#pragma unroll 1
+  for (int t = gw / p.parts; t < p.tokens; t += warps / p.parts) {
+    const __half *xq = p.x[0] + t * p.xs[0] + cq, *xk = p.x[1] + t * p.xs[1] + ck;
+    uint4 a0, b0, a1, b1;
+    load(xq, bq + group < eq, a0, b0);
+    load(xq + step, bq + kGroups + group < eq, a1, b1);
+    __syncwarp();  // the tables of the token before have been read
+    for (int pair = lane; pair < p.half_rot; pair += 32) {
+      const int axis = p.axis_of ? min(static_cast<int>(p.axis_of[pair]), p.axes - 1) : 0;
+      const int pos = p.positions[static_cast<long long>(axis) * p.tokens + t];
+      // angle / pi, reduced to [-1, 1] in fp64.
+      const double half_turns = static_cast<double>(pos) *
+                                static_cast<double>(p.inv_freq[pair]) * 0.31830988618379067154;
+      const double r = half_turns - 2.0 * rint(half_turns * 0.5);
+      float s, c;
+      sincospif(static_cast<float>(r), &s, &c);
+      const int e1 = INTERLEAVED ? 2 * pair : pair;
+      const int e2 = INTERLEAVED ? 2 * pair + 1 : pair + p.half_rot;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float a0 = xa[2 * e], b0 = xb[2 * e];
-            xa[2 * e] = fmaf(a0, c[e], -xa[2 * e + 1] * s[e]);
-            xa[2 * e + 1] = fmaf(xa[2 * e + 1], c[e], a0 * s[e]);
-            xb[2 * e] = fmaf(b0, c[4 + e], -xb[2 * e + 1] * s[4 + e]);
-            xb[2 * e + 1] = fmaf(xb[2 * e + 1], c[4 + e], b0 * s[4 + e]);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float a0 = xa[e];
-            xa[e] = fmaf(a0, c[e], -xb[e] * s[e]);
-            xb[e] = fmaf(xb[e], c[e], a0 * s[e]);
-          }
-        }
+      for (int j = 0; j < 2; ++j) {
+        const float w1 = s_w[j][e1], w2 = s_w[j][e2];
+        s_tab[warp][j][0][e1] = w1 * c;
+        s_tab[warp][j][0][e2] = w2 * c;
+        s_tab[warp][j][1][e1] = -w2 * s;
+        s_tab[warp][j][1][e2] = w1 * s;
       }
-      __half *y = (side ? p.y[1] + t * p.ys[1] : p.y[0] + t * p.ys[0]) +
-                  static_cast<long long>(head - (side ? p.heads_q : 0)) * p.head_dim;
-      if (live_a) *reinterpret_cast<uint4 *>(y + oa) = pack8(xa);
-      if (live_b) *reinterpret_cast<uint4 *>(y + ob) = pack8(xb);
     }
     __syncwarp();
-    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s_empty[slot]));
+    if (eq > bq) walk(0, xq, p.y[0] + t * p.ys[0] + cq, bq, eq, a0, b0, a1, b1);
+    if (ek > bk) {
+      load(xk, bk + group < ek, a0, b0);
+      load(xk + step, bk + kGroups + group < ek, a1, b1);
+      walk(1, xk, p.y[1] + t * p.ys[1] + ck, bk, ek, a0, b0, a1, b1);
+    }
   }
 }
 
 template <int LANES>
-int launch(const NormRopeParams &p, bool interleaved, unsigned grid, int dev, cudaStream_t stream) {
-  const auto kernel =
-      interleaved ? qk_norm_rope_kernel<LANES, true> : qk_norm_rope_kernel<LANES, false>;
-  static bool done[2][64];
-  const int st = op_smem(reinterpret_cast<const void *>(kernel), kSlots * kMaxSlotBytes, dev,
-                         done[interleaved]);
-  if (st != HGEMM_OK) return st;
-  kernel<<<grid, kThreads + 32, kSlots * p.slot_bytes, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_LAUNCH;
+void launch(const NormRopeParams &p, bool interleaved, unsigned grid, cudaStream_t stream) {
+  if (interleaved)
+    qk_norm_rope_kernel<LANES, true><<<grid, kWarps * 32, 0, stream>>>(p);
+  else
+    qk_norm_rope_kernel<LANES, false><<<grid, kWarps * 32, 0, stream>>>(p);
 }
 
 int check(const hgemm_qk_norm_rope_t *a) {
@@ -297,8 +254,8 @@ int run(const hgemm_qk_norm_rope_t *a, cudaStream_t stream) {
   p.x[1] = a->k;
   p.y[0] = a->q_out;
   p.y[1] = a->k_out;
-  p.w[0] = a->heads_q ? a->q_weight : nullptr;
-  p.w[1] = a->heads_kv ? a->k_weight : nullptr;
+  p.w[0] = a->q_weight;
+  p.w[1] = a->k_weight;
   p.xs[0] = a->q_stride;
   p.xs[1] = a->k_stride;
   p.ys[0] = a->q_out_stride;
@@ -307,29 +264,31 @@ int run(const hgemm_qk_norm_rope_t *a, cudaStream_t stream) {
   p.axis_of = a->axes > 1 ? a->axis_of : nullptr;
   p.inv_freq = a->inv_freq;
   p.tokens = a->tokens;
-  p.heads_q = a->heads_q;
-  p.heads = a->heads_q + a->heads_kv;
+  p.heads[0] = a->heads_q;
+  p.heads[1] = a->heads_kv;
   p.head_dim = a->head_dim;
   p.half_rot = a->rot_dim / 2;
   p.axes = a->axes;
   p.eps = a->eps;
   p.inv_dim = 1.0f / static_cast<float>(a->head_dim);
-  p.status_word = d.status_word;
-  p.timeout_ns = d.timeout_ns;
   const int lanes = a->head_dim <= 64 ? 4 : a->head_dim <= 128 ? 8 : 16;
-  const int slots = kCtasPerSm * d.sm_count;
-  // All heads of a token in one CTA as far as a slot holds them; with fewer tokens than CTAs, one
-  // head to a lane group, so that a token's heads are spread over CTAs.
-  p.part_heads = std::min(p.heads, kMaxSlotBytes / (2 * a->head_dim));
-  if (a->tokens < slots) p.part_heads = std::min(p.part_heads, kThreads / lanes);
-  p.parts = (p.heads + p.part_heads - 1) / p.part_heads;
-  p.slot_bytes = (p.part_heads * a->head_dim * 2 + 127) / 128 * 128;
-  const unsigned grid =
-      static_cast<unsigned>(std::min(a->tokens, std::max(1, slots / p.parts)) * p.parts);
+  const int groups = 32 / lanes;
+  p.passes[0] = (a->heads_q + groups - 1) / groups;
+  p.passes[1] = (a->heads_kv + groups - 1) / groups;
+  // A warp to a token where there are enough tokens for the warps that fit; otherwise a token's passes
+  // are shared by as many warps as that leaves, down to a single pass each.
+  const int warps = kWarps * kCtasPerSm * d.sm_count;
+  p.parts = std::max(1, std::min(p.passes[0] + p.passes[1], warps / a->tokens));
+  const long long need = (static_cast<long long>(a->tokens) * p.parts + kWarps - 1) / kWarps;
+  const long long grid = std::min<long long>(need, kCtasPerSm * d.sm_count);  // (need, with parts)
   const bool il = a->interleaved != 0;
-  return lanes == 4   ? launch<4>(p, il, grid, d.dev, stream)
-         : lanes == 8 ? launch<8>(p, il, grid, d.dev, stream)
-                      : launch<16>(p, il, grid, d.dev, stream);
+  if (lanes == 4)
+    launch<4>(p, il, static_cast<unsigned>(grid), stream);
+  else if (lanes == 8)
+    launch<8>(p, il, static_cast<unsigned>(grid), stream);
+  else
+    launch<16>(p, il, static_cast<unsigned>(grid), stream);
+  return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_LAUNCH;
 }
 
 }  // namespace
