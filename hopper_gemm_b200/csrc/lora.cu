@@ -1,13 +1,19 @@
 // A shared projection with the low-rank adapters of many requests beside it:
 //   Y[t,:] = X[t,:] W + scale[a] * (X[t,:] Down[a]) Up[a],  a the adapter of token t's segment.
 //
-// Two launches (and one that returns at once). lora_shrink_kernel forms H = scale (X Down): one
-// tcgen05 product for every (row tile, adapter in it), K split over a cluster, and leaves H as
+// Many tokens: two launches (and one that returns at once). lora_shrink_kernel forms H = scale (X Down):
+// one tcgen05 product for every (row tile, adapter in it), K split over a cluster, and leaves H as
 // operand blocks of the second product: for every adapter of a row tile a block of 64-column rows in
 // which the rows of other adapters are zero. The projection's own GEMM kernel (hgemm_sm100.cu) then
 // walks those blocks as additional k-blocks behind the k-blocks of X and W, so that Up's product
 // lands in the same fp32 accumulators and Y is written and rounded once; an adapter costs its row
 // tiles rank / K of the GEMM. H is rounded to binary16 because it is a tcgen05 operand next to Up.
+//
+// Few tokens (decoding): bound by the bytes of W and of the adapters in use. W is the M operand of the
+// product, 128 of its columns to a CTA, and the tokens are its N; K is split over a cluster, so that
+// every SM pulls weights, and joined through distributed shared memory. The adapters run on the CUDA
+// cores in fp32, H in a launch of its own under whose feet the main kernel already starts, and Up's part
+// in warps that would otherwise wait for the main loop.
 //
 // No counterpart in the reference.
 
@@ -30,7 +36,10 @@ constexpr int kStageBytes = kABytes + kBlocks * kBBytes;
 constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
 constexpr int kPartStride = kBlocks * 64 + 4;  // floats of a partial row, padded for the banks
 static_assert(kTileRows * kPartStride * 4 <= kStages * kStageBytes, "partials reuse the stages");
-constexpr int kThreads = 192;
+// Warps of a shrink CTA: X's loads, issue, four that join, and one for each 64-column block of Down. A
+// thread is held about 400 cycles by a TMA load whatever its size, so every box of a stage has a
+// warp of its own (one warp for all five boxes: 30 us for 8192 tokens).
+constexpr int kThreads = 32 * (6 + kBlocks);
 
 struct LoraParams {
   const __half *X, *W, *down, *up;
@@ -168,24 +177,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int cols = p.chunks * 64;  // accumulator columns of an adapter
   bool ok = true;
 
-  if (warp == 0) {
+  const int box = warp - 6;  // of Down
+  if (warp == 0 || (box >= 0 && box < nu * p.chunks)) {
     if (lane == 0) {
+      const int adapter = box >= 0 ? s_list[u0 + box / p.chunks] : 0;
       int it = 0;
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int st = it % kStages;
-        if (it >= kStages && !op_wait(empty + 8 * st, (it / kStages - 1) & 1, wc, kSiteLoraEmpty)) {
-          ok = false;
+        if (it >= kStages &&
+            !(ok = op_wait(empty + 8 * st, (it / kStages - 1) & 1, wc, kSiteLoraEmpty)))
           break;
+        const uint32_t dst = base + st * kStageBytes, bar = full + 8 * st;
+        if (box < 0) {
+          ptx::mbar_arrive_expect_tx(bar, kABytes + nu * p.chunks * kBBytes);
+          ptx::tma_load_2d(&tmX, dst, bar, kb * 64, row0);
+        } else {
+          // (counted on the barrier before or after the bytes are announced)
+          ptx::tma_load_3d(&tmDown, dst + kABytes + box * kBBytes, bar, 64 * (box % p.chunks), kb * 64,
+                           adapter);
         }
-        ptx::mbar_arrive_expect_tx(full + 8 * st, kABytes + nu * p.chunks * kBBytes);
-        const uint32_t dst = base + st * kStageBytes;
-        ptx::tma_load_2d(&tmX, dst, full + 8 * st, kb * 64, row0);
-        for (int u = 0; u < nu; ++u)
-          for (int c = 0; c < p.chunks; ++c)
-            ptx::tma_load_3d(&tmDown, dst + kABytes + (u * p.chunks + c) * kBBytes, full + 8 * st,
-                             64 * c, kb * 64, s_list[u0 + u]);
       }
-      if (!ok)
+      if (!ok && box < 0)
         for (int j = max(0, it - kStages); j < it; ++j)
           op_drain(full + 8 * (j % kStages), (j / kStages) & 1);
     }
@@ -218,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
   ptx::tc_fence_after();
   float *part = reinterpret_cast<float *>(smem);
-  if (warp >= 2) {
+  if (warp >= 2 && warp < 6) {
     const int q = warp & 3;
     const uint32_t t = tmem + (static_cast<uint32_t>(q) << 21);
     float *dst = part + (32 * q + lane) * kPartStride;
@@ -326,6 +338,303 @@ __global__ void __launch_bounds__(256) lora_repair_kernel(const LoraParams p) {
   }
 }
 
+// ------------------------------------------------------------------------------ few tokens
+constexpr int kFewTokens = 64;  // at most (the accumulator's columns)
+constexpr int kFewCols = 128;   // columns of W in a CTA
+constexpr int kAddWarps = 8;    // that form the adapters' part and join the partial sums
+constexpr int kLoadWarps = 4;   // two for W, two for X, each every other stage
+constexpr int kFewThreads = 32 * (1 + kAddWarps + kLoadWarps);
+constexpr int kFewPart = kFewCols + 4;  // floats of a partial row
+constexpr int kLowThreads = 256;
+constexpr int kMaxSlices = 16;
+constexpr int kFewSmem = 104 * 1024;    // two CTAs to an SM
+
+struct LoraFewParams {
+  const __half *X, *down, *up;
+  __half *Y;
+  const float *scale;
+  const int *seg_start, *seg_adapter;
+  float *low;  // slices x tokens x rank: partial sums of X Down
+  int tokens, N, K, rank, adapters, segments;
+  int slices, slice_rows;   // K ranges of the first product
+  int n16;                  // tokens rounded up to 16
+  int ksplit, num_kb, stages, share;  // share: tokens that a CTA of the cluster joins
+  int whole_blocks;  // N % 64 == 0: tmW is (64 columns, K, column blocks), one box for 128 columns
+  unsigned *status_word;
+  unsigned long long timeout_ns;
+};
+
+// Adapter of token t, or -1, by one warp: every segment is looked at at once, so that this costs one
+// round trip to memory (a binary search with the adapter behind it is a chain of several).
+__device__ __forceinline__ int warp_token_adapter(const int *seg_start, const int *seg_adapter,
+                                                  int segments, int adapters, int t) {
+  int hit = -1, mine = -1;
+#pragma unroll 2
+  for (int i = threadIdx.x & 31; i < segments; i += 32) {
+    const int b = seg_start[i], e = seg_start[i + 1], a = seg_adapter[i];
+    if (b <= t && t < e) {
+      hit = i;
+      mine = a;
+    }
+  }
+  const int last = __reduce_max_sync(0xffffffffu, hit);
+  if (last < 0) return -1;
+  const int a = __shfl_sync(0xffffffffu, mine, last & 31);
+  return (a >= 0 && a < adapters) ? a : -1;
+}
+
+// Partial sums of X Down for one token and K range: a thread takes 8 columns of every few rows.
+__global__ void __launch_bounds__(kLowThreads) lora_low_kernel(const LoraFewParams p) {
+  ptx::grid_launch_dependents();
+  __shared__ float s_sum[kLowThreads / 32][kMaxRank];
+  const int t = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
+  const int a = warp_token_adapter(p.seg_start, p.seg_adapter, p.segments, p.adapters, t);
+  if (a < 0) return;
+  const int g8 = p.rank / 8;  // 16-byte groups of a row of Down
+  const int width = g8 <= 1 ? 1 : 1 << (32 - __clz(g8 - 1));  // lanes of a row, a power of two
+  const int g = threadIdx.x & (width - 1), r0 = threadIdx.x / width, rows = kLowThreads / width;
+  const int k0 = slice * p.slice_rows, k1 = min(p.K, k0 + p.slice_rows);
+  const __half *x = p.X + static_cast<long long>(t) * p.K;
+  const __half *dn = p.down + static_cast<long long>(a) * p.K * p.rank + 8 * g;
+  float f[8] = {};
+  if (g < g8) {
+#pragma unroll 8
+    for (int k = k0 + r0; k < k1; k += rows) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4 *>(dn + static_cast<long long>(k) * p.rank));
+      const float xv = __half2float(x[k]);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        f[2 * i] = fmaf(xv, v.x, f[2 * i]);
+        f[2 * i + 1] = fmaf(xv, v.y, f[2 * i + 1]);
+      }
+    }
+  }
+  for (int m = 16; m >= width; m >>= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] += __shfl_xor_sync(0xffffffffu, f[i], m);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane < width && g < g8)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s_sum[warp][8 * g + i] = f[i];
+  __syncthreads();
+  if (threadIdx.x < p.rank) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kLowThreads / 32; ++w) sum += s_sum[w][threadIdx.x];
+    p.low[(static_cast<long long>(slice) * p.tokens + t) * p.rank + threadIdx.x] = sum;
+  }
+}
+
+__global__ void __launch_bounds__(kFewThreads, 2)
+    lora_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                    const LoraFewParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ float s_low[kAddWarps][kMaxRank];
+  __shared__ int s_adapter[kFewTokens];
+  __shared__ __align__(8) uint64_t s_full[8], s_empty[8], s_acc;
+  __shared__ int s_abort;
+  __shared__ uint32_t s_tmem;
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t *smem = smem_raw + (base - raw);
+  const int x_bytes = p.n16 * 128, stage_bytes = 2 * kBBytes + x_bytes;
+  float *delta = reinterpret_cast<float *>(smem + p.stages * stage_bytes);  // share x kFewCols
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.x % p.ksplit, n0 = blockIdx.x / p.ksplit * kFewCols;
+  const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * split / p.ksplit);
+  const int kb1 = static_cast<int>(static_cast<long long>(p.num_kb) * (split + 1) / p.ksplit);
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int i = 0; i < p.stages; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&s_full[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&s_empty[i]), 1);
+    }
+    ptx::mbar_init(ptx::smem_u32(&s_acc), 1);
+    ptx::fence_mbar_init_cluster();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<1>(ptx::smem_u32(&s_tmem), 64);
+    ptx::tmem_relinquish<1>();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&s_tmem);
+  const OpWait wc{&s_abort, p.status_word, p.timeout_ns};
+  // Tokens that this CTA joins, adds the adapters' part to and writes.
+  const int t0 = min(p.tokens, split * p.share), t1 = min(p.tokens, t0 + p.share);
+
+  // Warps 0.. 7 add, 8 issues products, 9.. load. A thread is held 400 to 600 cycles by a TMA load, which
+  // for one thread and stages of 16 KB would be a third of what an SM can take in.
+  constexpr int kIssueWarp = kAddWarps;
+  if (warp > kIssueWarp) {
+    const int me = warp - kIssueWarp - 1;
+    const bool loads_x = me >= kLoadWarps / 2;
+    if (lane == 0) {
+      bool ok = true;
+      int it = me & 1;
+      for (; it < kb1 - kb0; it += 2) {
+        const int st = it % p.stages, kb = kb0 + it;
+        if (it >= p.stages && !(ok = op_wait(ptx::smem_u32(&s_empty[st]), (it / p.stages - 1) & 1, wc,
+                                             kSiteLoraFewEmpty)))
+          break;
+        const uint32_t bar = ptx::smem_u32(&s_full[st]), dst = base + st * stage_bytes;
+        if (loads_x) {
+          // (counted on the barrier before or after the bytes are announced)
+          ptx::tma_load_2d(&tmX, dst + 2 * kBBytes, bar, kb * 64, 0);
+        } else {
+          ptx::mbar_arrive_expect_tx(bar, stage_bytes);
+          if (p.whole_blocks) {
+            ptx::tma_load_3d(&tmW, dst, bar, 0, kb * 64, n0 / 64);
+          } else {
+            ptx::tma_load_2d(&tmW, dst, bar, n0, kb * 64);
+            ptx::tma_load_2d(&tmW, dst + kBBytes, bar, n0 + 64, kb * 64);
+          }
+        }
+      }
+      if (!ok && !loads_x)
+        for (int j = max(me & 1, it - 2 * p.stages); j < it; j += 2)
+          op_drain(ptx::smem_u32(&s_full[j % p.stages]), (j / p.stages) & 1);
+    }
+  } else if (warp == kIssueWarp) {
+    if (lane == 0) {
+      const uint32_t idesc = ptx::umma_idesc_f16_f32(kFewCols, p.n16, true, true);
+      int it = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int st = it % p.stages;
+        if (!op_wait(ptx::smem_u32(&s_full[st]), (it / p.stages) & 1, wc, kSiteLoraFewFull)) break;
+        ptx::tc_fence_after();
+        const uint32_t src = base + st * stage_bytes;
+        // W: columns are M (64-column blocks 8 KB apart), 16 k are 16 rows of 128 bytes. X: K-major.
+        const uint64_t wd = ptx::umma_desc_sw128(src, kBBytes, 1024);
+        const uint64_t xd = ptx::umma_desc_sw128(src + 2 * kBBytes, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          ptx::umma_f16<1>(tmem, wd + 128 * k, xd + 2 * k, idesc, it > 0 || k > 0);
+        if (kb + p.stages < kb1) ptx::umma_commit<1>(ptx::smem_u32(&s_empty[st]));
+      }
+      ptx::umma_commit<1>(ptx::smem_u32(&s_acc));
+    }
+  } else {
+    // The adapters' part of this CTA's tokens, while the main loop runs: a warp takes a token, 16 lanes
+    // its 128 columns, the two halves of the warp every other row of Up.
+    const int w = warp, c = 8 * (lane & 15);
+    // What does not hang on the first product: whose token it is, and Up's rows into L2.
+    for (int t = t0 + w; t < t1; t += kAddWarps) {
+      const int a = warp_token_adapter(p.seg_start, p.seg_adapter, p.segments, p.adapters, t);
+      if (lane == 0) s_adapter[t] = a;
+      if (a >= 0 && n0 + c < p.N)
+        for (int r = lane >> 4; r < p.rank; r += 2)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(
+              p.up + (static_cast<long long>(a) * p.rank + r) * p.N + n0 + c));
+    }
+    ptx::grid_wait();
+    for (int t = t0 + w; t < t1; t += kAddWarps) {
+      __syncwarp();
+      const int a = s_adapter[t];
+      float f[8] = {};
+      if (a >= 0) {
+        const float sc = p.scale[a];
+        for (int r = lane; r < p.rank; r += 32) {
+          float h[kMaxSlices];
+#pragma unroll
+          for (int s = 0; s < kMaxSlices; ++s)
+            h[s] = s < p.slices ? p.low[(static_cast<long long>(s) * p.tokens + t) * p.rank + r] : 0.0f;
+          float sum = 0.0f;
+#pragma unroll
+          for (int s = 0; s < kMaxSlices; ++s) sum += h[s];
+          s_low[w][r] = sum * sc;
+        }
+        __syncwarp();
+        if (n0 + c < p.N) {
+          const __half *up = p.up + static_cast<long long>(a) * p.rank * p.N + n0 + c;
+#pragma unroll 8
+          for (int r = lane >> 4; r < p.rank; r += 2) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(up + static_cast<long long>(r) * p.N));
+            const float h = s_low[w][r];
+            const uint32_t v4[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&v4[i]));
+              f[2 * i] = fmaf(h, v.x, f[2 * i]);
+              f[2 * i + 1] = fmaf(h, v.y, f[2 * i + 1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] += __shfl_xor_sync(0xffffffffu, f[i], 16);
+      }
+      if (lane < 16) {
+        float *dst = delta + (t - t0) * kFewCols + c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dst[i] = f[i];
+      }
+    }
+  }
+  // Partial sums to shared memory (the stages are free once the last product has retired).
+  __syncwarp();
+  int okw = 1;
+  if (lane == 0) okw = op_wait(ptx::smem_u32(&s_acc), 0, wc, kSiteLoraFewAcc);
+  const bool ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
+  ptx::tc_fence_after();
+  float *part = reinterpret_cast<float *>(smem);  // token x column
+  const bool adds = warp < kAddWarps;
+  if (adds && ok) {
+    // (two warps to a lane quarter, every other 16 columns each)
+    const int q = warp & 3;
+    for (int c = 16 * (warp >> 2); c < p.n16; c += 32) {
+      uint32_t v[16];
+      ptx::tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q) << 21) + c, v);
+      ptx::tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) part[(c + i) * kFewPart + 32 * q + lane] = __uint_as_float(v[i]);
+    }
+  }
+  ptx::tc_fence_before();
+  if (p.ksplit > 1)
+    ptx::cluster_sync();
+  else
+    __syncthreads();
+  if (adds && ok) {
+    constexpr int kAhead = 2, kStep = kAddWarps / 4;  // tokens in flight of a thread; of the CTA
+    const int col = threadIdx.x & (kFewCols - 1);
+    const uint32_t part_addr = ptx::smem_u32(part);
+    for (int t = t0 + static_cast<int>(threadIdx.x) / kFewCols; t < t1; t += kAhead * kStep) {
+      float v[kAhead][8];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int tt = min(t + x * kStep, t1 - 1);
+        const uint32_t off = part_addr + (tt * kFewPart + col) * 4;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < p.ksplit) v[x][k] = ptx::ld_shared_cluster_f(ptx::mapa(off, k));
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int tt = t + x * kStep;
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < p.ksplit) sum += v[x][k];
+        if (tt < t1 && n0 + col < p.N)
+          p.Y[static_cast<long long>(tt) * p.N + n0 + col] =
+              __float2half_rn(sum + delta[(tt - t0) * kFewCols + col]);
+      }
+    }
+  }
+  if (p.ksplit > 1)
+    ptx::cluster_sync();  // nobody reads this CTA's partials any more
+  else
+    __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<1>(tmem, 64);
+  }
+}
+
 // ------------------------------------------------------------------------------ host side
 bool sizes_ok(int tokens, int N, int K, int rank, int adapters, int segments) {
   return tokens >= 0 && N >= 0 && K >= 8 && N % 8 == 0 && K % 8 == 0 && rank >= 8 &&
@@ -370,6 +679,86 @@ int check(const hgemm_lora_t *a) {
   return HGEMM_OK;
 }
 
+// Few tokens: K ranges of the first product, so that the CTAs of all tokens fill the SMs a few times, of
+// 64 rows at least (a workspace of `tokens` tokens holds them).
+int few_slices(int tokens, int K) {
+  return std::max(1, std::min({kMaxSlices, 592 / tokens, K / 64}));
+}
+
+int run_few(const hgemm_lora_t *a, const OpDevice &d, cudaStream_t stream) {
+  LoraFewParams p;
+  p.X = a->X;
+  p.down = a->down;
+  p.up = a->up;
+  p.Y = a->Y;
+  p.scale = a->scale;
+  p.seg_start = a->seg_start;
+  p.seg_adapter = a->seg_adapter;
+  p.low = static_cast<float *>(a->workspace);
+  p.tokens = a->tokens;
+  p.N = a->N;
+  p.K = a->K;
+  p.rank = a->rank;
+  p.adapters = a->adapters;
+  p.segments = a->segments;
+  p.slices = few_slices(a->tokens, a->K);
+  p.slice_rows = (a->K + p.slices - 1) / p.slices;
+  p.n16 = (a->tokens + 15) / 16 * 16;
+  p.num_kb = (a->K + 63) / 64;
+  p.status_word = d.status_word;
+  p.timeout_ns = d.timeout_ns;
+  // Two CTAs to an SM, and of K as many ranges as they take, a power of two, with 4 k-blocks or more each
+  const int tiles = (a->N + kFewCols - 1) / kFewCols;
+  // (clusters of 6 left CTAs for a second wave: 26 us against 20 us with 4 at N = 6144).
+  p.ksplit = 1;
+  while (p.ksplit < 8 && 2 * p.ksplit * tiles <= 2 * d.sm_count && p.num_kb >= 8 * p.ksplit) p.ksplit *= 2;
+  p.share = (a->tokens + p.ksplit - 1) / p.ksplit;
+  const int stage = 2 * kBBytes + p.n16 * 128, delta = p.share * kFewCols * 4;
+  p.stages = std::min(8, (kFewSmem - 1024 - delta) / stage);
+  const int smem = 1024 + p.stages * stage + delta;
+  CUtensorMap tw, tx;
+  const unsigned long long wd[2] = {static_cast<unsigned long long>(a->N),
+                                    static_cast<unsigned long long>(a->K)};
+  const unsigned long long ws[1] = {2ull * a->N};
+  const unsigned wb[2] = {64, 64};
+  const unsigned long long xd[2] = {static_cast<unsigned long long>(a->K),
+                                    static_cast<unsigned long long>(a->tokens)};
+  const unsigned long long xs[1] = {2ull * a->K};
+  const unsigned xb[2] = {64, static_cast<unsigned>(p.n16)};
+  const unsigned long long wd3[3] = {64, static_cast<unsigned long long>(a->K),
+                                     static_cast<unsigned long long>(a->N / 64)};
+  const unsigned long long ws3[2] = {2ull * a->N, 128};
+  const unsigned wb3[3] = {64, 64, 2};
+  p.whole_blocks = a->N % 64 == 0;
+  if (!(p.whole_blocks ? op_encode(&tw, a->W, 3, wd3, ws3, wb3) : op_encode(&tw, a->W, 2, wd, ws, wb)) ||
+      !op_encode(&tx, a->X, 2, xd, xs, xb))
+    return HGEMM_ERR_TENSOR_MAP;
+  static bool done[64];
+  const int st = op_smem(reinterpret_cast<const void *>(lora_few_kernel), kFewSmem, d.dev, done);
+  if (st != HGEMM_OK) return st;
+  lora_low_kernel<<<p.tokens * p.slices, kLowThreads, 0, stream>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return HGEMM_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.ksplit), 1, 1);
+  cfg.blockDim = dim3(kFewThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.ksplit;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.ksplit > 1 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, lora_few_kernel, tw, tx, p) != cudaSuccess) {
+    cudaGetLastError();
+    return HGEMM_ERR_LAUNCH;
+  }
+  return HGEMM_OK;
+}
+
 int run(const hgemm_lora_t *a, cudaStream_t stream) {
   int st = check(a);
   if (st != HGEMM_OK || a->tokens == 0 || a->N == 0) return st;
@@ -378,6 +767,7 @@ int run(const hgemm_lora_t *a, cudaStream_t stream) {
   OpDevice d;
   st = op_device(&d);
   if (st != HGEMM_OK) return st;
+  if (a->tokens <= kFewTokens) return run_few(a, d, stream);
   LoraParams p;
   st = lora_gemm_tile_rows(a->tokens, a->N, a->K, &p.tile_rows);
   if (st != HGEMM_OK) return st;
@@ -484,6 +874,8 @@ int hgemm_lora(const hgemm_lora_t *args, hgemm_stream_t stream) {
 size_t hgemm_lora_workspace_bytes(int tokens, int N, int K, int rank, int adapters, int segments) {
   if (!hgemm::sizes_ok(tokens, N, K, rank, adapters, segments)) return 0;
   if (tokens == 0 || N == 0 || adapters == 0 || segments == 0) return 0;
+  if (tokens <= hgemm::kFewTokens)
+    return static_cast<size_t>(hgemm::few_slices(tokens, K)) * tokens * rank * sizeof(float);
   return hgemm::layout(tokens, N, rank, segments).total;
 }
 

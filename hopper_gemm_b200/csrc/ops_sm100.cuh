@@ -60,6 +60,9 @@ enum OpWaitSite : unsigned {
   kSiteLoraEmpty = 40,
   kSiteLoraFull = 41,
   kSiteLoraAcc = 42,
+  kSiteLoraFewEmpty = 43,
+  kSiteLoraFewFull = 44,
+  kSiteLoraFewAcc = 45,
   kSiteOpDrain = 63,
 };
 

@@ -294,6 +294,11 @@ __device__ __forceinline__ float4 ld_shared_v4f(uint32_t addr) {
                : "memory");
   return v;
 }
+__device__ __forceinline__ float ld_shared_cluster_f(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float4 ld_shared_cluster_v4f(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -426,6 +431,16 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)
         "=r"(r[31])
       : "r"(taddr));
 }
+// 16 consecutive columns.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
 // Each thread of the warp writes 32 consecutive 32-bit columns of its own TMEM lane.
 __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -466,9 +481,21 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16_f32(int M, int N) {
          (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-// Same with the B operand's layout chosen: MN-major (as above) or K-major.
-__host__ __device__ constexpr uint32_t umma_idesc_f16_f32(int M, int N, bool b_k_major) {
-  return umma_idesc_f16_f32(M, N) & ~(b_k_major ? (1u << 16) : 0u);
+// Same with the operands' layouts chosen (K-major or MN-major).
+__host__ __device__ constexpr uint32_t umma_idesc_f16_f32(int M, int N, bool b_k_major,
+                                                          bool a_mn_major = false) {
+  return (umma_idesc_f16_f32(M, N) & ~(b_k_major ? (1u << 16) : 0u)) |
+         (a_mn_major ? (1u << 15) : 0u);
+}
+
+// ------------------------------------------------------------------------ dependent launches
+// Programmatic dependent launch: the next kernel of the stream (launched with the attribute) may start
+// now, and waits in grid_wait for this grid to have completed before it reads what it wrote.
+__device__ __forceinline__ void grid_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace ptx
