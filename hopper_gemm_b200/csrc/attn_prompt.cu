@@ -87,6 +87,7 @@ constexpr int kSmemLimit = 232448;
 // output is rescaled only when the maximum has grown past it. 2^8 times a weight below 1 stays far
 // inside binary16, and the fp32 sums do not care.
 constexpr float kLag = 8.0f;
+constexpr int kPolyEvery = 4;
 
 // DB: 64-element blocks of head_dim in shared memory (head_dim <= 64 DB); TILES: row tiles of a CTA,
 // each with its own four softmax warps.
@@ -113,15 +114,22 @@ struct AttnCfg {
   static_assert(O_COL + TILES * DB * 64 <= TMEM_COLS, "TMEM");
 };
 
-// Sequence of tile w (tiles of `span` queries, whole sequences one after the other, longest row range
-// first inside a sequence), by one warp. Returns the sequence or -1, and the tile inside it.
-__device__ __forceinline__ int find_tile(const AttnParams &p, int w, int span, int &tile) {
+// Work of a CTA: a sequence and a tile of `span` queries in it.
+struct Tile {
+  int q0, qlen, k0, klen;
+  int tile;  // -1: none (the grid is an upper bound)
+};
+
+// Tile w of all sequences one after the other, the last tile (with the most keys to see) of each first, by
+// one warp: 32 sequences at a time, with one round trip to memory for all of their four starts.
+__device__ __forceinline__ Tile find_tile(const AttnParams &p, int w, int span) {
   const int lane = threadIdx.x & 31;
+  Tile t = {0, 0, 0, 0, -1};
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    int n = 0;
+    int q0 = 0, q1 = 0, k0 = 0, k1 = 0, n = 0;
     if (b0 + lane < p.batch) {
-      int q0, q1;
       seq_range(p.cu_q, b0 + lane, p.total_q, q0, q1);
+      seq_range(p.cu_k, b0 + lane, p.total_k, k0, k1);
       n = (q1 - q0 + span - 1) / span;
     }
     int sum = n;
@@ -133,18 +141,47 @@ __device__ __forceinline__ int find_tile(const AttnParams &p, int w, int span, i
     const unsigned hit = __ballot_sync(0xffffffffu, w < sum);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const int end = __shfl_sync(0xffffffffu, sum, src);
-      tile = end - 1 - w;
-      return b0 + src;
+      t.q0 = __shfl_sync(0xffffffffu, q0, src);
+      t.qlen = __shfl_sync(0xffffffffu, q1, src) - t.q0;
+      t.k0 = __shfl_sync(0xffffffffu, k0, src);
+      t.klen = __shfl_sync(0xffffffffu, k1, src) - t.k0;
+      t.tile = __shfl_sync(0xffffffffu, sum, src) - 1 - w;
+      return t;
     }
     w -= __shfl_sync(0xffffffffu, sum, 31);
   }
-  return -1;
+  return t;
 }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 2^x for two values on the FMA pipe: x is cut into an integer n and f in [-1/2, 1/2] (Cody and
+// Waite), 2^f is a polynomial of degree 4 through 1 at 0 (fitted for the least relative error, 2.9e-6 in
+// fp32: 1/170 of the binary16 rounding that every weight gets), n goes into the exponent. Below
+// 2^-126 the result is some tiny value that rounds to zero; infinities and NaN leave as values that
+// overflow binary16, which the output's check sees.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: its ulp is 1
+  const float2 t = __fadd2_rn(x, big);
+  const float2 f = __fadd2_rn(x, __ffma2_rn(t, make_float2(-1.0f, -1.0f), big));
+  float2 r = __ffma2_rn(f, make_float2(9.582853e-3f, 9.582853e-3f),
+                        make_float2(5.5906425e-2f, 5.5906425e-2f));
+  r = __ffma2_rn(r, f, make_float2(2.4024099e-1f, 2.4024099e-1f));
+  r = __ffma2_rn(r, f, make_float2(6.9312419e-1f, 6.9312419e-1f));
+  r = __ffma2_rn(r, f, make_float2(1.0f, 1.0f));
+  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 
@@ -164,12 +201,12 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   const uint32_t empty = full + 8 * S;                // [S] the products that read them are done
   const uint32_t qfull = empty + 8 * S;               // [1] queries landed
   const uint32_t sfull = qfull + 8;                   // [TILES] scores ready (and the last O product done)
-  const uint32_t pfull = sfull + 8 * TILES;           // [TILES] weights ready (and O rescaled)
-  const uint32_t ofull = pfull + 8 * TILES;           // [TILES] output ready
-  int *misc = reinterpret_cast<int *>(bars + 2 * S + 1 + 3 * TILES);
+  const uint32_t pfull = sfull + 8 * TILES;           // [TILES][2] half of the weights ready (and O rescaled)
+  const uint32_t ofull = pfull + 16 * TILES;          // [TILES] output ready
+  int *misc = reinterpret_cast<int *>(bars + 2 * S + 1 + 4 * TILES);
   volatile int *abort_flag = misc;
-  volatile int *found = misc + 1;  // sequence, tile
-  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(misc + 3);
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(misc + 1);
+  Tile *found = reinterpret_cast<Tile *>(misc + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kLoadWarp = TILES * 4, kMmaWarp = TILES * 4 + 1;
@@ -179,11 +216,13 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   const int span = TILES * p.tile_q;  // queries of this CTA
 
   if (warp == 0) {
-    int tile = 0;
-    const int s = find_tile(p, w, span, tile);
+    const Tile t = find_tile(p, w, span);
+    if (lane == 0) *found = t;
+  } else if (warp == kLoadWarp) {
     if (lane == 0) {
-      found[0] = s;
-      found[1] = tile;
+      ptx::prefetch_tmap(&tmQ);
+      ptx::prefetch_tmap(&tmK);
+      ptx::prefetch_tmap(&tmV);
       *abort_flag = 0;
       for (int i = 0; i < S; ++i) {
         ptx::mbar_init(full + 8 * i, 1);
@@ -192,47 +231,36 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       ptx::mbar_init(qfull, 1);
       for (int i = 0; i < TILES; ++i) {
         ptx::mbar_init(sfull + 8 * i, 1);
-        ptx::mbar_init(pfull + 8 * i, 4);
+        ptx::mbar_init(pfull + 16 * i, 4);
+        ptx::mbar_init(pfull + 16 * i + 8, 4);
         ptx::mbar_init(ofull + 8 * i, 1);
       }
       ptx::fence_mbar_init_cluster();
     }
-  } else if (warp == kLoadWarp && lane == 0) {
-    ptx::prefetch_tmap(&tmQ);
-    ptx::prefetch_tmap(&tmK);
-    ptx::prefetch_tmap(&tmV);
-  }
-  __syncthreads();
-  const int s = found[0], qt = found[1];
-  if (s < 0) return;  // behind the last tile (the grid is an upper bound)
-
-  int q0, q1, k0, k1;
-  seq_range(p.cu_q, s, p.total_q, q0, q1);
-  seq_range(p.cu_k, s, p.total_k, k0, k1);
-  const int qlen = q1 - q0, klen = k1 - k0;
-  // Blocks of keys that tile i needs: [0, need_i); this CTA's share is [b0, b0 + count_i).
-  auto need_of = [&](int i) {
-    const int first = qt * span + i * p.tile_q;
-    if (first >= qlen) return 0;
-    const int last = min(first + p.tile_q, qlen) - 1;
-    const int seen = p.causal ? max(0, min(klen, last + 1 + klen - qlen)) : klen;
-    return (seen + kKeys - 1) / kKeys;
-  };
-  const int need = need_of(TILES - 1) > need_of(0) ? need_of(TILES - 1) : need_of(0);
-  const int per = (need + p.nsplit - 1) / p.nsplit;
-  const int b0 = split * per;
-  auto count_of = [&](int i) { return max(0, min(need_of(i) - b0, per)); };
-  const int count0 = count_of(0), count1 = TILES == 2 ? count_of(1) : 0;
-  const int count = max(count0, count1);
-
-  if (count > 0 && warp == kMmaWarp) {
+  } else if (warp == kMmaWarp) {
     ptx::tmem_alloc<1>(ptx::smem_u32(tmem_holder), Cfg::TMEM_COLS);
     ptx::tmem_relinquish<1>();
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = count > 0 ? *reinterpret_cast<volatile uint32_t *>(tmem_holder) : 0u;
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(tmem_holder);
+  const Tile work = *found;
+  const int q0 = work.q0, qlen = work.qlen, k0 = work.k0, klen = work.klen, qt = work.tile;
+  // Blocks of keys that tile i needs: [0, need_i); this CTA's share is [b0, b0 + count_i).
+  auto need_of = [&](int i) {
+    const int first = qt * span + i * p.tile_q;
+    if (qt < 0 || first >= qlen) return 0;
+    const int last = min(first + p.tile_q, qlen) - 1;
+    const int seen = p.causal ? max(0, min(klen, last + 1 + klen - qlen)) : klen;
+    return (seen + kKeys - 1) / kKeys;
+  };
+  const int need = max(need_of(0), need_of(TILES - 1));
+  const int per = (need + p.nsplit - 1) / p.nsplit;
+  const int b0 = split * per;
+  auto count_of = [&](int i) { return max(0, min(need_of(i) - b0, per)); };
+  const int count0 = count_of(0), count1 = TILES == 2 ? count_of(1) : 0;
+  const int count = max(count0, count1);
   OpWait wc{abort_flag, p.status_word, p.timeout_ns};
 
   if (warp >= TILES * 4) {
@@ -265,50 +293,78 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         for (int j = max(0, it - S); j < it; ++j) op_drain(full + 8 * (j % S), (j / S) & 1);
       }
     }
-    if (warp == kMmaWarp && lane == 0 && count > 0) {
+    if (warp == kMmaWarp && count > 0) {
+      // The whole warp walks the loop and one lane issues: descriptors then stay in uniform registers.
+      // (Walked by one lane, a product took about 130 cycles to issue, twice its time on the tensor core.)
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t idesc_s = ptx::umma_idesc_f16_f32(kRows, kKeys, true);
       const uint32_t idesc_o = ptx::umma_idesc_f16_f32(kRows, p.dim16, false);
       const int ksteps = p.dim16 / 16;
-      bool ok = op_wait(qfull, 0, wc, kSiteAttnQ);
+      const bool one = ptx::elect_one();
+      bool ok = __all_sync(0xffffffffu, op_wait(qfull, 0, wc, kSiteAttnQ));
+      auto wait = [&](uint32_t bar, int phase, unsigned site) {
+        return __all_sync(0xffffffffu, op_wait(bar, phase & 1, wc, site)) != 0;
+      };
+      auto commit = [&](uint32_t bar) {
+        if (one) ptx::umma_commit<1>(bar);
+      };
       auto scores = [&](int i, int stage) {
         const uint64_t qd = ptx::umma_desc_sw128(sQ + i * Cfg::TILE_BYTES, 16, 1024);
         const uint64_t kd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES, 16, 1024);
-        for (int k = 0; k < ksteps; ++k) {
-          // 16 elements are 32 bytes of a 128-byte row; the next 64 lie one block of 16 KB on.
-          const uint64_t off = static_cast<uint64_t>((k >> 2) * (kRows * 128 / 16) + (k & 3) * 2);
-          ptx::umma_f16<1>(tmem + i * kKeys, qd + off, kd + off, idesc_s, k > 0);
-        }
-        ptx::umma_commit<1>(sfull + 8 * i);
-      };
-      auto output = [&](int i, int stage, bool first) {
-        const uint64_t vd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES, kKeys * 128, 1024);
+        if (one) {
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          ptx::umma_f16_ts(tmem + Cfg::O_COL + i * (DB * 64), tmem + i * kKeys + 8 * k, vd + 128 * k,
-                           idesc_o, !(first && k == 0));
+          for (int k = 0; k < DB * 4; ++k) {
+            // 16 elements are 32 bytes of a 128-byte row; the next 64 lie one block of 16 KB on.
+            const uint64_t off = static_cast<uint64_t>((k >> 2) * (kRows * 128 / 16) + (k & 3) * 2);
+            if (k < ksteps) ptx::umma_f16<1>(tm + i * kKeys, qd + off, kd + off, idesc_s, k > 0);
+          }
+          ptx::umma_commit<1>(sfull + 8 * i);
+        }
       };
-      auto cnt = [&](int i) { return i == 0 ? count0 : count1; };
-      if (ok) ok = op_wait(full, 0, wc, kSiteAttnKvFull);
+      // Half of a block's keys at a time, as the weights come.
+      auto output = [&](int i, int stage, bool first, int half) {
+        const uint64_t vd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES, kKeys * 128, 1024);
+        if (one) {
+#pragma unroll
+          for (int x = 0; x < kKeys / 32; ++x) {
+            const int k = half * (kKeys / 32) + x;
+            ptx::umma_f16_ts(tm + Cfg::O_COL + i * (DB * 64), tm + i * kKeys + 8 * k, vd + 128 * k,
+                             idesc_o, !(first && k == 0));
+          }
+        }
+      };
+      if (ok) ok = wait(full, 0, kSiteAttnKvFull);
       if (ok) {
         ptx::tc_fence_after();
+#pragma unroll
         for (int i = 0; i < TILES; ++i)
-          if (cnt(i) > 0) scores(i, 0);
-        if (S < 2 * count) ptx::umma_commit<1>(empty);
+          if ((i == 0 ? count0 : count1) > 0) scores(i, 0);
+        if (S < 2 * count) commit(empty);
       }
+      int vst = 1, vph = 0;  // stage and phase of block j's values; its successor's keys lie behind them
+#pragma unroll 1
       for (int j = 0; ok && j < count; ++j) {
-        const int vs = 2 * j + 1, ks = 2 * j + 2;
-        const int vst = vs % S, kst = ks % S;
-        if (!(ok = op_wait(full + 8 * vst, (vs / S) & 1, wc, kSiteAttnKvFull))) break;
+        int kst = vst + 1, kph = vph;
+        if (kst == S) {
+          kst = 0;
+          kph ^= 1;
+        }
+        if (!(ok = wait(full + 8 * vst, vph, kSiteAttnKvFull))) break;
         bool k_here = false;
+#pragma unroll
         for (int i = 0; i < TILES; ++i) {
-          if (j >= cnt(i)) continue;
-          if (!(ok = op_wait(pfull + 8 * i, j & 1, wc, kSiteAttnWeights))) break;
+          const int cnt = i == 0 ? count0 : count1;
+          if (!ok || j >= cnt) continue;
+          if (!(ok = wait(pfull + 16 * i, j, kSiteAttnWeights))) continue;
           ptx::tc_fence_after();
-          output(i, vst, j == 0);
-          if (j + 1 == cnt(i)) {
-            ptx::umma_commit<1>(ofull + 8 * i);
+          output(i, vst, j == 0, 0);
+          if (!(ok = wait(pfull + 16 * i + 8, j, kSiteAttnWeights))) continue;
+          ptx::tc_fence_after();
+          output(i, vst, j == 0, 1);
+          if (j + 1 == cnt) {
+            commit(ofull + 8 * i);
           } else {
-            if (!k_here && !(ok = op_wait(full + 8 * kst, (ks / S) & 1, wc, kSiteAttnKvFull))) break;
+            if (!k_here && !(ok = wait(full + 8 * kst, kph, kSiteAttnKvFull))) continue;
             k_here = true;
             ptx::tc_fence_after();
             // Issued behind the product that reads this tile's weights, whose columns it overwrites;
@@ -318,14 +374,21 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         }
         if (!ok) break;
         // A stage that nothing is loaded into any more is not announced: no arrival outlives the CTA.
-        if (vs + S < 2 * count) ptx::umma_commit<1>(empty + 8 * vst);
-        if (ks + S < 2 * count) ptx::umma_commit<1>(empty + 8 * kst);
+        if (2 * j + 1 + S < 2 * count) commit(empty + 8 * vst);
+        if (2 * j + 2 + S < 2 * count) commit(empty + 8 * kst);
+        vst = kst + 1;
+        vph = kph;
+        if (vst == S) {
+          vst = 0;
+          vph ^= 1;
+        }
       }
       if (!ok) {
         // Unwinding: every product retires before TMEM is freed.
-        ptx::umma_commit<1>(qfull);
+        commit(qfull);
         op_drain(qfull, 1);
       }
+      __syncwarp();
     }
   } else {
     // ---------------------------------------------------------------- softmax warps
@@ -335,12 +398,13 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     const int first = qt * span + i * p.tile_q;
     const int n = i == 0 ? count0 : count1;
     const int qi = first + row / p.group;  // query of this row, inside the sequence
-    const bool live = row < p.tile_q * p.group && qi < qlen;
+    const bool live = qt >= 0 && row < p.tile_q * p.group && qi < qlen;
     const int limit = p.causal ? max(0, min(klen, qi + 1 + klen - qlen)) : klen;
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp, lane << 16
     const uint32_t tS = tmem + lane_base + i * kKeys;
     const uint32_t tO = tmem + lane_base + Cfg::O_COL + i * (DB * 64);
-    float m = -INFINITY, l = 0.0f;  // maximum that the weights are relative to (scaled), their sum
+    float m = -INFINITY;  // maximum that the weights are relative to (scaled)
+    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};  // of the weights, in four parts
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       int okw = 1;
@@ -349,32 +413,41 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       if (!ok) break;
       ptx::tc_fence_after();
       uint32_t sr[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(tS + 32 * c, sr[c]);
+      ptx::tmem_ld_32x32b_x32(tS, sr[0]);
+      ptx::tmem_ld_32x32b_x32(tS + 32, sr[1]);
       ptx::tmem_ld_wait();
+      ptx::tmem_ld_32x32b_x32(tS + 64, sr[2]);
+      ptx::tmem_ld_32x32b_x32(tS + 96, sr[3]);
       const int left = limit - (b0 + j) * kKeys;  // keys of this block that the row sees
-      if (__any_sync(0xffffffffu, left < kKeys)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
+      const bool cut = __any_sync(0xffffffffu, left < kKeys);
+      float mx[2] = {-INFINITY, -INFINITY};
+      auto mask_and_max = [&](int c) {
+        if (cut)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (32 * c + e >= left) sr[c][e] = 0xff800000u;  // -infinity
-      }
-      float mx[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(sr[c][0]);
-#pragma unroll
-        for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(sr[c][e]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2;
+        for (int e = 0; e < 32; e += 4) {
+          mx[0] = max3(mx[0], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
+          mx[1] = max3(mx[1], __uint_as_float(sr[c][e + 2]), __uint_as_float(sr[c][e + 3]));
+        }
+      };
+      mask_and_max(0);
+      mask_and_max(1);
+      ptx::tmem_ld_wait();
+      mask_and_max(2);
+      mask_and_max(3);
+      const float top = fmaxf(mx[0], mx[1]) * p.scale2;
       const bool grow = top > m + kLag;  // true of the first key, from -infinity
       const float m_old = m;
       if (grow) m = top;
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
         // The scores of block j were committed behind block j - 1's product, so O is at rest.
         const float f = (grow && m_old != -INFINITY) ? ex2(m_old - m) : 1.0f;
-        l *= f;
+        sum[0].x *= f;
+        sum[0].y *= f;
+        sum[1].x *= f;
+        sum[1].y *= f;
         for (int c = 0; c < DB * 2; ++c) {
           uint32_t o[32];
           ptx::tmem_ld_32x32b_x32(tO + 32 * c, o);
@@ -384,28 +457,30 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
           ptx::tmem_st_32x32b_x32(tO + 32 * c, o);
         }
       }
-      const float neg = m == -INFINITY ? 0.0f : -m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const float neg1 = m == -INFINITY ? 0.0f : -m;
+      const float2 neg = make_float2(neg1, neg1), scale = make_float2(p.scale2, p.scale2);
 #pragma unroll
-      for (int c = 0; c < 4; c += 2) {
+      for (int half = 0; half < 2; ++half) {
         uint32_t w2[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const int cc = c + (e >> 4), ee = (e & 15) * 2;
-          const float a = ex2(fmaf(__uint_as_float(sr[cc][ee]), p.scale2, neg));
-          const float b = ex2(fmaf(__uint_as_float(sr[cc][ee + 1]), p.scale2, neg));
-          sum[(e & 1) * 2] += a;
-          sum[(e & 1) * 2 + 1] += b;
-          const __half2 ab = __floats2half2_rn(a, b);
-          w2[e] = *reinterpret_cast<const uint32_t *>(&ab);
+          const int cc = 2 * half + (e >> 4), ee = (e & 15) * 2;
+          const float2 x = __ffma2_rn(
+              make_float2(__uint_as_float(sr[cc][ee]), __uint_as_float(sr[cc][ee + 1])), scale, neg);
+          // The special function unit would be as long at work as the tensor core; every kPolyEvery-th
+          // pair goes through the FMA pipe instead.
+          const float2 ab = (e % kPolyEvery == kPolyEvery - 1) ? ex2_poly(x)
+                                                                : make_float2(ex2(x.x), ex2(x.y));
+          sum[e & 1] = __fadd2_rn(sum[e & 1], ab);
+          const __half2 h = __float22half2_rn(ab);
+          w2[e] = *reinterpret_cast<const uint32_t *>(&h);
         }
-        ptx::tmem_st_32x32b_x32(tS + 16 * c, w2);
+        ptx::tmem_st_32x32b_x32(tS + 32 * half, w2);
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(pfull + 16 * i + 8 * half);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      ptx::tmem_st_wait();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(pfull + 8 * i);
     }
     if (ok && n > 0) {
       int okw = 1;
@@ -419,21 +494,28 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       const bool any = ke > kb;
       const long long orow =
           static_cast<long long>(q0 + qi) * p.heads_q + h * p.group + row % p.group;
-      const float inv = any ? 1.0f / l : 0.0f;
-      bool odd = any && !(l > 0.0f && l < INFINITY);  // a sum that no finite scores give
+      const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      const float inv1 = any ? 1.0f / l : 0.0f;
+      const float2 inv = make_float2(inv1, inv1), zero = make_float2(0.0f, 0.0f);
+      const bool clear = !__all_sync(0xffffffffu, any);  // rows without a key: zeros, whatever stands in O
+      float2 check[2] = {zero, zero};  // stays 0 with finite outputs, NaN otherwise
       uint8_t *stage = smem + i * Cfg::TILE_BYTES;
       float *part = p.part_o + (static_cast<long long>(split) * p.total_q * p.heads_q + orow) * p.dim16;
+#pragma unroll
       for (int c = 0; c < DB * 2; ++c) {
+        if (32 * c >= p.dim16) break;
         uint32_t o[32];
         if (n > 0) {
           ptx::tmem_ld_32x32b_x32(tO + 32 * c, o);
           ptx::tmem_ld_wait();
         }
-        float f[32];
+        float2 f[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          f[e] = any ? __uint_as_float(o[e]) * inv : 0.0f;
-          if (32 * c + e < p.head_dim) odd |= !(fabsf(f[e]) < INFINITY);
+        for (int e = 0; e < 16; ++e) {
+          f[e] = __fmul2_rn(make_float2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])), inv);
+          if (clear && !any) f[e] = zero;
+          // (columns behind dim16 hold nothing)
+          if (e < 8 || 32 * c + 16 < p.dim16) check[e & 1] = __ffma2_rn(f[e], zero, check[e & 1]);
         }
         if (p.nsplit == 1) {
           // Through the tile's own query buffer (its last product has retired), so that rows leave
@@ -443,34 +525,40 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
             uint32_t u[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const __half2 ab = __floats2half2_rn(f[8 * g + 2 * x], f[8 * g + 2 * x + 1]);
+              const __half2 ab = __float22half2_rn(f[4 * g + x]);
               u[x] = *reinterpret_cast<const uint32_t *>(&ab);
             }
-            const int grp = (4 * c + g) & 7;
             *reinterpret_cast<uint4 *>(stage + (c >> 1) * (kRows * 128) + row * 128 +
-                                       ((grp ^ (row & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+                                       ((((4 * c + g) & 7) ^ (row & 7)) << 4)) =
+                make_uint4(u[0], u[1], u[2], u[3]);
           }
         } else if (live && any) {
 #pragma unroll
           for (int g = 0; g < 8; ++g)
-            if (32 * c + 4 * g < p.dim16)
+            if (g < 4 || 32 * c + 16 < p.dim16)
               *reinterpret_cast<float4 *>(part + 32 * c + 4 * g) =
-                  make_float4(f[4 * g], f[4 * g + 1], f[4 * g + 2], f[4 * g + 3]);
+                  make_float4(f[2 * g].x, f[2 * g].y, f[2 * g + 1].x, f[2 * g + 1].y);
         }
       }
+      const float chk = (check[0].x + check[0].y) + (check[1].x + check[1].y);
+      const bool odd = any && !(chk == 0.0f && l > 0.0f && l < INFINITY);
       float lse2 = any ? m + log2f(l) : -INFINITY;
       if (p.nsplit == 1) {
         __syncwarp();
+        // 8 or 16 lanes write a row; where it goes, its own lane knows.
+        __half *mine = p.out + (q0 + qi) * p.out_stride +
+                       static_cast<long long>(h * p.group + row % p.group) * p.head_dim;
+        if (!live) mine = nullptr;
         const int groups = p.head_dim / 8;
-        for (int x = lane; x < 32 * groups; x += 32) {
-          const int r = (row & ~31) + x / groups, grp = x % groups;
-          const int q = first + r / p.group;
-          if (r < p.tile_q * p.group && q < qlen)
-            *reinterpret_cast<uint4 *>(p.out + (q0 + q) * p.out_stride +
-                                       static_cast<long long>(h * p.group + r % p.group) * p.head_dim +
-                                       8 * grp) =
-                *reinterpret_cast<const uint4 *>(stage + (grp >> 3) * (kRows * 128) + r * 128 +
-                                                 (((grp & 7) ^ (r & 7)) << 4));
+        const int wide = DB == 1 ? 8 : 16, grp = lane % wide;
+#pragma unroll 4
+        for (int r0 = 0; r0 < 32; r0 += 32 / wide) {
+          const int r = r0 + lane / wide, rr = (row & ~31) + r;
+          __half *dst = reinterpret_cast<__half *>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), r));
+          if (dst && grp < groups)
+            *reinterpret_cast<uint4 *>(dst + 8 * grp) = *reinterpret_cast<const uint4 *>(
+                stage + (grp >> 3) * (kRows * 128) + rr * 128 + (((grp & 7) ^ (rr & 7)) << 4));
         }
       }
       __syncwarp();
@@ -512,7 +600,8 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     }
   }
   __syncthreads();
-  if (count > 0 && warp == kMmaWarp) {
+  if (warp == kMmaWarp) {
+    __syncwarp();
     ptx::tc_fence_after();
     ptx::tmem_dealloc<1>(tmem, Cfg::TMEM_COLS);
   }

@@ -75,11 +75,13 @@ struct OpWait {
 };
 __device__ __forceinline__ bool op_wait(uint32_t bar, uint32_t parity, const OpWait &w,
                                         unsigned site) {
-  if (ptx::mbar_try_wait(bar, parity)) return true;
+  // Polls without suspending: a suspended thread comes back late, which a chain of short waits
+  // (scores, weights, products) pays at every link.
+  if (ptx::mbar_test_wait(bar, parity)) return true;
   const uint64_t t0 = ptx::globaltimer();
   for (uint32_t n = 1;; ++n) {
-    if (ptx::mbar_try_wait(bar, parity)) return true;
-    if ((n & 15u) == 0) {
+    if (ptx::mbar_test_wait(bar, parity)) return true;
+    if ((n & 255u) == 0) {
       if (*w.abort_flag) return false;
       if (ptx::globaltimer() - t0 > w.timeout_ns) {
         atomicCAS(w.status_word, 0u, 0x100u | site);
