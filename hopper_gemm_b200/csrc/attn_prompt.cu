@@ -87,31 +87,39 @@ constexpr int kSmemLimit = 232448;
 // output is rescaled only when the maximum has grown past it. 2^8 times a weight below 1 stays far
 // inside binary16, and the fp32 sums do not care.
 constexpr float kLag = 8.0f;
-constexpr int kPolyEvery = 4;
+constexpr int kPolyEvery = 1000;
 
 // DB: 64-element blocks of head_dim in shared memory (head_dim <= 64 DB); TILES: row tiles of a CTA,
-// each with its own four softmax warps.
+// each with its own eight softmax warps, two to a quarter of the rows: one for the first 64 keys of a block,
+// one for the others. (With one warp for all 128 keys a block's softmax took 2300 cycles, twice what its
+// exponentials cost: one warp's instructions depend on each other too often to fill a scheduler.)
 template <int DB, int TILES>
 struct AttnCfg {
   static constexpr int TILE_BYTES = DB * kRows * 128;  // queries of a tile, or keys / values of a block
   static constexpr int CTAS = TILES == 1 ? 2 : 1;      // per SM
-  // One warpgroup loads and issues; its registers go to the softmax warps, which hold a row of
-  // scores each (LAUNCH_REGS x the warpgroups is what the shares add up to).
-  static constexpr int THREADS = (TILES + 1) * 128;
-  static constexpr int LAUNCH_REGS = TILES == 2 ? 168 : 128;
-  static constexpr int ISSUE_REGS = 56;
-  static constexpr int SOFTMAX_REGS = TILES == 2 ? 224 : 200;
-  static_assert(TILES * SOFTMAX_REGS + ISSUE_REGS == (TILES + 1) * LAUNCH_REGS, "register shares");
-  static constexpr int BUDGET = (kSmemLimit - (CTAS - 1) * 1024) / CTAS - 1024 - 256;
+  // One warpgroup loads and issues; its registers go to the softmax warps (LAUNCH_REGS x the
+  // warpgroups is what the shares add up to).
+  static constexpr int SOFTMAX_WARPS = TILES * 8;
+  static constexpr int THREADS = (TILES * 2 + 1) * 128;
+  static constexpr int LAUNCH_REGS = TILES == 2 ? 96 : 80;
+  static constexpr int ISSUE_REGS = TILES == 2 ? 64 : 48;
+  static constexpr int SOFTMAX_REGS = TILES == 2 ? 104 : 96;
+  static_assert(TILES * 2 * SOFTMAX_REGS + ISSUE_REGS == (TILES * 2 + 1) * LAUNCH_REGS,
+                "register shares");
+  // Barriers and the halves' exchange (HEAD bytes), then whole 1024-byte swizzle atoms.
+  static constexpr int BAR_BYTES = 256;
+  static constexpr int HEAD = (BAR_BYTES + TILES * 2 * kRows * 4 + 1023) / 1024 * 1024;
+  static constexpr int BUDGET = (kSmemLimit - (CTAS - 1) * 1024) / CTAS - HEAD;
   static constexpr int STAGES_FIT = (BUDGET - TILES * TILE_BYTES) / TILE_BYTES;
   static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
-  static constexpr int SMEM = 1024 + (TILES + STAGES) * TILE_BYTES + 256;
+  static constexpr int SMEM = HEAD + (TILES + STAGES) * TILE_BYTES;
   // TMEM columns: scores of each tile (the weights take the place of their first half), then the
   // outputs.
   static constexpr int O_COL = TILES * kKeys;
   static constexpr int TMEM_COLS = TILES == 2 ? 512 : 256;
   static_assert(STAGES >= 2, "a stage for keys and one for values");
   static_assert(O_COL + TILES * DB * 64 <= TMEM_COLS, "TMEM");
+  static_assert(8 * (2 * STAGES + 1 + 4 * TILES) + 32 <= BAR_BYTES, "barriers");
 };
 
 // Work of a CTA: a sequence and a tile of `span` queries in it.
@@ -191,17 +199,16 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
                 const __grid_constant__ CUtensorMap tmV, const AttnParams p) {
   using Cfg = AttnCfg<DB, TILES>;
   constexpr int S = Cfg::STAGES;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = ptx::smem_u32(smem_raw);
-  const uint32_t base = (raw + 1023u) & ~1023u;
-  uint8_t *smem = smem_raw + (base - raw);
-  const uint32_t sQ = base, sKV = base + TILES * Cfg::TILE_BYTES;
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (TILES + S) * Cfg::TILE_BYTES);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = ptx::smem_u32(smem);
+  const uint32_t sQ = base + Cfg::HEAD, sKV = sQ + TILES * Cfg::TILE_BYTES;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem);
+  float *swap = reinterpret_cast<float *>(smem + Cfg::BAR_BYTES);  // [TILES][2 halves][kRows]
   const uint32_t full = ptx::smem_u32(bars);          // [S] keys or values landed
   const uint32_t empty = full + 8 * S;                // [S] the products that read them are done
   const uint32_t qfull = empty + 8 * S;               // [1] queries landed
   const uint32_t sfull = qfull + 8;                   // [TILES] scores ready (and the last O product done)
-  const uint32_t pfull = sfull + 8 * TILES;           // [TILES][2] half of the weights ready (and O rescaled)
+  const uint32_t pfull = sfull + 8 * TILES;           // [TILES][2] part of the weights ready (and O rescaled)
   const uint32_t ofull = pfull + 16 * TILES;          // [TILES] output ready
   int *misc = reinterpret_cast<int *>(bars + 2 * S + 1 + 4 * TILES);
   volatile int *abort_flag = misc;
@@ -209,7 +216,11 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   Tile *found = reinterpret_cast<Tile *>(misc + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kLoadWarp = TILES * 4, kMmaWarp = TILES * 4 + 1;
+  if (base & 1023u) {  // swizzle atoms would be off (the declaration asks for this alignment)
+    if (threadIdx.x == 0) atomicCAS(p.status_word, 0u, 0x100u | kSiteAttnQ);
+    return;
+  }
+  constexpr int kLoadWarp = Cfg::SOFTMAX_WARPS, kMmaWarp = kLoadWarp + 1;
   const int h = blockIdx.x % p.heads_kv;
   const int split = (blockIdx.x / p.heads_kv) % p.nsplit;
   const int w = blockIdx.x / p.heads_kv / p.nsplit;
@@ -231,8 +242,8 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       ptx::mbar_init(qfull, 1);
       for (int i = 0; i < TILES; ++i) {
         ptx::mbar_init(sfull + 8 * i, 1);
-        ptx::mbar_init(pfull + 16 * i, 4);
-        ptx::mbar_init(pfull + 16 * i + 8, 4);
+        ptx::mbar_init(pfull + 16 * i, 8);
+        ptx::mbar_init(pfull + 16 * i + 8, 8);
         ptx::mbar_init(ofull + 8 * i, 1);
       }
       ptx::fence_mbar_init_cluster();
@@ -263,7 +274,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   const int count = max(count0, count1);
   OpWait wc{abort_flag, p.status_word, p.timeout_ns};
 
-  if (warp >= TILES * 4) {
+  if (warp >= Cfg::SOFTMAX_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::ISSUE_REGS));
     if (warp == kLoadWarp && lane == 0 && count > 0) {
       // Both tiles' queries in one transaction (a tile without blocks is not read).
@@ -321,15 +332,15 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
           ptx::umma_commit<1>(sfull + 8 * i);
         }
       };
-      // Half of a block's keys at a time, as the weights come.
-      auto output = [&](int i, int stage, bool first, int half) {
+      // Half of a block's keys at a time, as the weights come: the first or second 32 of each 64.
+      auto output = [&](int i, int stage, bool first, int part) {
         const uint64_t vd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES, kKeys * 128, 1024);
         if (one) {
 #pragma unroll
           for (int x = 0; x < kKeys / 32; ++x) {
-            const int k = half * (kKeys / 32) + x;
+            const int k = (x >> 1) * (kKeys / 32) + 2 * part + (x & 1);
             ptx::umma_f16_ts(tm + Cfg::O_COL + i * (DB * 64), tm + i * kKeys + 8 * k, vd + 128 * k,
-                             idesc_o, !(first && k == 0));
+                             idesc_o, !(first && part == 0 && x == 0));
           }
         }
       };
@@ -393,7 +404,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   } else {
     // ---------------------------------------------------------------- softmax warps
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::SOFTMAX_REGS));
-    const int i = warp >> 2;
+    const int i = warp >> 3, half = (warp >> 2) & 1;
     const int row = threadIdx.x & 127;
     const int first = qt * span + i * p.tile_q;
     const int n = i == 0 ? count0 : count1;
@@ -401,43 +412,46 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     const bool live = qt >= 0 && row < p.tile_q * p.group && qi < qlen;
     const int limit = p.causal ? max(0, min(klen, qi + 1 + klen - qlen)) : klen;
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp, lane << 16
-    const uint32_t tS = tmem + lane_base + i * kKeys;
-    const uint32_t tO = tmem + lane_base + Cfg::O_COL + i * (DB * 64);
+    const uint32_t tS = tmem + lane_base + i * kKeys + half * (kKeys / 2);
+    const uint32_t tP = tmem + lane_base + i * kKeys + half * (kKeys / 4);
+    // This warp's half of the output's columns.
+    constexpr int kOut = DB * 32;
+    const uint32_t tO = tmem + lane_base + Cfg::O_COL + i * (DB * 64) + half * kOut;
+    float *mine = swap + (2 * i + half) * kRows + row, *other = swap + (2 * i + (half ^ 1)) * kRows + row;
+    auto meet = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + i) : "memory"); };
     float m = -INFINITY;  // maximum that the weights are relative to (scaled)
-    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};  // of the weights, in four parts
+    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};  // of this half's weights
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       int okw = 1;
       if (lane == 0) okw = op_wait(sfull + 8 * i, j & 1, wc, kSiteAttnScores);
-      ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
-      if (!ok) break;
+      ok &= __shfl_sync(0xffffffffu, okw, 0) != 0;  // (both halves go on, so that they meet)
       ptx::tc_fence_after();
-      uint32_t sr[4][32];
+      uint32_t sr[2][32];
       ptx::tmem_ld_32x32b_x32(tS, sr[0]);
       ptx::tmem_ld_32x32b_x32(tS + 32, sr[1]);
       ptx::tmem_ld_wait();
-      ptx::tmem_ld_32x32b_x32(tS + 64, sr[2]);
-      ptx::tmem_ld_32x32b_x32(tS + 96, sr[3]);
-      const int left = limit - (b0 + j) * kKeys;  // keys of this block that the row sees
-      const bool cut = __any_sync(0xffffffffu, left < kKeys);
-      float mx[2] = {-INFINITY, -INFINITY};
-      auto mask_and_max = [&](int c) {
-        if (cut)
+      // Keys of this half block that the row sees.
+      const int left = limit - (b0 + j) * kKeys - half * (kKeys / 2);
+      if (__any_sync(0xffffffffu, left < kKeys / 2)) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (32 * c + e >= left) sr[c][e] = 0xff800000u;  // -infinity
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          mx[0] = max3(mx[0], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
-          mx[1] = max3(mx[1], __uint_as_float(sr[c][e + 2]), __uint_as_float(sr[c][e + 3]));
-        }
-      };
-      mask_and_max(0);
-      mask_and_max(1);
-      ptx::tmem_ld_wait();
-      mask_and_max(2);
-      mask_and_max(3);
-      const float top = fmaxf(mx[0], mx[1]) * p.scale2;
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+          mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
+      // The two halves of a row go by one maximum. Nobody writes weights over scores that are not
+      // loaded, nor a maximum over one that is not read: the next scores come behind both halves' weights.
+      const float part_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      *mine = part_max;
+      meet();
+      const float top = fmaxf(part_max, *other) * p.scale2;
       const bool grow = top > m + kLag;  // true of the first key, from -infinity
       const float m_old = m;
       if (grow) m = top;
@@ -448,45 +462,47 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         sum[0].y *= f;
         sum[1].x *= f;
         sum[1].y *= f;
-        for (int c = 0; c < DB * 2; ++c) {
-          uint32_t o[32];
-          ptx::tmem_ld_32x32b_x32(tO + 32 * c, o);
+#pragma unroll 1
+        for (int c = 0; c < kOut / 16; ++c) {
+          uint32_t o[16];
+          ptx::tmem_ld_32x32b_x16(tO + 16 * c, o);
           ptx::tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          ptx::tmem_st_32x32b_x32(tO + 32 * c, o);
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          ptx::tmem_st_32x32b_x16(tO + 16 * c, o);
         }
       }
       const float neg1 = m == -INFINITY ? 0.0f : -m;
       const float2 neg = make_float2(neg1, neg1), scale = make_float2(p.scale2, p.scale2);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w2[32];
+      for (int c = 0; c < 2; ++c) {
+        uint32_t w2[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int cc = 2 * half + (e >> 4), ee = (e & 15) * 2;
+        for (int e = 0; e < 16; ++e) {
           const float2 x = __ffma2_rn(
-              make_float2(__uint_as_float(sr[cc][ee]), __uint_as_float(sr[cc][ee + 1])), scale, neg);
+              make_float2(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])), scale, neg);
           // The special function unit would be as long at work as the tensor core; every kPolyEvery-th
           // pair goes through the FMA pipe instead.
           const float2 ab = (e % kPolyEvery == kPolyEvery - 1) ? ex2_poly(x)
                                                                 : make_float2(ex2(x.x), ex2(x.y));
           sum[e & 1] = __fadd2_rn(sum[e & 1], ab);
-          const __half2 h = __float22half2_rn(ab);
-          w2[e] = *reinterpret_cast<const uint32_t *>(&h);
+          const __half2 h2 = __float22half2_rn(ab);
+          w2[e] = *reinterpret_cast<const uint32_t *>(&h2);
         }
-        ptx::tmem_st_32x32b_x32(tS + 32 * half, w2);
+        ptx::tmem_st_32x32b_x16(tP + 16 * c, w2);
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(pfull + 16 * i + 8 * half);
+        if (lane == 0) ptx::mbar_arrive(pfull + 16 * i + 8 * c);
       }
     }
-    if (ok && n > 0) {
+    if (n > 0) {
       int okw = 1;
       if (lane == 0) okw = op_wait(ofull + 8 * i, 0, wc, kSiteAttnOut);
-      ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
+      ok &= __shfl_sync(0xffffffffu, okw, 0) != 0;
       ptx::tc_fence_after();
+      *mine = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      meet();
     }
     if (ok) {
       const int kb = b0 * kKeys;                                   // first key of this CTA
@@ -494,50 +510,49 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       const bool any = ke > kb;
       const long long orow =
           static_cast<long long>(q0 + qi) * p.heads_q + h * p.group + row % p.group;
-      const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      const float l = n > 0 ? swap[2 * i * kRows + row] + swap[(2 * i + 1) * kRows + row] : 0.0f;
       const float inv1 = any ? 1.0f / l : 0.0f;
       const float2 inv = make_float2(inv1, inv1), zero = make_float2(0.0f, 0.0f);
       const bool clear = !__all_sync(0xffffffffu, any);  // rows without a key: zeros, whatever stands in O
       float2 check[2] = {zero, zero};  // stays 0 with finite outputs, NaN otherwise
-      uint8_t *stage = smem + i * Cfg::TILE_BYTES;
+      uint8_t *stage = smem + Cfg::HEAD + i * Cfg::TILE_BYTES;
       float *part = p.part_o + (static_cast<long long>(split) * p.total_q * p.heads_q + orow) * p.dim16;
 #pragma unroll
-      for (int c = 0; c < DB * 2; ++c) {
-        if (32 * c >= p.dim16) break;
-        uint32_t o[32];
+      for (int c = 0; c < kOut / 16; ++c) {
+        const int col = half * kOut + 16 * c;
+        if (col >= p.dim16) break;
+        uint32_t o[16];
         if (n > 0) {
-          ptx::tmem_ld_32x32b_x32(tO + 32 * c, o);
+          ptx::tmem_ld_32x32b_x16(tO + 16 * c, o);
           ptx::tmem_ld_wait();
         }
-        float2 f[16];
+        float2 f[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 8; ++e) {
           f[e] = __fmul2_rn(make_float2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])), inv);
           if (clear && !any) f[e] = zero;
-          // (columns behind dim16 hold nothing)
-          if (e < 8 || 32 * c + 16 < p.dim16) check[e & 1] = __ffma2_rn(f[e], zero, check[e & 1]);
+          check[e & 1] = __ffma2_rn(f[e], zero, check[e & 1]);
         }
         if (p.nsplit == 1) {
           // Through the tile's own query buffer (its last product has retired), so that rows leave
           // in whole 16-byte groups next to each other.
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
+          for (int g = 0; g < 2; ++g) {
             uint32_t u[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const __half2 ab = __float22half2_rn(f[4 * g + x]);
               u[x] = *reinterpret_cast<const uint32_t *>(&ab);
             }
-            *reinterpret_cast<uint4 *>(stage + (c >> 1) * (kRows * 128) + row * 128 +
-                                       ((((4 * c + g) & 7) ^ (row & 7)) << 4)) =
-                make_uint4(u[0], u[1], u[2], u[3]);
+            const int grp = col / 8 + g;
+            *reinterpret_cast<uint4 *>(stage + (grp >> 3) * (kRows * 128) + row * 128 +
+                                       (((grp & 7) ^ (row & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
           }
         } else if (live && any) {
 #pragma unroll
-          for (int g = 0; g < 8; ++g)
-            if (g < 4 || 32 * c + 16 < p.dim16)
-              *reinterpret_cast<float4 *>(part + 32 * c + 4 * g) =
-                  make_float4(f[2 * g].x, f[2 * g].y, f[2 * g + 1].x, f[2 * g + 1].y);
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4 *>(part + col + 4 * g) =
+                make_float4(f[2 * g].x, f[2 * g].y, f[2 * g + 1].x, f[2 * g + 1].y);
         }
       }
       const float chk = (check[0].x + check[0].y) + (check[1].x + check[1].y);
@@ -545,18 +560,18 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       float lse2 = any ? m + log2f(l) : -INFINITY;
       if (p.nsplit == 1) {
         __syncwarp();
-        // 8 or 16 lanes write a row; where it goes, its own lane knows.
-        __half *mine = p.out + (q0 + qi) * p.out_stride +
-                       static_cast<long long>(h * p.group + row % p.group) * p.head_dim;
-        if (!live) mine = nullptr;
-        const int groups = p.head_dim / 8;
-        const int wide = DB == 1 ? 8 : 16, grp = lane % wide;
+        // A few lanes write this half of a row; where it goes, its own lane knows.
+        __half *to = p.out + (q0 + qi) * p.out_stride +
+                     static_cast<long long>(h * p.group + row % p.group) * p.head_dim;
+        if (!live) to = nullptr;
+        constexpr int wide = kOut / 8;
+        const int grp = half * wide + lane % wide;
 #pragma unroll 4
         for (int r0 = 0; r0 < 32; r0 += 32 / wide) {
           const int r = r0 + lane / wide, rr = (row & ~31) + r;
           __half *dst = reinterpret_cast<__half *>(
-              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), r));
-          if (dst && grp < groups)
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), r));
+          if (dst && 8 * grp < p.head_dim)
             *reinterpret_cast<uint4 *>(dst + 8 * grp) = *reinterpret_cast<const uint4 *>(
                 stage + (grp >> 3) * (kRows * 128) + rr * 128 + (((grp & 7) ^ (rr & 7)) << 4));
         }
@@ -574,7 +589,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
                  p.k + k0 * p.k_stride + static_cast<long long>(h) * p.head_dim,
                  p.v + k0 * p.v_stride + static_cast<long long>(h) * p.head_dim, kb, end, o, mr, lr);
         const float ir = 1.0f / lr;
-        if (4 * lane < p.head_dim) {
+        if (4 * lane < p.head_dim && 4 * lane / kOut == half) {
           if (p.nsplit == 1) {
             const __half2 a = __floats2half2_rn(o[0] * ir, o[1] * ir);
             const __half2 b = __floats2half2_rn(o[2] * ir, o[3] * ir);
@@ -591,7 +606,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         }
         if (lane == src) lse2 = mr + log2f(lr);
       }
-      if (live) {
+      if (live && half == 0) {
         if (p.nsplit > 1)
           p.part_lse[static_cast<long long>(split) * p.total_q * p.heads_q + orow] = lse2;
         else if (p.lse)
