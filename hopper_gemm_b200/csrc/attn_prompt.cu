@@ -81,45 +81,41 @@ __device__ void attn_row(const AttnParams &p, const __half *qrow, const __half *
 
 // ------------------------------------------------------------------------------ the kernel
 constexpr int kRows = 128;  // (query, head of the group) rows of a tile = TMEM lanes
-constexpr int kKeys = 128;  // keys of a block
+constexpr int kKeys = 128;  // keys of a load
+constexpr int kBlock = 64;  // keys of a block, the unit of the softmax and of the masks
 constexpr int kSmemLimit = 232448;
 // A row's weights are relative to a maximum that may lag the true one by this factor (log2): its
 // output is rescaled only when the maximum has grown past it. 2^8 times a weight below 1 stays far
 // inside binary16, and the fp32 sums do not care.
 constexpr float kLag = 8.0f;
-constexpr int kPolyEvery = 1000;
 
 // DB: 64-element blocks of head_dim in shared memory (head_dim <= 64 DB); TILES: row tiles of a CTA,
-// each with its own eight softmax warps, two to a quarter of the rows: one for the first 64 keys of a block,
-// one for the others. (With one warp for all 128 keys a block's softmax took 2300 cycles, twice what its
-// exponentials cost: one warp's instructions depend on each other too often to fill a scheduler.)
+// each with four softmax warps, a thread to a row.
+//
+// Keys are loaded 128 at a time and worked on 64 at a time, because a tile's scores then have two places
+// in TMEM: the next block's scores are formed while a block's softmax runs, and no tile ever waits
+// for the way from its weights through two products to its next scores. (With blocks of 128 keys in one
+// place that way, 1300 cycles, stood in a row with the softmax's 1600: 3800 cycles for two tiles
+// where the exponentials take 2100 and the products 2050.)
 template <int DB, int TILES>
 struct AttnCfg {
-  static constexpr int TILE_BYTES = DB * kRows * 128;  // queries of a tile, or keys / values of a block
+  static constexpr int TILE_BYTES = DB * kRows * 128;  // queries of a tile, or keys / values of a load
   static constexpr int CTAS = TILES == 1 ? 2 : 1;      // per SM
-  // One warpgroup loads and issues; its registers go to the softmax warps (LAUNCH_REGS x the
-  // warpgroups is what the shares add up to).
-  static constexpr int SOFTMAX_WARPS = TILES * 8;
-  static constexpr int THREADS = (TILES * 2 + 1) * 128;
-  static constexpr int LAUNCH_REGS = TILES == 2 ? 96 : 80;
-  static constexpr int ISSUE_REGS = TILES == 2 ? 64 : 48;
-  static constexpr int SOFTMAX_REGS = TILES == 2 ? 104 : 96;
-  static_assert(TILES * 2 * SOFTMAX_REGS + ISSUE_REGS == (TILES * 2 + 1) * LAUNCH_REGS,
-                "register shares");
-  // Barriers and the halves' exchange (HEAD bytes), then whole 1024-byte swizzle atoms.
-  static constexpr int BAR_BYTES = 256;
-  static constexpr int HEAD = (BAR_BYTES + TILES * 2 * kRows * 4 + 1023) / 1024 * 1024;
+  static constexpr int SOFTMAX_WARPS = TILES * 4;
+  static constexpr int THREADS = (SOFTMAX_WARPS + 2) * 32;
+  // Barriers, then whole 1024-byte swizzle atoms.
+  static constexpr int HEAD = 1024;
   static constexpr int BUDGET = (kSmemLimit - (CTAS - 1) * 1024) / CTAS - HEAD;
   static constexpr int STAGES_FIT = (BUDGET - TILES * TILE_BYTES) / TILE_BYTES;
   static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
   static constexpr int SMEM = HEAD + (TILES + STAGES) * TILE_BYTES;
-  // TMEM columns: scores of each tile (the weights take the place of their first half), then the
-  // outputs.
-  static constexpr int O_COL = TILES * kKeys;
+  // TMEM columns: two blocks of scores of each tile (the weights take the place of their first half),
+  // then the outputs.
+  static constexpr int O_COL = TILES * 2 * kBlock;
   static constexpr int TMEM_COLS = TILES == 2 ? 512 : 256;
   static_assert(STAGES >= 2, "a stage for keys and one for values");
   static_assert(O_COL + TILES * DB * 64 <= TMEM_COLS, "TMEM");
-  static_assert(8 * (2 * STAGES + 1 + 4 * TILES) + 32 <= BAR_BYTES, "barriers");
+  static_assert(8 * (2 * STAGES + 1 + 6 * TILES) + 32 <= HEAD, "barriers");
 };
 
 // Work of a CTA: a sequence and a tile of `span` queries in it.
@@ -167,26 +163,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 2^x for two values on the FMA pipe: x is cut into an integer n and f in [-1/2, 1/2] (Cody and
-// Waite), 2^f is a polynomial of degree 4 through 1 at 0 (fitted for the least relative error, 2.9e-6 in
-// fp32: 1/170 of the binary16 rounding that every weight gets), n goes into the exponent. Below
-// 2^-126 the result is some tiny value that rounds to zero; infinities and NaN leave as values that
-// overflow binary16, which the output's check sees.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
-  const float2 big = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: its ulp is 1
-  const float2 t = __fadd2_rn(x, big);
-  const float2 f = __fadd2_rn(x, __ffma2_rn(t, make_float2(-1.0f, -1.0f), big));
-  float2 r = __ffma2_rn(f, make_float2(9.582853e-3f, 9.582853e-3f),
-                        make_float2(5.5906425e-2f, 5.5906425e-2f));
-  r = __ffma2_rn(r, f, make_float2(2.4024099e-1f, 2.4024099e-1f));
-  r = __ffma2_rn(r, f, make_float2(6.9312419e-1f, 6.9312419e-1f));
-  r = __ffma2_rn(r, f, make_float2(1.0f, 1.0f));
-  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -203,14 +179,14 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   const uint32_t base = ptx::smem_u32(smem);
   const uint32_t sQ = base + Cfg::HEAD, sKV = sQ + TILES * Cfg::TILE_BYTES;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem);
-  float *swap = reinterpret_cast<float *>(smem + Cfg::BAR_BYTES);  // [TILES][2 halves][kRows]
   const uint32_t full = ptx::smem_u32(bars);          // [S] keys or values landed
   const uint32_t empty = full + 8 * S;                // [S] the products that read them are done
   const uint32_t qfull = empty + 8 * S;               // [1] queries landed
-  const uint32_t sfull = qfull + 8;                   // [TILES] scores ready (and the last O product done)
-  const uint32_t pfull = sfull + 8 * TILES;           // [TILES][2] part of the weights ready (and O rescaled)
-  const uint32_t ofull = pfull + 16 * TILES;          // [TILES] output ready
-  int *misc = reinterpret_cast<int *>(bars + 2 * S + 1 + 4 * TILES);
+  const uint32_t sfull = qfull + 8;                   // [TILES][2] scores ready
+  const uint32_t pfull = sfull + 16 * TILES;          // [TILES][2] weights ready (and O rescaled)
+  const uint32_t odone = pfull + 16 * TILES;          // [TILES] one more block is in the output
+  const uint32_t ofull = odone + 8 * TILES;           // [TILES] the last one is
+  int *misc = reinterpret_cast<int *>(bars + 2 * S + 1 + 6 * TILES);
   volatile int *abort_flag = misc;
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(misc + 1);
   Tile *found = reinterpret_cast<Tile *>(misc + 2);
@@ -240,12 +216,11 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         ptx::mbar_init(empty + 8 * i, 1);
       }
       ptx::mbar_init(qfull, 1);
-      for (int i = 0; i < TILES; ++i) {
+      for (int i = 0; i < 2 * TILES; ++i) {
         ptx::mbar_init(sfull + 8 * i, 1);
-        ptx::mbar_init(pfull + 16 * i, 8);
-        ptx::mbar_init(pfull + 16 * i + 8, 8);
-        ptx::mbar_init(ofull + 8 * i, 1);
+        ptx::mbar_init(pfull + 8 * i, 4);
       }
+      for (int i = 0; i < 2 * TILES; ++i) ptx::mbar_init(odone + 8 * i, 1);  // and ofull
       ptx::fence_mbar_init_cluster();
     }
   } else if (warp == kMmaWarp) {
@@ -258,13 +233,13 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(tmem_holder);
   const Tile work = *found;
   const int q0 = work.q0, qlen = work.qlen, k0 = work.k0, klen = work.klen, qt = work.tile;
-  // Blocks of keys that tile i needs: [0, need_i); this CTA's share is [b0, b0 + count_i).
+  // Blocks of 64 keys that tile i needs: [0, need_i); this CTA's share is [b0, b0 + count_i).
   auto need_of = [&](int i) {
     const int first = qt * span + i * p.tile_q;
     if (qt < 0 || first >= qlen) return 0;
     const int last = min(first + p.tile_q, qlen) - 1;
     const int seen = p.causal ? max(0, min(klen, last + 1 + klen - qlen)) : klen;
-    return (seen + kKeys - 1) / kKeys;
+    return (seen + kBlock - 1) / kBlock;
   };
   const int need = max(need_of(0), need_of(TILES - 1));
   const int per = (need + p.nsplit - 1) / p.nsplit;
@@ -272,11 +247,11 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   auto count_of = [&](int i) { return max(0, min(need_of(i) - b0, per)); };
   const int count0 = count_of(0), count1 = TILES == 2 ? count_of(1) : 0;
   const int count = max(count0, count1);
+  const int items = (count + 1) / 2 * 2;  // loads: keys, values, keys, ..
   OpWait wc{abort_flag, p.status_word, p.timeout_ns};
 
-  if (warp >= Cfg::SOFTMAX_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::ISSUE_REGS));
-    if (warp == kLoadWarp && lane == 0 && count > 0) {
+  if (warp == kLoadWarp) {
+    if (lane == 0 && count > 0) {
       // Both tiles' queries in one transaction (a tile without blocks is not read).
       ptx::mbar_arrive_expect_tx(qfull, ((count0 > 0) + (count1 > 0)) * DB * p.q_box_bytes);
       for (int i = 0; i < TILES; ++i)
@@ -286,14 +261,14 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
                              h * p.group, q0 + qt * span + i * p.tile_q);
       bool ok = true;
       int it = 0;
-      for (; it < 2 * count; ++it) {
+      for (; it < items; ++it) {
         const int st = it % S;
         if (it >= S && !op_wait(empty + 8 * st, (it / S - 1) & 1, wc, kSiteAttnKvEmpty)) {
           ok = false;
           break;
         }
         ptx::mbar_arrive_expect_tx(full + 8 * st, Cfg::TILE_BYTES);
-        const int row = k0 + (b0 + (it >> 1)) * kKeys;
+        const int row = k0 + b0 * kBlock + (it >> 1) * kKeys;
         for (int x = 0; x < DB; ++x)
           ptx::tma_load_3d((it & 1) ? &tmV : &tmK, sKV + st * Cfg::TILE_BYTES + x * (kKeys * 128),
                            full + 8 * st, 64 * x, h, row);
@@ -304,94 +279,91 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         for (int j = max(0, it - S); j < it; ++j) op_drain(full + 8 * (j % S), (j / S) & 1);
       }
     }
-    if (warp == kMmaWarp && count > 0) {
+  } else if (warp == kMmaWarp) {
+    if (count > 0) {
       // The whole warp walks the loop and one lane issues: descriptors then stay in uniform registers.
       // (Walked by one lane, a product took about 130 cycles to issue, twice its time on the tensor core.)
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint32_t idesc_s = ptx::umma_idesc_f16_f32(kRows, kKeys, true);
+      const uint32_t idesc_s = ptx::umma_idesc_f16_f32(kRows, kBlock, true);
       const uint32_t idesc_o = ptx::umma_idesc_f16_f32(kRows, p.dim16, false);
       const int ksteps = p.dim16 / 16;
       const bool one = ptx::elect_one();
-      bool ok = __all_sync(0xffffffffu, op_wait(qfull, 0, wc, kSiteAttnQ));
       auto wait = [&](uint32_t bar, int phase, unsigned site) {
         return __all_sync(0xffffffffu, op_wait(bar, phase & 1, wc, site)) != 0;
       };
       auto commit = [&](uint32_t bar) {
         if (one) ptx::umma_commit<1>(bar);
       };
-      auto scores = [&](int i, int stage) {
+      // Scores of tile i and a half of a load's keys, into place `half`.
+      auto scores = [&](int i, int stage, int half) {
         const uint64_t qd = ptx::umma_desc_sw128(sQ + i * Cfg::TILE_BYTES, 16, 1024);
-        const uint64_t kd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES, 16, 1024);
+        const uint64_t kd =
+            ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES + half * (kBlock * 128), 16, 1024);
         if (one) {
 #pragma unroll
           for (int k = 0; k < DB * 4; ++k) {
             // 16 elements are 32 bytes of a 128-byte row; the next 64 lie one block of 16 KB on.
             const uint64_t off = static_cast<uint64_t>((k >> 2) * (kRows * 128 / 16) + (k & 3) * 2);
-            if (k < ksteps) ptx::umma_f16<1>(tm + i * kKeys, qd + off, kd + off, idesc_s, k > 0);
+            if (k < ksteps)
+              ptx::umma_f16<1>(tm + (2 * i + half) * kBlock, qd + off, kd + off, idesc_s, k > 0);
           }
-          ptx::umma_commit<1>(sfull + 8 * i);
+          ptx::umma_commit<1>(sfull + 16 * i + 8 * half);
         }
       };
-      // Half of a block's keys at a time, as the weights come: the first or second 32 of each 64.
-      auto output = [&](int i, int stage, bool first, int part) {
-        const uint64_t vd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES, kKeys * 128, 1024);
+      auto output = [&](int i, int stage, int half, bool first, bool last) {
+        const uint64_t vd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES + half * (kBlock * 128),
+                                                 kKeys * 128, 1024);
         if (one) {
 #pragma unroll
-          for (int x = 0; x < kKeys / 32; ++x) {
-            const int k = (x >> 1) * (kKeys / 32) + 2 * part + (x & 1);
-            ptx::umma_f16_ts(tm + Cfg::O_COL + i * (DB * 64), tm + i * kKeys + 8 * k, vd + 128 * k,
-                             idesc_o, !(first && part == 0 && x == 0));
-          }
+          for (int k = 0; k < kBlock / 16; ++k)
+            ptx::umma_f16_ts(tm + Cfg::O_COL + i * (DB * 64), tm + (2 * i + half) * kBlock + 8 * k,
+                             vd + 128 * k, idesc_o, !(first && k == 0));
+          ptx::umma_commit<1>((last ? ofull : odone) + 8 * i);
         }
       };
-      if (ok) ok = wait(full, 0, kSiteAttnKvFull);
+      bool ok = wait(qfull, 0, kSiteAttnQ) && wait(full, 0, kSiteAttnKvFull);
       if (ok) {
         ptx::tc_fence_after();
 #pragma unroll
-        for (int i = 0; i < TILES; ++i)
-          if ((i == 0 ? count0 : count1) > 0) scores(i, 0);
-        if (S < 2 * count) commit(empty);
-      }
-      int vst = 1, vph = 0;  // stage and phase of block j's values; its successor's keys lie behind them
-#pragma unroll 1
-      for (int j = 0; ok && j < count; ++j) {
-        int kst = vst + 1, kph = vph;
-        if (kst == S) {
-          kst = 0;
-          kph ^= 1;
-        }
-        if (!(ok = wait(full + 8 * vst, vph, kSiteAttnKvFull))) break;
-        bool k_here = false;
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-          const int cnt = i == 0 ? count0 : count1;
-          if (!ok || j >= cnt) continue;
-          if (!(ok = wait(pfull + 16 * i, j, kSiteAttnWeights))) continue;
-          ptx::tc_fence_after();
-          output(i, vst, j == 0, 0);
-          if (!(ok = wait(pfull + 16 * i + 8, j, kSiteAttnWeights))) continue;
-          ptx::tc_fence_after();
-          output(i, vst, j == 0, 1);
-          if (j + 1 == cnt) {
-            commit(ofull + 8 * i);
-          } else {
-            if (!k_here && !(ok = wait(full + 8 * kst, kph, kSiteAttnKvFull))) continue;
-            k_here = true;
+          for (int i = 0; i < TILES; ++i)
+            if (half < (i == 0 ? count0 : count1)) scores(i, 0, half);
+        if (S < items) commit(empty);
+      }
+      // Stages and phases of the values of blocks u, u + 1 and of the keys of the two behind them.
+      int vst = 1, vph = 0, kst = 2 % S, kph = 2 / S;
+#pragma unroll 1
+      for (int u = 0; ok && u < count; u += 2) {
+        if (!(ok = wait(full + 8 * vst, vph, kSiteAttnKvFull))) break;
+        if (u + 2 < count && !(ok = wait(full + 8 * kst, kph, kSiteAttnKvFull))) break;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int i = 0; i < TILES; ++i) {
+            const int cnt = i == 0 ? count0 : count1;
+            if (!ok || u + half >= cnt) continue;
+            if (!(ok = wait(pfull + 16 * i + 8 * half, u >> 1, kSiteAttnWeights))) continue;
             ptx::tc_fence_after();
-            // Issued behind the product that reads this tile's weights, whose columns it overwrites;
-            // the tensor core works in issue order.
-            scores(i, kst);
+            output(i, vst, half, u + half == 0, u + half + 1 == cnt);
+            // Behind the product that reads the weights in the place that these scores take; the
+            // tensor core works in issue order.
+            if (u + half + 2 < cnt) scores(i, kst, half);
           }
         }
         if (!ok) break;
         // A stage that nothing is loaded into any more is not announced: no arrival outlives the CTA.
-        if (2 * j + 1 + S < 2 * count) commit(empty + 8 * vst);
-        if (2 * j + 2 + S < 2 * count) commit(empty + 8 * kst);
-        vst = kst + 1;
-        vph = kph;
-        if (vst == S) {
-          vst = 0;
+        if (u + 1 + S < items) commit(empty + 8 * vst);
+        if (u + 2 + S < items) commit(empty + 8 * kst);
+        vst += 2;
+        if (vst >= S) {
+          vst -= S;
           vph ^= 1;
+        }
+        kst += 2;
+        if (kst >= S) {
+          kst -= S;
+          kph ^= 1;
         }
       }
       if (!ok) {
@@ -403,8 +375,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     }
   } else {
     // ---------------------------------------------------------------- softmax warps
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::SOFTMAX_REGS));
-    const int i = warp >> 3, half = (warp >> 2) & 1;
+    const int i = warp >> 2;
     const int row = threadIdx.x & 127;
     const int first = qt * span + i * p.tile_q;
     const int n = i == 0 ? count0 : count1;
@@ -412,28 +383,28 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     const bool live = qt >= 0 && row < p.tile_q * p.group && qi < qlen;
     const int limit = p.causal ? max(0, min(klen, qi + 1 + klen - qlen)) : klen;
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp, lane << 16
-    const uint32_t tS = tmem + lane_base + i * kKeys + half * (kKeys / 2);
-    const uint32_t tP = tmem + lane_base + i * kKeys + half * (kKeys / 4);
-    // This warp's half of the output's columns.
-    constexpr int kOut = DB * 32;
-    const uint32_t tO = tmem + lane_base + Cfg::O_COL + i * (DB * 64) + half * kOut;
-    float *mine = swap + (2 * i + half) * kRows + row, *other = swap + (2 * i + (half ^ 1)) * kRows + row;
-    auto meet = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + i) : "memory"); };
+    const uint32_t tS = tmem + lane_base + i * (2 * kBlock);
+    const uint32_t tO = tmem + lane_base + Cfg::O_COL + i * (DB * 64);
     float m = -INFINITY;  // maximum that the weights are relative to (scaled)
-    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};  // of this half's weights
+    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};  // of the weights, in four parts
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
+    auto wait = [&](uint32_t bar, int phase, unsigned site) {
       int okw = 1;
-      if (lane == 0) okw = op_wait(sfull + 8 * i, j & 1, wc, kSiteAttnScores);
-      ok &= __shfl_sync(0xffffffffu, okw, 0) != 0;  // (both halves go on, so that they meet)
+      if (lane == 0) okw = op_wait(bar, phase & 1, wc, site);
+      okw = __shfl_sync(0xffffffffu, okw, 0);
       ptx::tc_fence_after();
+      return okw != 0;
+    };
+#pragma unroll 1
+    for (int u = 0; u < n; ++u) {
+      const uint32_t place = tS + (u & 1) * kBlock;
+      if (!(ok = wait(sfull + 16 * i + 8 * (u & 1), u >> 1, kSiteAttnScores))) break;
       uint32_t sr[2][32];
-      ptx::tmem_ld_32x32b_x32(tS, sr[0]);
-      ptx::tmem_ld_32x32b_x32(tS + 32, sr[1]);
+      ptx::tmem_ld_32x32b_x32(place, sr[0]);
+      ptx::tmem_ld_32x32b_x32(place + 32, sr[1]);
       ptx::tmem_ld_wait();
-      // Keys of this half block that the row sees.
-      const int left = limit - (b0 + j) * kKeys - half * (kKeys / 2);
-      if (__any_sync(0xffffffffu, left < kKeys / 2)) {
+      const int left = limit - (b0 + u) * kBlock;  // keys of this block that the row sees
+      if (__any_sync(0xffffffffu, left < kBlock)) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -446,24 +417,21 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
 #pragma unroll
         for (int e = 0; e < 32; e += 2)
           mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
-      // The two halves of a row go by one maximum. Nobody writes weights over scores that are not
-      // loaded, nor a maximum over one that is not read: the next scores come behind both halves' weights.
-      const float part_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      *mine = part_max;
-      meet();
-      const float top = fmaxf(part_max, *other) * p.scale2;
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2;
       const bool grow = top > m + kLag;  // true of the first key, from -infinity
       const float m_old = m;
       if (grow) m = top;
-      if (j > 0 && __any_sync(0xffffffffu, grow)) {
-        // The scores of block j were committed behind block j - 1's product, so O is at rest.
+      if (u > 0 && __any_sync(0xffffffffu, grow)) {
+        // O comes to rest with the block before. (The one before that was done when these scores were
+        // formed and this one is not begun, so the phase is one of two and its parity tells which.)
+        if (!(ok = wait(odone + 8 * i, u - 1, kSiteAttnOut))) break;
         const float f = (grow && m_old != -INFINITY) ? ex2(m_old - m) : 1.0f;
         sum[0].x *= f;
         sum[0].y *= f;
         sum[1].x *= f;
         sum[1].y *= f;
 #pragma unroll 1
-        for (int c = 0; c < kOut / 16; ++c) {
+        for (int c = 0; c < DB * 4; ++c) {
           uint32_t o[16];
           ptx::tmem_ld_32x32b_x16(tO + 16 * c, o);
           ptx::tmem_ld_wait();
@@ -481,36 +449,26 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         for (int e = 0; e < 16; ++e) {
           const float2 x = __ffma2_rn(
               make_float2(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])), scale, neg);
-          // The special function unit would be as long at work as the tensor core; every kPolyEvery-th
-          // pair goes through the FMA pipe instead.
-          const float2 ab = (e % kPolyEvery == kPolyEvery - 1) ? ex2_poly(x)
-                                                                : make_float2(ex2(x.x), ex2(x.y));
+          const float2 ab = make_float2(ex2(x.x), ex2(x.y));
           sum[e & 1] = __fadd2_rn(sum[e & 1], ab);
           const __half2 h2 = __float22half2_rn(ab);
           w2[e] = *reinterpret_cast<const uint32_t *>(&h2);
         }
-        ptx::tmem_st_32x32b_x16(tP + 16 * c, w2);
-        ptx::tmem_st_wait();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(pfull + 16 * i + 8 * c);
+        ptx::tmem_st_32x32b_x16(place + 16 * c, w2);
       }
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(pfull + 16 * i + 8 * (u & 1));
     }
-    if (n > 0) {
-      int okw = 1;
-      if (lane == 0) okw = op_wait(ofull + 8 * i, 0, wc, kSiteAttnOut);
-      ok &= __shfl_sync(0xffffffffu, okw, 0) != 0;
-      ptx::tc_fence_after();
-      *mine = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-      meet();
-    }
+    if (ok && n > 0) ok = wait(ofull + 8 * i, 0, kSiteAttnOut);
     if (ok) {
-      const int kb = b0 * kKeys;                                   // first key of this CTA
-      const int ke = min(limit, kb + n * kKeys);                   // behind the last that the row sees
+      const int kb = b0 * kBlock;                                  // first key of this CTA
+      const int ke = min(limit, kb + n * kBlock);                  // behind the last that the row sees
       const bool any = ke > kb;
       const long long orow =
           static_cast<long long>(q0 + qi) * p.heads_q + h * p.group + row % p.group;
-      const float l = n > 0 ? swap[2 * i * kRows + row] + swap[(2 * i + 1) * kRows + row] : 0.0f;
+      const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       const float inv1 = any ? 1.0f / l : 0.0f;
       const float2 inv = make_float2(inv1, inv1), zero = make_float2(0.0f, 0.0f);
       const bool clear = !__all_sync(0xffffffffu, any);  // rows without a key: zeros, whatever stands in O
@@ -518,41 +476,43 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       uint8_t *stage = smem + Cfg::HEAD + i * Cfg::TILE_BYTES;
       float *part = p.part_o + (static_cast<long long>(split) * p.total_q * p.heads_q + orow) * p.dim16;
 #pragma unroll
-      for (int c = 0; c < kOut / 16; ++c) {
-        const int col = half * kOut + 16 * c;
+      for (int c = 0; c < DB * 2; ++c) {
+        const int col = 32 * c;
         if (col >= p.dim16) break;
-        uint32_t o[16];
+        uint32_t o[32];
         if (n > 0) {
-          ptx::tmem_ld_32x32b_x16(tO + 16 * c, o);
+          ptx::tmem_ld_32x32b_x32(tO + col, o);
           ptx::tmem_ld_wait();
         }
-        float2 f[8];
+        float2 f[16];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 16; ++e) {
           f[e] = __fmul2_rn(make_float2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])), inv);
           if (clear && !any) f[e] = zero;
-          check[e & 1] = __ffma2_rn(f[e], zero, check[e & 1]);
+          // (columns behind dim16 hold nothing)
+          if (e < 8 || col + 16 < p.dim16) check[e & 1] = __ffma2_rn(f[e], zero, check[e & 1]);
         }
         if (p.nsplit == 1) {
           // Through the tile's own query buffer (its last product has retired), so that rows leave
           // in whole 16-byte groups next to each other.
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            uint32_t u[4];
+          for (int g = 0; g < 4; ++g) {
+            uint32_t w[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const __half2 ab = __float22half2_rn(f[4 * g + x]);
-              u[x] = *reinterpret_cast<const uint32_t *>(&ab);
+              w[x] = *reinterpret_cast<const uint32_t *>(&ab);
             }
             const int grp = col / 8 + g;
             *reinterpret_cast<uint4 *>(stage + (grp >> 3) * (kRows * 128) + row * 128 +
-                                       (((grp & 7) ^ (row & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+                                       (((grp & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else if (live && any) {
 #pragma unroll
-          for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4 *>(part + col + 4 * g) =
-                make_float4(f[2 * g].x, f[2 * g].y, f[2 * g + 1].x, f[2 * g + 1].y);
+          for (int g = 0; g < 8; ++g)
+            if (g < 4 || col + 16 < p.dim16)
+              *reinterpret_cast<float4 *>(part + col + 4 * g) =
+                  make_float4(f[2 * g].x, f[2 * g].y, f[2 * g + 1].x, f[2 * g + 1].y);
         }
       }
       const float chk = (check[0].x + check[0].y) + (check[1].x + check[1].y);
@@ -560,12 +520,12 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       float lse2 = any ? m + log2f(l) : -INFINITY;
       if (p.nsplit == 1) {
         __syncwarp();
-        // A few lanes write this half of a row; where it goes, its own lane knows.
+        // 8 or 16 lanes write a row; where it goes, its own lane knows.
         __half *to = p.out + (q0 + qi) * p.out_stride +
                      static_cast<long long>(h * p.group + row % p.group) * p.head_dim;
         if (!live) to = nullptr;
-        constexpr int wide = kOut / 8;
-        const int grp = half * wide + lane % wide;
+        constexpr int wide = DB * 8;
+        const int grp = lane % wide;
 #pragma unroll 4
         for (int r0 = 0; r0 < 32; r0 += 32 / wide) {
           const int r = r0 + lane / wide, rr = (row & ~31) + r;
@@ -589,7 +549,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
                  p.k + k0 * p.k_stride + static_cast<long long>(h) * p.head_dim,
                  p.v + k0 * p.v_stride + static_cast<long long>(h) * p.head_dim, kb, end, o, mr, lr);
         const float ir = 1.0f / lr;
-        if (4 * lane < p.head_dim && 4 * lane / kOut == half) {
+        if (4 * lane < p.head_dim) {
           if (p.nsplit == 1) {
             const __half2 a = __floats2half2_rn(o[0] * ir, o[1] * ir);
             const __half2 b = __floats2half2_rn(o[2] * ir, o[3] * ir);
@@ -606,7 +566,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         }
         if (lane == src) lse2 = mr + log2f(lr);
       }
-      if (live && half == 0) {
+      if (live) {
         if (p.nsplit > 1)
           p.part_lse[static_cast<long long>(split) * p.total_q * p.heads_q + orow] = lse2;
         else if (p.lse)
