@@ -102,7 +102,7 @@ struct AttnCfg {
   static constexpr int TILE_BYTES = DB * kRows * 128;  // queries of a tile, or keys / values of a load
   static constexpr int CTAS = TILES == 1 ? 2 : 1;      // per SM
   static constexpr int SOFTMAX_WARPS = TILES * 4;
-  static constexpr int THREADS = (SOFTMAX_WARPS + 2) * 32;
+  static constexpr int THREADS = (SOFTMAX_WARPS + 2 + TILES) * 32;  // ... loads of keys, of values, products
   // Barriers, then whole 1024-byte swizzle atoms.
   static constexpr int HEAD = 1024;
   static constexpr int BUDGET = (kSmemLimit - (CTAS - 1) * 1024) / CTAS - HEAD;
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   const uint32_t qfull = empty + 8 * S;               // [1] queries landed
   const uint32_t sfull = qfull + 8;                   // [TILES][2] scores ready
   const uint32_t pfull = sfull + 16 * TILES;          // [TILES][2] weights ready (and O rescaled)
-  const uint32_t odone = pfull + 16 * TILES;          // [TILES] one more block is in the output
+  const uint32_t odone = pfull + 16 * TILES;          // [TILES] the last block but one is in the output
   const uint32_t ofull = odone + 8 * TILES;           // [TILES] the last one is
   int *misc = reinterpret_cast<int *>(bars + 2 * S + 1 + 6 * TILES);
   volatile int *abort_flag = misc;
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     if (threadIdx.x == 0) atomicCAS(p.status_word, 0u, 0x100u | kSiteAttnQ);
     return;
   }
-  constexpr int kLoadWarp = Cfg::SOFTMAX_WARPS, kMmaWarp = kLoadWarp + 1;
+  constexpr int kLoadWarp = Cfg::SOFTMAX_WARPS, kMmaWarp = kLoadWarp + 2;
   const int h = blockIdx.x % p.heads_kv;
   const int split = (blockIdx.x / p.heads_kv) % p.nsplit;
   const int w = blockIdx.x / p.heads_kv / p.nsplit;
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       *abort_flag = 0;
       for (int i = 0; i < S; ++i) {
         ptx::mbar_init(full + 8 * i, 1);
-        ptx::mbar_init(empty + 8 * i, 1);
+        ptx::mbar_init(empty + 8 * i, TILES);
       }
       ptx::mbar_init(qfull, 1);
       for (int i = 0; i < 2 * TILES; ++i) {
@@ -250,40 +250,53 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   const int items = (count + 1) / 2 * 2;  // loads: keys, values, keys, ..
   OpWait wc{abort_flag, p.status_word, p.timeout_ns};
 
-  if (warp == kLoadWarp) {
-    if (lane == 0 && count > 0) {
-      // Both tiles' queries in one transaction (a tile without blocks is not read).
-      ptx::mbar_arrive_expect_tx(qfull, ((count0 > 0) + (count1 > 0)) * DB * p.q_box_bytes);
-      for (int i = 0; i < TILES; ++i)
-        if ((i == 0 ? count0 : count1) > 0)
-          for (int x = 0; x < DB; ++x)
-            ptx::tma_load_3d(&tmQ, sQ + i * Cfg::TILE_BYTES + x * (kRows * 128), qfull, 64 * x,
-                             h * p.group, q0 + qt * span + i * p.tile_q);
-      bool ok = true;
-      int it = 0;
-      for (; it < items; ++it) {
-        const int st = it % S;
-        if (it >= S && !op_wait(empty + 8 * st, (it / S - 1) & 1, wc, kSiteAttnKvEmpty)) {
-          ok = false;
-          break;
-        }
-        ptx::mbar_arrive_expect_tx(full + 8 * st, Cfg::TILE_BYTES);
-        const int row = k0 + b0 * kBlock + (it >> 1) * kKeys;
-        for (int x = 0; x < DB; ++x)
-          ptx::tma_load_3d((it & 1) ? &tmV : &tmK, sKV + st * Cfg::TILE_BYTES + x * (kKeys * 128),
-                           full + 8 * st, 64 * x, h, row);
-      }
-      if (!ok) {
-        // Unwinding: the loads in flight land before the CTA may exit.
-        op_drain(qfull, 0);
-        for (int j = max(0, it - S); j < it; ++j) op_drain(full + 8 * (j % S), (j / S) & 1);
-      }
-    }
-  } else if (warp == kMmaWarp) {
+  if (warp == kLoadWarp || warp == kLoadWarp + 1) {
+    // A warp for the keys (and queries), one for the values, a lane for each 64-element block: a thread
+    // is held about 400 cycles by a TMA load, and one thread for all of them kept the products waiting.
+    const bool values = warp != kLoadWarp;
     if (count > 0) {
-      // The whole warp walks the loop and one lane issues: descriptors then stay in uniform registers.
-      // (Walked by one lane, a product took about 130 cycles to issue, twice its time on the tensor core.)
+      if (!values) {
+        // Both tiles' queries in one transaction (a tile without blocks is not read).
+        if (lane == 0)
+          ptx::mbar_arrive_expect_tx(qfull, ((count0 > 0) + (count1 > 0)) * DB * p.q_box_bytes);
+        __syncwarp();
+        const int i = lane / DB, x = lane % DB;
+        if (i < TILES && (i == 0 ? count0 : count1) > 0)
+          ptx::tma_load_3d(&tmQ, sQ + i * Cfg::TILE_BYTES + x * (kRows * 128), qfull, 64 * x,
+                           h * p.group, q0 + qt * span + i * p.tile_q);
+      }
+      const CUtensorMap *map = values ? &tmV : &tmK;
+      bool ok = true;
+      int it = values ? 1 : 0;
+      for (; it < items; it += 2) {
+        const int st = it % S;
+        int okw = 1;
+        if (lane == 0) {
+          if (it >= S) okw = op_wait(empty + 8 * st, (it / S - 1) & 1, wc, kSiteAttnKvEmpty);
+          if (okw) ptx::mbar_arrive_expect_tx(full + 8 * st, Cfg::TILE_BYTES);
+        }
+        ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
+        if (!ok) break;
+        if (lane < DB)
+          ptx::tma_load_3d(map, sKV + st * Cfg::TILE_BYTES + lane * (kKeys * 128), full + 8 * st,
+                           64 * lane, h, k0 + b0 * kBlock + (it >> 1) * kKeys);
+      }
+      if (!ok && lane == 0) {
+        // Unwinding: the loads in flight land before the CTA may exit.
+        if (!values) op_drain(qfull, 0);
+        for (int j = max(it & 1, it - 2 * S); j < it; j += 2) op_drain(full + 8 * (j % S), (j / S) & 1);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= kMmaWarp) {
+    if (count > 0) {
+      // A warp for each tile's products, so that one's waits lie under the other's work. The whole warp
+      // walks the loop and one lane issues: descriptors then stay in uniform registers. (Walked by one
+      // lane, a product took about 130 cycles to issue, twice its time on the tensor core.)
+      const int i = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0);
+      const int cnt = i == 0 ? count0 : count1;
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t tmS = tm + 2 * i * kBlock, tmO = tm + Cfg::O_COL + i * (DB * 64);
       const uint32_t idesc_s = ptx::umma_idesc_f16_f32(kRows, kBlock, true);
       const uint32_t idesc_o = ptx::umma_idesc_f16_f32(kRows, p.dim16, false);
       const int ksteps = p.dim16 / 16;
@@ -294,9 +307,9 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       auto commit = [&](uint32_t bar) {
         if (one) ptx::umma_commit<1>(bar);
       };
-      // Scores of tile i and a half of a load's keys, into place `half`.
-      auto scores = [&](int i, int stage, int half) {
-        const uint64_t qd = ptx::umma_desc_sw128(sQ + i * Cfg::TILE_BYTES, 16, 1024);
+      // Scores of a half of a load's keys, into place `half`.
+      const uint64_t qd = ptx::umma_desc_sw128(sQ + i * Cfg::TILE_BYTES, 16, 1024);
+      auto scores = [&](int stage, int half) {
         const uint64_t kd =
             ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES + half * (kBlock * 128), 16, 1024);
         if (one) {
@@ -304,34 +317,29 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
           for (int k = 0; k < DB * 4; ++k) {
             // 16 elements are 32 bytes of a 128-byte row; the next 64 lie one block of 16 KB on.
             const uint64_t off = static_cast<uint64_t>((k >> 2) * (kRows * 128 / 16) + (k & 3) * 2);
-            if (k < ksteps)
-              ptx::umma_f16<1>(tm + (2 * i + half) * kBlock, qd + off, kd + off, idesc_s, k > 0);
+            if (k < ksteps) ptx::umma_f16<1>(tmS + half * kBlock, qd + off, kd + off, idesc_s, k > 0);
           }
           ptx::umma_commit<1>(sfull + 16 * i + 8 * half);
         }
       };
-      auto output = [&](int i, int stage, int half, bool first, bool last) {
+      auto output = [&](int stage, int half, bool first) {
         const uint64_t vd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES + half * (kBlock * 128),
                                                  kKeys * 128, 1024);
         if (one) {
 #pragma unroll
           for (int k = 0; k < kBlock / 16; ++k)
-            ptx::umma_f16_ts(tm + Cfg::O_COL + i * (DB * 64), tm + (2 * i + half) * kBlock + 8 * k,
-                             vd + 128 * k, idesc_o, !(first && k == 0));
-          ptx::umma_commit<1>((last ? ofull : odone) + 8 * i);
+            ptx::umma_f16_ts(tmO, tmS + half * kBlock + 8 * k, vd + 128 * k, idesc_o, !(first && k == 0));
         }
       };
       bool ok = wait(qfull, 0, kSiteAttnQ) && wait(full, 0, kSiteAttnKvFull);
       if (ok) {
         ptx::tc_fence_after();
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int i = 0; i < TILES; ++i)
-            if (half < (i == 0 ? count0 : count1)) scores(i, 0, half);
+        if (cnt > 0) scores(0, 0);
+        if (cnt > 1) scores(0, 1);
         if (S < items) commit(empty);
       }
-      // Stages and phases of the values of blocks u, u + 1 and of the keys of the two behind them.
+      // Stages and phases of the values of blocks u, u + 1 and of the keys of the two behind them. A warp
+      // whose tile is through goes on to wait for the loads: it gives a stage back once a load, not sooner.
       int vst = 1, vph = 0, kst = 2 % S, kph = 2 / S;
 #pragma unroll 1
       for (int u = 0; ok && u < count; u += 2) {
@@ -339,17 +347,16 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         if (u + 2 < count && !(ok = wait(full + 8 * kst, kph, kSiteAttnKvFull))) break;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-#pragma unroll
-          for (int i = 0; i < TILES; ++i) {
-            const int cnt = i == 0 ? count0 : count1;
-            if (!ok || u + half >= cnt) continue;
-            if (!(ok = wait(pfull + 16 * i + 8 * half, u >> 1, kSiteAttnWeights))) continue;
-            ptx::tc_fence_after();
-            output(i, vst, half, u + half == 0, u + half + 1 == cnt);
-            // Behind the product that reads the weights in the place that these scores take; the
-            // tensor core works in issue order.
-            if (u + half + 2 < cnt) scores(i, kst, half);
-          }
+          if (!ok || u + half >= cnt) continue;
+          if (!(ok = wait(pfull + 16 * i + 8 * half, u >> 1, kSiteAttnWeights))) continue;
+          ptx::tc_fence_after();
+          output(vst, half, u + half == 0);
+          // The next scores come behind the product that reads the weights in their place (the tensor
+          // core works in issue order), and their announcement tells of that product too.
+          if (u + half + 2 < cnt)
+            scores(kst, half);
+          else
+            commit((u + half + 1 == cnt ? ofull : odone) + 8 * i);
         }
         if (!ok) break;
         // A stage that nothing is loaded into any more is not announced: no arrival outlives the CTA.
@@ -368,8 +375,8 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       }
       if (!ok) {
         // Unwinding: every product retires before TMEM is freed.
-        commit(qfull);
-        op_drain(qfull, 1);
+        commit(ofull + 8 * i);
+        op_drain(ofull + 8 * i, 0);
       }
       __syncwarp();
     }
@@ -422,9 +429,10 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       const float m_old = m;
       if (grow) m = top;
       if (u > 0 && __any_sync(0xffffffffu, grow)) {
-        // O comes to rest with the block before. (The one before that was done when these scores were
-        // formed and this one is not begun, so the phase is one of two and its parity tells which.)
-        if (!(ok = wait(odone + 8 * i, u - 1, kSiteAttnOut))) break;
+        // O comes to rest with the block before: the scores behind this block's are formed after it.
+        if (!(ok = u + 1 < n ? wait(sfull + 16 * i + 8 * ((u + 1) & 1), (u + 1) >> 1, kSiteAttnScores)
+                             : wait(odone + 8 * i, 0, kSiteAttnOut)))
+          break;
         const float f = (grow && m_old != -INFINITY) ? ex2(m_old - m) : 1.0f;
         sum[0].x *= f;
         sum[0].y *= f;
