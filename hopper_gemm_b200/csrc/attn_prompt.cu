@@ -23,9 +23,11 @@ struct AttnParams {
   int dim16;         // head_dim rounded up to 16
   int tile_q;        // queries of a row tile (each with the group's heads)
   int q_box_bytes;   // bytes of one 64-element block of a tile's queries
-  int nsplit;        // key ranges of a row tile, joined by attn_join_kernel when there are several
-  float *part_o;     // nsplit x total_q x heads_q x dim16, each range's own weighted mean
-  float *part_lse;   // nsplit x total_q x heads_q, log2 of each range's sum
+  // Blocks of a key range and the most ranges of a sequence; chunk 0: no ranges. With ranges a row's parts
+  // are joined by attn_join_kernel.
+  int chunk, max_chunks;
+  float *part_o;     // max_chunks x total_q x heads_q x dim16, each range's own weighted mean
+  float *part_lse;   // max_chunks x total_q x heads_q, log2 of each range's sum
   unsigned *status_word;
   unsigned long long timeout_ns;
 };
@@ -81,9 +83,10 @@ __device__ void attn_row(const AttnParams &p, const __half *qrow, const __half *
 
 // ------------------------------------------------------------------------------ the kernel
 constexpr int kRows = 128;  // (query, head of the group) rows of a tile = TMEM lanes
-constexpr int kKeys = 128;  // keys of a load
 constexpr int kBlock = 64;  // keys of a block, the unit of the softmax and of the masks
 constexpr int kSmemLimit = 232448;
+constexpr int kSms = 148;        // what plans (and with them workspaces) reckon with
+constexpr int kMaxChunks = 64;   // key ranges of a sequence
 // A row's weights are relative to a maximum that may lag the true one by this factor (log2): its
 // output is rescaled only when the maximum has grown past it. 2^8 times a weight below 1 stays far
 // inside binary16, and the fp32 sums do not care.
@@ -92,49 +95,64 @@ constexpr float kLag = 8.0f;
 // DB: 64-element blocks of head_dim in shared memory (head_dim <= 64 DB); TILES: row tiles of a CTA,
 // each with four softmax warps, a thread to a row.
 //
-// Keys are loaded 128 at a time and worked on 64 at a time, because a tile's scores then have two places
-// in TMEM: the next block's scores are formed while a block's softmax runs, and no tile ever waits
-// for the way from its weights through two products to its next scores. (With blocks of 128 keys in one
-// place that way, 1300 cycles, stood in a row with the softmax's 1600: 3800 cycles for two tiles
-// where the exponentials take 2100 and the products 2050.)
+// Blocks of 64 keys, because a tile's scores then have two places in TMEM: the next block's scores are
+// formed while a block's softmax runs, and no tile ever waits for the way from its weights through two
+// products to its next scores. (With blocks of 128 keys in one place that way, 1300 cycles, stood in a
+// row with the softmax's 1600: 3800 cycles for two tiles and 128 keys, where the exponentials take 2100 and the
+// products 2050.)
 template <int DB, int TILES>
 struct AttnCfg {
-  static constexpr int TILE_BYTES = DB * kRows * 128;  // queries of a tile, or keys / values of a load
+  static constexpr int TILE_BYTES = DB * kRows * 128;   // queries of a tile
+  // Blocks of a load. One CTA to an SM has the stages for two at a time, which takes half the loads and
+  // announcements (16384 tokens: 1.89 ms against 2.04); two CTAs do not (141 us against 125 for 16 tokens
+  // over long keys, with one).
+  static constexpr int LOAD = TILES;
+  static constexpr int LOAD_ROWS = LOAD * kBlock;
+  static constexpr int LOAD_BYTES = DB * LOAD_ROWS * 128;
   static constexpr int CTAS = TILES == 1 ? 2 : 1;      // per SM
   static constexpr int SOFTMAX_WARPS = TILES * 4;
   static constexpr int THREADS = (SOFTMAX_WARPS + 2 + TILES) * 32;  // ... loads of keys, of values, products
   // Barriers, then whole 1024-byte swizzle atoms.
   static constexpr int HEAD = 1024;
   static constexpr int BUDGET = (kSmemLimit - (CTAS - 1) * 1024) / CTAS - HEAD;
-  static constexpr int STAGES_FIT = (BUDGET - TILES * TILE_BYTES) / TILE_BYTES;
-  static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
-  static constexpr int SMEM = HEAD + (TILES + STAGES) * TILE_BYTES;
+  static constexpr int STAGES_FIT = (BUDGET - TILES * TILE_BYTES) / LOAD_BYTES;
+  static constexpr int STAGES = STAGES_FIT > 10 ? 10 : STAGES_FIT;
+  static constexpr int SMEM = HEAD + TILES * TILE_BYTES + STAGES * LOAD_BYTES;
   // TMEM columns: two blocks of scores of each tile (the weights take the place of their first half),
   // then the outputs.
   static constexpr int O_COL = TILES * 2 * kBlock;
   static constexpr int TMEM_COLS = TILES == 2 ? 512 : 256;
-  static_assert(STAGES >= 2, "a stage for keys and one for values");
+  static_assert(STAGES * LOAD >= 4, "the keys of two blocks, the values of two");
   static_assert(O_COL + TILES * DB * 64 <= TMEM_COLS, "TMEM");
   static_assert(8 * (2 * STAGES + 1 + 6 * TILES) + 32 <= HEAD, "barriers");
 };
 
-// Work of a CTA: a sequence and a tile of `span` queries in it.
+// Key ranges of a sequence with klen keys.
+__device__ __forceinline__ int chunks_of(const AttnParams &p, int klen) {
+  if (p.chunk == 0) return 1;
+  const int blocks = (klen + kBlock - 1) / kBlock;
+  return min(max((blocks + p.chunk - 1) / p.chunk, 1), p.max_chunks);
+}
+
+// Work of a CTA: a sequence, a tile of `span` queries in it and a range of its keys.
 struct Tile {
   int q0, qlen, k0, klen;
   int tile;  // -1: none (the grid is an upper bound)
+  int chunk;
 };
 
-// Tile w of all sequences one after the other, the last tile (with the most keys to see) of each first, by
+// Item w of all sequences one after the other, the last tile (with the most keys to see) of each first, by
 // one warp: 32 sequences at a time, with one round trip to memory for all of their four starts.
 __device__ __forceinline__ Tile find_tile(const AttnParams &p, int w, int span) {
   const int lane = threadIdx.x & 31;
-  Tile t = {0, 0, 0, 0, -1};
+  Tile t = {0, 0, 0, 0, -1, 0};
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    int q0 = 0, q1 = 0, k0 = 0, k1 = 0, n = 0;
+    int q0 = 0, q1 = 0, k0 = 0, k1 = 0, n = 0, chunks = 1;
     if (b0 + lane < p.batch) {
       seq_range(p.cu_q, b0 + lane, p.total_q, q0, q1);
       seq_range(p.cu_k, b0 + lane, p.total_k, k0, k1);
-      n = (q1 - q0 + span - 1) / span;
+      chunks = chunks_of(p, k1 - k0);
+      n = (q1 - q0 + span - 1) / span * chunks;
     }
     int sum = n;
 #pragma unroll
@@ -149,7 +167,10 @@ __device__ __forceinline__ Tile find_tile(const AttnParams &p, int w, int span) 
       t.qlen = __shfl_sync(0xffffffffu, q1, src) - t.q0;
       t.k0 = __shfl_sync(0xffffffffu, k0, src);
       t.klen = __shfl_sync(0xffffffffu, k1, src) - t.k0;
-      t.tile = __shfl_sync(0xffffffffu, sum, src) - 1 - w;
+      const int back = __shfl_sync(0xffffffffu, sum, src) - 1 - w;
+      chunks = __shfl_sync(0xffffffffu, chunks, src);
+      t.tile = back / chunks;
+      t.chunk = back % chunks;
       return t;
     }
     w -= __shfl_sync(0xffffffffu, sum, 31);
@@ -198,8 +219,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   }
   constexpr int kLoadWarp = Cfg::SOFTMAX_WARPS, kMmaWarp = kLoadWarp + 2;
   const int h = blockIdx.x % p.heads_kv;
-  const int split = (blockIdx.x / p.heads_kv) % p.nsplit;
-  const int w = blockIdx.x / p.heads_kv / p.nsplit;
+  const int w = blockIdx.x / p.heads_kv;
   const int span = TILES * p.tile_q;  // queries of this CTA
 
   if (warp == 0) {
@@ -242,12 +262,13 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     return (seen + kBlock - 1) / kBlock;
   };
   const int need = max(need_of(0), need_of(TILES - 1));
-  const int per = (need + p.nsplit - 1) / p.nsplit;
-  const int b0 = split * per;
+  const bool whole = p.chunk == 0;
+  const int per = whole ? need : p.chunk;
+  const int split = work.chunk, b0 = split * per;
   auto count_of = [&](int i) { return max(0, min(need_of(i) - b0, per)); };
   const int count0 = count_of(0), count1 = TILES == 2 ? count_of(1) : 0;
   const int count = max(count0, count1);
-  const int items = (count + 1) / 2 * 2;  // loads: keys, values, keys, ..
+  const int items = (count + Cfg::LOAD - 1) / Cfg::LOAD * 2;  // loads: keys, values, keys, ..
   OpWait wc{abort_flag, p.status_word, p.timeout_ns};
 
   if (warp == kLoadWarp || warp == kLoadWarp + 1) {
@@ -273,13 +294,13 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         int okw = 1;
         if (lane == 0) {
           if (it >= S) okw = op_wait(empty + 8 * st, (it / S - 1) & 1, wc, kSiteAttnKvEmpty);
-          if (okw) ptx::mbar_arrive_expect_tx(full + 8 * st, Cfg::TILE_BYTES);
+          if (okw) ptx::mbar_arrive_expect_tx(full + 8 * st, Cfg::LOAD_BYTES);
         }
         ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
         if (!ok) break;
         if (lane < DB)
-          ptx::tma_load_3d(map, sKV + st * Cfg::TILE_BYTES + lane * (kKeys * 128), full + 8 * st,
-                           64 * lane, h, k0 + b0 * kBlock + (it >> 1) * kKeys);
+          ptx::tma_load_3d(map, sKV + st * Cfg::LOAD_BYTES + lane * (Cfg::LOAD_ROWS * 128), full + 8 * st,
+                           64 * lane, h, k0 + b0 * kBlock + (it >> 1) * Cfg::LOAD_ROWS);
       }
       if (!ok && lane == 0) {
         // Unwinding: the loads in flight land before the CTA may exit.
@@ -307,70 +328,92 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       auto commit = [&](uint32_t bar) {
         if (one) ptx::umma_commit<1>(bar);
       };
-      // Scores of a half of a load's keys, into place `half`.
+      // Scores of a block, into one of their two places; a 16-element step is 32 bytes of a 128-byte row,
+      // the next 64 elements lie a block of rows on.
       const uint64_t qd = ptx::umma_desc_sw128(sQ + i * Cfg::TILE_BYTES, 16, 1024);
-      auto scores = [&](int stage, int half) {
+      auto scores = [&](int stage, int sub, int place) {
         const uint64_t kd =
-            ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES + half * (kBlock * 128), 16, 1024);
+            ptx::umma_desc_sw128(sKV + stage * Cfg::LOAD_BYTES + sub * (kBlock * 128), 16, 1024);
         if (one) {
 #pragma unroll
-          for (int k = 0; k < DB * 4; ++k) {
-            // 16 elements are 32 bytes of a 128-byte row; the next 64 lie one block of 16 KB on.
-            const uint64_t off = static_cast<uint64_t>((k >> 2) * (kRows * 128 / 16) + (k & 3) * 2);
-            if (k < ksteps) ptx::umma_f16<1>(tmS + half * kBlock, qd + off, kd + off, idesc_s, k > 0);
-          }
-          ptx::umma_commit<1>(sfull + 16 * i + 8 * half);
+          for (int k = 0; k < DB * 4; ++k)
+            if (k < ksteps)
+              ptx::umma_f16<1>(tmS + place * kBlock, qd + (k >> 2) * (kRows * 128 / 16) + (k & 3) * 2,
+                               kd + (k >> 2) * (Cfg::LOAD_ROWS * 128 / 16) + (k & 3) * 2, idesc_s, k > 0);
+          ptx::umma_commit<1>(sfull + 16 * i + 8 * place);
         }
       };
-      auto output = [&](int stage, int half, bool first) {
-        const uint64_t vd = ptx::umma_desc_sw128(sKV + stage * Cfg::TILE_BYTES + half * (kBlock * 128),
-                                                 kKeys * 128, 1024);
+      auto output = [&](int stage, int sub, int place, bool first) {
+        const uint64_t vd = ptx::umma_desc_sw128(sKV + stage * Cfg::LOAD_BYTES + sub * (kBlock * 128),
+                                                 Cfg::LOAD_ROWS * 128, 1024);
         if (one) {
 #pragma unroll
           for (int k = 0; k < kBlock / 16; ++k)
-            ptx::umma_f16_ts(tmO, tmS + half * kBlock + 8 * k, vd + 128 * k, idesc_o, !(first && k == 0));
+            ptx::umma_f16_ts(tmO, tmS + place * kBlock + 8 * k, vd + 128 * k, idesc_o, !(first && k == 0));
         }
       };
-      bool ok = wait(qfull, 0, kSiteAttnQ) && wait(full, 0, kSiteAttnKvFull);
+      // Load `item` lies in stage item % S; it is waited for and given back once by either tile's warp,
+      // whether its tile needs it or not (a warp that is through must not give back a stage's next load
+      // before this one is there). A stage that nothing is loaded into any more is not announced: no
+      // arrival outlives the CTA.
+      int st = 0, ph = 0;  // of the next item
+      auto arrived = [&](int step) {
+        int x = st + step, y = ph;
+        if (x >= S) {
+          x -= S;
+          y ^= 1;
+        }
+        return wait(full + 8 * x, y, kSiteAttnKvFull);
+      };
+      auto give_back = [&](int item, int stage) {
+        if (item + S < items) commit(empty + 8 * stage);
+      };
+      constexpr int LOAD = Cfg::LOAD;
+      auto last_of_load = [&](int u) { return u % LOAD == LOAD - 1 || u + 1 == count; };
+      bool ok = wait(qfull, 0, kSiteAttnQ) && arrived(0);
       if (ok) {
         ptx::tc_fence_after();
-        if (cnt > 0) scores(0, 0);
-        if (cnt > 1) scores(0, 1);
-        if (S < items) commit(empty);
-      }
-      // Stages and phases of the values of blocks u, u + 1 and of the keys of the two behind them. A warp
-      // whose tile is through goes on to wait for the loads: it gives a stage back once a load, not sooner.
-      int vst = 1, vph = 0, kst = 2 % S, kph = 2 / S;
-#pragma unroll 1
-      for (int u = 0; ok && u < count; u += 2) {
-        if (!(ok = wait(full + 8 * vst, vph, kSiteAttnKvFull))) break;
-        if (u + 2 < count && !(ok = wait(full + 8 * kst, kph, kSiteAttnKvFull))) break;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (!ok || u + half >= cnt) continue;
-          if (!(ok = wait(pfull + 16 * i + 8 * half, u >> 1, kSiteAttnWeights))) continue;
+        if (cnt > 0) scores(0, 0, 0);
+        if (last_of_load(0)) give_back(0, 0);
+        constexpr int k1 = 2 * (1 / LOAD);  // load with the keys of block 1
+        if (count > 1 && (ok = arrived(k1))) {
           ptx::tc_fence_after();
-          output(vst, half, u + half == 0);
+          if (cnt > 1) scores(k1, 1 % LOAD, 1);
+          if (last_of_load(1)) give_back(k1, k1);
+        }
+      }
+      st = 1;
+#pragma unroll 1
+      for (int u = 0; ok && u < count; ++u) {
+        // The values of block u are load 2 (u / LOAD) + 1, at st; the keys of block u + 2 a few further.
+        const int item = u / LOAD * 2 + 1;
+        if (u % LOAD == 0 && !(ok = arrived(0))) break;
+        const int place = u & 1;
+        if (u < cnt) {
+          if (!(ok = wait(pfull + 16 * i + 8 * place, u >> 1, kSiteAttnWeights))) break;
+          ptx::tc_fence_after();
+          output(st, u % LOAD, place, u == 0);
+          if (u + 2 >= cnt) commit((u + 1 == cnt ? ofull : odone) + 8 * i);
+        }
+        if (last_of_load(u)) give_back(item, st);
+        if (u + 2 < count) {
+          constexpr int ahead = LOAD == 1 ? 3 : 1;
+          if (u % LOAD == 0 && !(ok = arrived(ahead))) break;
+          const int ks = st + ahead >= S ? st + ahead - S : st + ahead;
           // The next scores come behind the product that reads the weights in their place (the tensor
           // core works in issue order), and their announcement tells of that product too.
-          if (u + half + 2 < cnt)
-            scores(kst, half);
-          else
-            commit((u + half + 1 == cnt ? ofull : odone) + 8 * i);
+          if (u + 2 < cnt) {
+            ptx::tc_fence_after();
+            scores(ks, u % LOAD, place);
+          }
+          if (last_of_load(u + 2)) give_back(item + ahead, ks);
         }
-        if (!ok) break;
-        // A stage that nothing is loaded into any more is not announced: no arrival outlives the CTA.
-        if (u + 1 + S < items) commit(empty + 8 * vst);
-        if (u + 2 + S < items) commit(empty + 8 * kst);
-        vst += 2;
-        if (vst >= S) {
-          vst -= S;
-          vph ^= 1;
-        }
-        kst += 2;
-        if (kst >= S) {
-          kst -= S;
-          kph ^= 1;
+        if (u % LOAD == LOAD - 1) {
+          st += 2;
+          if (st >= S) {
+            st -= S;
+            ph ^= 1;
+          }
         }
       }
       if (!ok) {
@@ -500,7 +543,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
           // (columns behind dim16 hold nothing)
           if (e < 8 || col + 16 < p.dim16) check[e & 1] = __ffma2_rn(f[e], zero, check[e & 1]);
         }
-        if (p.nsplit == 1) {
+        if (whole) {
           // Through the tile's own query buffer (its last product has retired), so that rows leave
           // in whole 16-byte groups next to each other.
 #pragma unroll
@@ -526,7 +569,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       const float chk = (check[0].x + check[0].y) + (check[1].x + check[1].y);
       const bool odd = any && !(chk == 0.0f && l > 0.0f && l < INFINITY);
       float lse2 = any ? m + log2f(l) : -INFINITY;
-      if (p.nsplit == 1) {
+      if (whole) {
         __syncwarp();
         // 8 or 16 lanes write a row; where it goes, its own lane knows.
         __half *to = p.out + (q0 + qi) * p.out_stride +
@@ -558,7 +601,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
                  p.v + k0 * p.v_stride + static_cast<long long>(h) * p.head_dim, kb, end, o, mr, lr);
         const float ir = 1.0f / lr;
         if (4 * lane < p.head_dim) {
-          if (p.nsplit == 1) {
+          if (whole) {
             const __half2 a = __floats2half2_rn(o[0] * ir, o[1] * ir);
             const __half2 b = __floats2half2_rn(o[2] * ir, o[3] * ir);
             *reinterpret_cast<uint2 *>(p.out + (q0 + q) * p.out_stride +
@@ -575,7 +618,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         if (lane == src) lse2 = mr + log2f(lr);
       }
       if (live) {
-        if (p.nsplit > 1)
+        if (!whole)
           p.part_lse[static_cast<long long>(split) * p.total_q * p.heads_q + orow] = lse2;
         else if (p.lse)
           p.lse[orow] = lse2 * 0.69314718055994530942f;
@@ -597,33 +640,52 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
   const int i = static_cast<int>(row / p.heads_q), h = static_cast<int>(row % p.heads_q);
-  // Rows of no sequence hold nothing and are left as they were.
-  int in = 0;
+  // Ranges of the row's sequence; rows of no sequence hold nothing and are left as they were.
+  int mine = 0;
   for (int b = lane; b < p.batch; b += 32) {
-    int q0, q1;
+    int q0, q1, k0, k1;
     seq_range(p.cu_q, b, p.total_q, q0, q1);
-    in |= i >= q0 && i < q1;
+    seq_range(p.cu_k, b, p.total_k, k0, k1);
+    if (i >= q0 && i < q1) mine = chunks_of(p, k1 - k0);
   }
-  if (!__any_sync(0xffffffffu, in)) return;
-  float top = -INFINITY;
-  for (int c = 0; c < p.nsplit; ++c) {
-    const float z = p.part_lse[c * rows + row];
-    top = z != z ? z : fmaxf(top, z);  // a NaN stays
-    if (z != z) break;
+  const int chunks = __reduce_max_sync(0xffffffffu, mine);
+  if (chunks == 0) return;
+  // A lane holds the sums of ranges lane, lane + 32, .. .
+  constexpr int kEach = kMaxChunks / 32;
+  float z[kEach], top = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int x = 0; x < kEach; ++x) {
+    const int c = lane + 32 * x;
+    z[x] = c < chunks ? p.part_lse[c * rows + row] : -INFINITY;
+    nan |= z[x] != z[x];
+    top = fmaxf(top, z[x]);
   }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  if (__any_sync(0xffffffffu, nan)) top = __int_as_float(0x7fffffff);
   float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
   if (top != -INFINITY) {
-    for (int c = 0; c < p.nsplit; ++c) {
-      const float z = p.part_lse[c * rows + row];
-      if (z == -INFINITY) continue;
-      const float f = z == top ? 1.0f : exp2f(z - top);
-      l += f;
-      if (4 * lane < p.head_dim) {
-        const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (c * rows + row) * p.dim16 + 4 * lane);
-        o[0] = fmaf(f, v.x, o[0]);
-        o[1] = fmaf(f, v.y, o[1]);
-        o[2] = fmaf(f, v.z, o[2]);
-        o[3] = fmaf(f, v.w, o[3]);
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+      if (32 * x >= chunks) break;
+      const float f = z[x] == -INFINITY ? 0.0f : z[x] == top ? 1.0f : exp2f(z[x] - top);
+      const unsigned used = __ballot_sync(0xffffffffu, z[x] != -INFINITY);
+      const int end = min(32, chunks - 32 * x);
+#pragma unroll 8
+      for (int c = 0; c < end; ++c) {
+        // (a range without keys for this row has written no output)
+        const float fc = __shfl_sync(0xffffffffu, f, c);
+        if (((used >> c) & 1u) == 0) continue;
+        l += fc;
+        if (4 * lane < p.head_dim) {
+          const float4 v = *reinterpret_cast<const float4 *>(
+              p.part_o + ((c + 32 * x) * rows + row) * p.dim16 + 4 * lane);
+          o[0] = fmaf(fc, v.x, o[0]);
+          o[1] = fmaf(fc, v.y, o[1]);
+          o[2] = fmaf(fc, v.z, o[2]);
+          o[3] = fmaf(fc, v.w, o[3]);
+        }
       }
     }
   }
@@ -643,8 +705,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
 struct AttnPlan {
   int tiles;       // row tiles of a CTA
   int tile_q;      // queries of a row tile
-  int max_tiles;   // upper bound of the CTAs' query ranges
-  int nsplit;      // key ranges
+  int chunk, max_chunks;
+  long long items;  // upper bound of (tile, key range) pairs of all sequences
   size_t workspace;
 };
 
@@ -652,22 +714,38 @@ AttnPlan make_plan(int total_q, int total_k, int batch, int heads_q, int heads_k
   AttnPlan pl;
   const int group = heads_q / heads_kv;
   pl.tile_q = kRows / group;
-  const int avg_q = (total_q + batch - 1) / batch;
-  pl.tiles = avg_q <= pl.tile_q ? 1 : 2;
+  const long long avg_q = (total_q + batch - 1) / batch, avg_k = (total_k + batch - 1) / batch;
+  // Two row tiles to a CTA share the loaded keys, one tile each to two CTAs of an SM lets one's start
+  // and end lie under the other's work: measured equal near 6000 keys a sequence at head_dim 128 (4 x 2048
+  // tokens 174 and 166 us, 8192 tokens 475 and 495, 16384 tokens 1.89 and 2.06 ms), in favour of
+  // one tile at head_dim 64 up to 8192.
+  pl.tiles = head_dim > 64 && avg_k >= 6144 && avg_q > pl.tile_q ? 2 : 1;
   const int span = pl.tiles * pl.tile_q;
-  pl.max_tiles = static_cast<int>(
-      std::min<long long>(total_q, total_q / span + static_cast<long long>(batch)));
-  const long long units = static_cast<long long>(pl.max_tiles) * heads_kv;
-  const int slots = 148 * (pl.tiles == 1 ? 2 : 1);
-  const int blocks = (static_cast<int>((static_cast<long long>(total_k) + batch - 1) / batch) + kKeys - 1) / kKeys;
-  pl.nsplit = 1;
-  if (units < slots) {
-    pl.nsplit = static_cast<int>(std::min<long long>((2 * slots + units - 1) / units, blocks / 4));
-    pl.nsplit = std::max(1, std::min(pl.nsplit, 64));
+  const long long max_tiles = std::min<long long>(total_q, total_q / span + static_cast<long long>(batch));
+  // Key ranges where there are few tiles: of single tokens (whose lengths set the pace) up to two
+  // waves of CTAs, of prompts up to half a wave, beyond which writing and joining the parts costs more
+  // than the idle SMs. About four ranges to a CTA slot, of 1024 keys at least.
+  const long long slots = kSms * (pl.tiles == 1 ? 2 : 1);
+  const long long est_tiles = std::max<long long>((total_q + span - 1) / span, batch);
+  const long long units = est_tiles * heads_kv;
+  const long long blocks = total_k / kBlock + static_cast<long long>(batch);  // >= those of all sequences
+  pl.chunk = 0;
+  pl.max_chunks = 1;
+  pl.items = max_tiles;
+  if (avg_q <= pl.tile_q ? units < 2 * slots : 2 * units <= slots) {
+    const long long work = units * blocks / batch;
+    long long chunk = std::max<long long>(16, (work + 4 * slots - 1) / (4 * slots));
+    chunk = std::max(chunk, (blocks + kMaxChunks - 1) / kMaxChunks);
+    const long long chunks = (blocks + chunk - 1) / chunk;
+    if (chunks > 1) {
+      pl.chunk = static_cast<int>(chunk);
+      pl.max_chunks = static_cast<int>(chunks);
+      pl.items = max_tiles + (total_q + span - 1) / span * chunks;
+    }
   }
   pl.workspace = 0;
-  if (pl.nsplit > 1) {
-    const size_t rows = static_cast<size_t>(pl.nsplit) * total_q * heads_q;
+  if (pl.chunk > 0) {
+    const size_t rows = static_cast<size_t>(pl.max_chunks) * total_q * heads_q;
     pl.workspace = rows * ((head_dim + 15) / 16 * 16) * sizeof(float) + rows * sizeof(float);
   }
   return pl;
@@ -746,9 +824,10 @@ int run(const hgemm_attn_prompt_t *a, cudaStream_t stream) {
   const AttnPlan pl = make_plan(a->total_q, a->total_k, a->batch, a->heads_q, a->heads_kv, a->head_dim);
   p.tile_q = pl.tile_q;
   p.q_box_bytes = pl.tile_q * p.group * 128;
-  p.nsplit = pl.nsplit;
+  p.chunk = pl.chunk;
+  p.max_chunks = pl.max_chunks;
   p.part_o = static_cast<float *>(a->workspace);
-  p.part_lse = p.part_o + static_cast<size_t>(pl.nsplit) * a->total_q * a->heads_q * p.dim16;
+  p.part_lse = p.part_o + static_cast<size_t>(pl.max_chunks) * a->total_q * a->heads_q * p.dim16;
 
   CUtensorMap tq, tk, tv;
   auto encode = [&](CUtensorMap *map, const void *ptr, int heads, int rows, long long stride,
@@ -764,20 +843,19 @@ int run(const hgemm_attn_prompt_t *a, cudaStream_t stream) {
   if (!encode(&tq, a->q, a->heads_q, a->total_q, a->q_stride, p.group, pl.tile_q))
     return HGEMM_ERR_TENSOR_MAP;
   if (a->total_k > 0) {
-    if (!encode(&tk, a->k, a->heads_kv, a->total_k, a->k_stride, 1, kKeys) ||
-        !encode(&tv, a->v, a->heads_kv, a->total_k, a->v_stride, 1, kKeys))
+    if (!encode(&tk, a->k, a->heads_kv, a->total_k, a->k_stride, 1, pl.tiles * kBlock) ||
+        !encode(&tv, a->v, a->heads_kv, a->total_k, a->v_stride, 1, pl.tiles * kBlock))
       return HGEMM_ERR_TENSOR_MAP;
   } else {
     tk = tv = tq;  // no key: never loaded from
   }
-  const long long ctas = static_cast<long long>(pl.max_tiles) * a->heads_kv * pl.nsplit;
+  const long long ctas = pl.items * a->heads_kv;
   const long long joins = (static_cast<long long>(a->total_q) * a->heads_q + 7) / 8;
   if (ctas > 0x7fffffffll || joins > 0x7fffffffll) return HGEMM_ERR_TOO_LARGE;
-  st = a->head_dim <= 64 ? (pl.tiles == 1 ? launch<1, 1>(tq, tk, tv, p, d, ctas, stream)
-                                          : launch<1, 2>(tq, tk, tv, p, d, ctas, stream))
-                         : (pl.tiles == 1 ? launch<2, 1>(tq, tk, tv, p, d, ctas, stream)
-                                          : launch<2, 2>(tq, tk, tv, p, d, ctas, stream));
-  if (st != HGEMM_OK || pl.nsplit == 1) return st;
+  st = a->head_dim <= 64 ? launch<1, 1>(tq, tk, tv, p, d, ctas, stream)
+       : pl.tiles == 1   ? launch<2, 1>(tq, tk, tv, p, d, ctas, stream)
+                         : launch<2, 2>(tq, tk, tv, p, d, ctas, stream);
+  if (st != HGEMM_OK || pl.chunk == 0) return st;
   attn_join_kernel<<<static_cast<unsigned>(joins), 256, 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_LAUNCH;
 }
