@@ -164,7 +164,7 @@ struct PeerMaps {
 // Additional k-blocks of a row tile (see LoraExt in ops_sm100.cuh), as the kernel takes them.
 struct alignas(64) ExtArgs : PeerMaps {
   CUtensorMap tmLow;  // rows of `low`, 64 columns
-  CUtensorMap tmUp;   // N, rank, adapters
+  CUtensorMap tmUp;   // N, rank, adapters; with KParams::b4 as encode_b4's view of B and adapters
   const int *base, *count, *adapter;
   int chunks;
   unsigned *odd_count;
@@ -454,16 +454,23 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
                 ptx::tma_load_2d_pair(&peers.tmLow, dA, fbar, 0, lrow);
               else
                 ptx::tma_load_2d(&peers.tmLow, dA, fbar, 0, lrow);
+              if (p.b4) {
+                if (PAIR == 2)
+                  ptx::tma_load_5d_pair(&peers.tmUp, dB, fbar, 0, chunk * BK, bcol / 64, 0, adapter);
+                else
+                  ptx::tma_load_5d(&peers.tmUp, dB, fbar, 0, chunk * BK, bcol / 64, 0, adapter);
+              } else {
 #pragma unroll
-              for (int j = 0; j < Cfg::N_SUB; ++j) {
+                for (int j = 0; j < Cfg::N_SUB; ++j) {
 #pragma unroll
-                for (int b = 0; b < Cfg::SUB_BOXES; ++b) {
-                  const uint32_t dst = dB + static_cast<uint32_t>(j * Cfg::SUB_BOXES + b) * (BK * 128);
-                  const int col = bcol + j * Cfg::UMMA_N + 64 * b;
-                  if (PAIR == 2)
-                    ptx::tma_load_3d_pair(&peers.tmUp, dst, fbar, col, chunk * BK, adapter);
-                  else
-                    ptx::tma_load_3d(&peers.tmUp, dst, fbar, col, chunk * BK, adapter);
+                  for (int b = 0; b < Cfg::SUB_BOXES; ++b) {
+                    const uint32_t dst = dB + static_cast<uint32_t>(j * Cfg::SUB_BOXES + b) * (BK * 128);
+                    const int col = bcol + j * Cfg::UMMA_N + 64 * b;
+                    if (PAIR == 2)
+                      ptx::tma_load_3d_pair(&peers.tmUp, dst, fbar, col, chunk * BK, adapter);
+                    else
+                      ptx::tma_load_3d(&peers.tmUp, dst, fbar, col, chunk * BK, adapter);
+                  }
                 }
               }
               ++issued;
@@ -2441,10 +2448,15 @@ int lora_gemm(const __half *A, const __half *B, __half *C, int M, int N, int K, 
                                          static_cast<unsigned long long>(ext.adapters)};
   const unsigned long long up_strides[2] = {2ull * N, 2ull * N * ext.rank};
   const unsigned up_box[3] = {64, BK, 1};
+  const unsigned long long up5_dims[5] = {64, up_dims[1], static_cast<unsigned long long>(N / 64),
+                                          static_cast<unsigned long long>(N / umma_n), up_dims[2]};
+  const unsigned long long up5_strides[4] = {2ull * N, 128, 2ull * umma_n, 2ull * N * ext.rank};
+  const unsigned up5_box[5] = {64, BK, static_cast<unsigned>(sub_boxes), static_cast<unsigned>(n_sub), 1};
   if (!encode_2d(&ta, A, M, K, K, CTA_M, BK) || (!b4 && !encode_2d(&tb, B, K, N, N, BK, 64)) ||
       !encode_2d(&tc, C, M, N, N, EPI_ROWS, EPI_COLS) ||
       !encode_2d(&ea.tmLow, ext.low, ext.entries * ext.chunks * pl.tile_m, BK, BK, CTA_M, BK) ||
-      !op_encode(&ea.tmUp, ext.up, 3, up_dims, up_strides, up_box))
+      !(b4 ? op_encode(&ea.tmUp, ext.up, 5, up5_dims, up5_strides, up5_box)
+           : op_encode(&ea.tmUp, ext.up, 3, up_dims, up_strides, up_box)))
     return HGEMM_ERR_TENSOR_MAP;
   ea.base = ext.base;
   ea.count = ext.count;

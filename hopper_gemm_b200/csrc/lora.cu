@@ -28,6 +28,7 @@ constexpr int kMaxRank = 256;
 constexpr int kTileRows = 128;     // rows of a shrink CTA
 constexpr int kMaxTileRows = 256;  // rows of a GEMM tile
 constexpr int kSegCache = 1024;    // segment starts kept in shared memory
+constexpr int kAdapterCache = 1024;  // adapters whose first row in a tile is kept there
 constexpr int kStages = 4;
 constexpr int kBlocks = 4;         // 64-column blocks of Down in a stage
 constexpr int kABytes = kTileRows * 128;
@@ -86,6 +87,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                        const __grid_constant__ CUtensorMap tmDown, const LoraParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_seg[kSegCache];
+  __shared__ int s_first[kAdapterCache];
   __shared__ int s_adapter[kMaxTileRows];
   __shared__ int s_list[kMaxTileRows];
   __shared__ unsigned s_mask[kMaxTileRows / 32];
@@ -108,12 +110,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tile0 = tile * p.tile_rows, row0 = tile0 + half * kTileRows;
 
   // The adapters of the GEMM tile, in the order of their first row.
+  if (warp == 1) {
+    ptx::tmem_alloc<1>(ptx::smem_u32(&s_tmem), 256);
+    ptx::tmem_relinquish<1>();
+  }
   const int *starts = p.seg_start;
+  const bool cached = p.adapters <= kAdapterCache;
   if (p.segments < kSegCache) {
     for (int i = threadIdx.x; i <= p.segments; i += kThreads) s_seg[i] = p.seg_start[i];
     starts = s_seg;
-    __syncthreads();
   }
+  if (cached)
+    for (int i = threadIdx.x; i < p.adapters; i += kThreads) s_first[i] = kMaxTileRows;
+  __syncthreads();
   for (int i = threadIdx.x; i < p.tile_rows; i += kThreads)
     s_adapter[i] = tile0 + i < p.tokens
                        ? token_adapter(starts, p.seg_adapter, p.segments, p.adapters, tile0 + i)
@@ -130,10 +139,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::fence_mbar_init_cluster();
   }
   __syncthreads();
+  if (cached) {
+    for (int i = threadIdx.x; i < p.tile_rows; i += kThreads)
+      if (s_adapter[i] >= 0) atomicMin(&s_first[s_adapter[i]], i);
+    __syncthreads();
+  }
   for (int i0 = warp * 32; i0 < p.tile_rows; i0 += kThreads) {
     const int i = i0 + lane, a = s_adapter[i];
     bool first = a >= 0 && (i == 0 || s_adapter[i - 1] != a);
-    for (int j = 0; first && j < i; ++j) first = s_adapter[j] != a;
+    if (cached)
+      first = first && s_first[a] == i;
+    else
+      for (int j = 0; first && j < i; ++j) first = s_adapter[j] != a;
     const unsigned m = __ballot_sync(0xffffffffu, first);
     if (lane == 0) s_mask[i0 / 32] = m;
   }
@@ -147,6 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int entry0 = min(s_base, p.entries - 1);
   n = min(n, p.entries - entry0);  // (only starts that are not ascending get here with more)
+  ptx::tc_fence_before();
   __syncthreads();
   if (half == 0 && split == 0) {
     if (group == 0 && threadIdx.x == 0) {
@@ -161,16 +179,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int nu = min(n - u0, p.per_group);
   // The same for every CTA of the cluster: no adapters left, or no rows (their products are never
   // stored).
-  if (nu <= 0 || row0 >= p.tokens) return;
-
-  if (warp == 1) {
-    ptx::tmem_alloc<1>(ptx::smem_u32(&s_tmem), 256);
-    ptx::tmem_relinquish<1>();
-  }
-  ptx::tc_fence_before();
-  __syncthreads();
-  ptx::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&s_tmem);
+  if (nu <= 0 || row0 >= p.tokens) {
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem, 256);
+    return;
+  }
+  ptx::tc_fence_after();
   const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * split / p.ksplit);
   const int kb1 = static_cast<int>(static_cast<long long>(p.num_kb) * (split + 1) / p.ksplit);
   const OpWait wc{&s_abort, p.status_word, p.timeout_ns};
@@ -202,27 +216,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           op_drain(full + 8 * (j % kStages), (j / kStages) & 1);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const int n16 = (p.rank + 15) / 16 * 16;
-      const uint32_t idesc = ptx::umma_idesc_f16_f32(kTileRows, n16);
-      int it = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int st = it % kStages;
-        if (!op_wait(full + 8 * st, (it / kStages) & 1, wc, kSiteLoraFull)) break;
-        ptx::tc_fence_after();
-        const uint32_t src = base + st * kStageBytes;
-        const uint64_t ad = ptx::umma_desc_sw128(src, 16, 1024);
-        for (int u = 0; u < nu; ++u) {
-          const uint64_t bd =
-              ptx::umma_desc_sw128(src + kABytes + u * p.chunks * kBBytes, kBBytes, 1024);
+    // One product for all adapters of the group: their blocks of 64 columns lie one behind the other, and
+    // so do their accumulators. The whole warp walks the loop and one lane issues, so that descriptors
+    // stay in uniform registers (walked by one lane a product took twice its time to issue).
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int width = __shfl_sync(0xffffffffu, nu * cols, 0);
+    const uint32_t idesc = ptx::umma_idesc_f16_f32(kTileRows, width);
+    const bool one = ptx::elect_one();
+    int it = 0;
+    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+      const int st = it % kStages;
+      if (!__all_sync(0xffffffffu, op_wait(full + 8 * st, (it / kStages) & 1, wc, kSiteLoraFull))) break;
+      ptx::tc_fence_after();
+      const uint32_t src = base + st * kStageBytes;
+      const uint64_t ad = ptx::umma_desc_sw128(src, 16, 1024);
+      const uint64_t bd = ptx::umma_desc_sw128(src + kABytes, kBBytes, 1024);
+      if (one) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            ptx::umma_f16<1>(tmem + u * cols, ad + 2 * k, bd + 128 * k, idesc, it > 0 || k > 0);
-        }
+        for (int k = 0; k < 4; ++k)
+          ptx::umma_f16<1>(tm, ad + 2 * k, bd + 128 * k, idesc, it > 0 || k > 0);
         if (kb + kStages < kb1) ptx::umma_commit<1>(empty + 8 * st);
       }
-      ptx::umma_commit<1>(acc);
     }
+    if (one) ptx::umma_commit<1>(acc);
+    __syncwarp();
   }
   // Partial sums to shared memory (the stages are free once the last product has retired).
   int okw = 1;
@@ -499,24 +516,30 @@ __global__ void __launch_bounds__(kFewThreads, 2)
           op_drain(ptx::smem_u32(&s_full[j % p.stages]), (j / p.stages) & 1);
     }
   } else if (warp == kIssueWarp) {
-    if (lane == 0) {
-      const uint32_t idesc = ptx::umma_idesc_f16_f32(kFewCols, p.n16, true, true);
-      int it = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int st = it % p.stages;
-        if (!op_wait(ptx::smem_u32(&s_full[st]), (it / p.stages) & 1, wc, kSiteLoraFewFull)) break;
-        ptx::tc_fence_after();
-        const uint32_t src = base + st * stage_bytes;
-        // W: columns are M (64-column blocks 8 KB apart), 16 k are 16 rows of 128 bytes. X: K-major.
-        const uint64_t wd = ptx::umma_desc_sw128(src, kBBytes, 1024);
-        const uint64_t xd = ptx::umma_desc_sw128(src + 2 * kBBytes, 16, 1024);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t idesc = ptx::umma_idesc_f16_f32(kFewCols, p.n16, true, true);
+    const bool one = ptx::elect_one();
+    int st = 0, ph = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!__all_sync(0xffffffffu, op_wait(ptx::smem_u32(&s_full[st]), ph, wc, kSiteLoraFewFull))) break;
+      ptx::tc_fence_after();
+      const uint32_t src = base + st * stage_bytes;
+      // W: columns are M (64-column blocks 8 KB apart), 16 k are 16 rows of 128 bytes. X: K-major.
+      const uint64_t wd = ptx::umma_desc_sw128(src, kBBytes, 1024);
+      const uint64_t xd = ptx::umma_desc_sw128(src + 2 * kBBytes, 16, 1024);
+      if (one) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          ptx::umma_f16<1>(tmem, wd + 128 * k, xd + 2 * k, idesc, it > 0 || k > 0);
+          ptx::umma_f16<1>(tm, wd + 128 * k, xd + 2 * k, idesc, kb > kb0 || k > 0);
         if (kb + p.stages < kb1) ptx::umma_commit<1>(ptx::smem_u32(&s_empty[st]));
       }
-      ptx::umma_commit<1>(ptx::smem_u32(&s_acc));
+      if (++st == p.stages) {
+        st = 0;
+        ph ^= 1;
+      }
     }
+    if (one) ptx::umma_commit<1>(ptx::smem_u32(&s_acc));
+    __syncwarp();
   } else {
     // The adapters' part of this CTA's tokens, while the main loop runs: a warp takes a token, 16 lanes
     // its 128 columns, the two halves of the warp every other row of Up.
@@ -804,10 +827,12 @@ int run(const hgemm_lora_t *a, cudaStream_t stream) {
   p.per_group = std::max(1, kBlocks / p.chunks);
   const int most = std::min(std::min(p.tile_rows, a->segments), a->adapters);
   p.groups = (most + p.per_group - 1) / p.per_group;
-  // K is split over a cluster until the CTAs fill the SMs, with at least 4 k-blocks for each.
+  // K is split over a cluster until the CTAs fill the SMs twice (not every tile has adapters for every
+  // group), with at least 4 k-blocks for each.
   const int tiles128 = (a->tokens + kTileRows - 1) / kTileRows;
   p.ksplit = 1;
-  while (p.ksplit < 8 && 2ll * p.ksplit * tiles128 * p.groups <= d.sm_count && p.num_kb >= 8 * p.ksplit)
+  while (p.ksplit < 8 && 2ll * p.ksplit * tiles128 * p.groups <= (p.groups > 1 ? 2 : 1) * d.sm_count &&
+         p.num_kb >= 8 * p.ksplit)
     p.ksplit *= 2;
   const long long ctas =
       static_cast<long long>(tiles) * (p.tile_rows / kTileRows) * p.groups * p.ksplit;
