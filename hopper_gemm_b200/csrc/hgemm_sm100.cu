@@ -430,13 +430,19 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
         decode_tile(tile, p, tm, tn);
         const int arow = tm * Cfg::UMMA_M + static_cast<int>(rank) * CTA_M;
         const int bcol = tn * BN + static_cast<int>(rank) * Cfg::SUB_COLS;
+        // EXT: additional k-blocks, known (and looked for) once the tile's own are on their way, so that
+        // the launch that makes them may still be at work before.
         int ext_base = 0, ext_blocks = 0;
-        if constexpr (EXT) {
-          ext_base = peers.base[tm];
-          ext_blocks = peers.count[tm] * peers.chunks;
-        }
-        // (the count is looked at only behind the tile's own k-blocks, so its load hides)
-        for (int kb = kb_begin; kb < kb_end || (EXT && kb < kb_end + ext_blocks); ++kb) {
+        for (int kb = kb_begin;; ++kb) {
+          if (kb == kb_end) {
+            if constexpr (!EXT) break;
+            if constexpr (EXT) {
+              ptx::grid_wait();
+              ext_base = peers.base[tm];
+              ext_blocks = peers.count[tm] * peers.chunks;
+            }
+          }
+          if (kb >= kb_end + ext_blocks) break;
           if (!wait_bar<false>(ptx::smem_u32(&empty[s]), ph ^ 1u, wctx, kSiteProducerEmpty))
             return false;
           const uint32_t fbar = full_leader0 + static_cast<uint32_t>(s) * 8u;
@@ -649,11 +655,15 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
         int next = -1;
         bool have_next = false;
         int kb_stop = kb_end;  // behind this tile's last k-block
-        if constexpr (EXT) {
-          int tm, tn;
-          decode_tile(tile, p, tm, tn);
-          kb_stop += peers.count[tm] * peers.chunks;
-        }
+        // EXT: looked for near the end of the tile's own k-blocks (see the producer).
+        auto find_stop = [&]() {
+          if constexpr (EXT) {
+            int tm, tn;
+            decode_tile(tile, p, tm, tn);
+            ptx::grid_wait();
+            kb_stop = kb_end + peers.count[tm] * peers.chunks;
+          }
+        };
         auto poll_next = [&](int kb) {
           if (!have_next && kb >= kb_stop - S && sched_try_read(sslot, sph, next)) have_next = true;
         };
@@ -683,6 +693,7 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
             return true;
           };
           for (int kb = kb_begin; kb < main_kb && ok; ++kb) ok = kblock(kb);
+          find_stop();
           for (int kb = main_kb; kb < kb_stop && ok; ++kb) {
             ok = kblock(kb);
             poll_next(kb);
@@ -723,6 +734,7 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
           };
           const int tail_from = p.num_kb - S;  // k-blocks at or past this one are skewed
           for (int kb = 0; kb < p.num_kb || (EXT && kb < kb_stop); ++kb) {
+            if (EXT && kb == (tail_from > 0 ? tail_from : 0)) find_stop();
             if (!wait_bar<false>(ptx::smem_u32(&full[s]), ph, wctx, kSiteMmaFull)) {
               ok = false;
               break;
@@ -890,7 +902,7 @@ __global__ void __launch_bounds__(TileCfg<PAIR, BN, EPIW>::THREADS, 1)
     auto note_odd = [&](uint32_t odd, int brow, int bcol) {
       if constexpr (EXT) {
         const bool mine = (odd & 0x80008000u) != 0 && brow + lane < p.M && bcol < p.N;
-        if (__any_sync(0xffffffffu, mine) && lane == 0)
+        if (__any_sync(0xffffffffu, mine) && lane == 0)  // (the count was cleared before find_stop)
           peers.odd_list[atomicAdd(peers.odd_count, 1u)] =
               static_cast<unsigned long long>(brow) | (static_cast<unsigned long long>(bcol) << 32);
       }
@@ -2487,13 +2499,16 @@ int lora_gemm(const __half *A, const __half *B, __half *C, int M, int N, int K, 
   cfg.blockDim = dim3(fi.threads, 1, 1);
   cfg.dynamicSmemBytes = fi.smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  // Starts while the launch before it (which makes `ext`) is at work; waits for it in the kernel.
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = ti.pair == 2 ? 1 : 0;
+  cfg.numAttrs = ti.pair == 2 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, k, ta, tb, tc, kp, ea) != cudaSuccess) {
     cudaGetLastError();
     return HGEMM_ERR_LAUNCH;

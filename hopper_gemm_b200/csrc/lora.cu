@@ -85,6 +85,7 @@ __device__ __forceinline__ int token_adapter(const int *seg_start, const int *se
 __global__ void __launch_bounds__(kThreads, 1)
     lora_shrink_kernel(const __grid_constant__ CUtensorMap tmX,
                        const __grid_constant__ CUtensorMap tmDown, const LoraParams p) {
+  ptx::grid_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_seg[kSegCache];
   __shared__ int s_first[kAdapterCache];
@@ -122,7 +123,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (cached)
     for (int i = threadIdx.x; i < p.adapters; i += kThreads) s_first[i] = kMaxTileRows;
+  const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * split / p.ksplit);
+  const int kb1 = static_cast<int>(static_cast<long long>(p.num_kb) * (split + 1) / p.ksplit);
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int i = 0; i < kStages; ++i) {
+      ptx::mbar_init(full + 8 * i, 2);  // X; the blocks of Down
+      ptx::mbar_init(empty + 8 * i, 1);
+    }
+    ptx::mbar_init(acc, 1);
+    ptx::fence_mbar_init_cluster();
+  }
   __syncthreads();
+  // X's first stages are asked for before the adapters are known, by the CTAs that any adapter makes use of.
+  const int early = group == 0 && row0 < p.tokens ? min(kStages, kb1 - kb0) : 0;
+  if (threadIdx.x == 0)
+    for (int it = 0; it < early; ++it) {
+      ptx::mbar_arrive_expect_tx(full + 8 * it, kABytes);
+      ptx::tma_load_2d(&tmX, base + it * kStageBytes, full + 8 * it, (kb0 + it) * 64, row0);
+    }
+  __syncwarp();
   for (int i = threadIdx.x; i < p.tile_rows; i += kThreads)
     s_adapter[i] = tile0 + i < p.tokens
                        ? token_adapter(starts, p.seg_adapter, p.segments, p.adapters, tile0 + i)
@@ -130,13 +150,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     // Tiles before this one have at most one entry each more than the segments that begin in them.
     s_base = tile + starts_upto(starts, p.segments, tile0 - 1);
-    s_abort = 0;
-    for (int i = 0; i < kStages; ++i) {
-      ptx::mbar_init(full + 8 * i, 1);
-      ptx::mbar_init(empty + 8 * i, 1);
-    }
-    ptx::mbar_init(acc, 1);
-    ptx::fence_mbar_init_cluster();
   }
   __syncthreads();
   if (cached) {
@@ -182,11 +195,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&s_tmem);
   if (nu <= 0 || row0 >= p.tokens) {
     if (warp == 1) ptx::tmem_dealloc<1>(tmem, 256);
+    if (threadIdx.x == 0)
+      for (int it = 0; it < early; ++it) {  // the loads in flight land before the CTA may exit
+        ptx::mbar_arrive(full + 8 * it);
+        op_drain(full + 8 * it, 0);
+      }
     return;
   }
   ptx::tc_fence_after();
-  const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * split / p.ksplit);
-  const int kb1 = static_cast<int>(static_cast<long long>(p.num_kb) * (split + 1) / p.ksplit);
   const OpWait wc{&s_abort, p.status_word, p.timeout_ns};
   const int cols = p.chunks * 64;  // accumulator columns of an adapter
   bool ok = true;
@@ -195,18 +211,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0 || (box >= 0 && box < nu * p.chunks)) {
     if (lane == 0) {
       const int adapter = box >= 0 ? s_list[u0 + box / p.chunks] : 0;
-      int it = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+      int it = box < 0 ? early : 0;
+      for (int kb = kb0 + it; kb < kb1; ++kb, ++it) {
         const int st = it % kStages;
         if (it >= kStages &&
             !(ok = op_wait(empty + 8 * st, (it / kStages - 1) & 1, wc, kSiteLoraEmpty)))
           break;
         const uint32_t dst = base + st * kStageBytes, bar = full + 8 * st;
         if (box < 0) {
-          ptx::mbar_arrive_expect_tx(bar, kABytes + nu * p.chunks * kBBytes);
+          ptx::mbar_arrive_expect_tx(bar, kABytes);
           ptx::tma_load_2d(&tmX, dst, bar, kb * 64, row0);
         } else {
-          // (counted on the barrier before or after the bytes are announced)
+          // (the first box's warp announces all of them; bytes may be counted before that)
+          if (box == 0) ptx::mbar_arrive_expect_tx(bar, nu * p.chunks * kBBytes);
           ptx::tma_load_3d(&tmDown, dst + kABytes + box * kBBytes, bar, 64 * (box % p.chunks), kb * 64,
                            adapter);
         }
@@ -827,12 +844,10 @@ int run(const hgemm_lora_t *a, cudaStream_t stream) {
   p.per_group = std::max(1, kBlocks / p.chunks);
   const int most = std::min(std::min(p.tile_rows, a->segments), a->adapters);
   p.groups = (most + p.per_group - 1) / p.per_group;
-  // K is split over a cluster until the CTAs fill the SMs twice (not every tile has adapters for every
-  // group), with at least 4 k-blocks for each.
+  // K is split over a cluster until the CTAs fill the SMs, with at least 4 k-blocks for each.
   const int tiles128 = (a->tokens + kTileRows - 1) / kTileRows;
   p.ksplit = 1;
-  while (p.ksplit < 8 && 2ll * p.ksplit * tiles128 * p.groups <= (p.groups > 1 ? 2 : 1) * d.sm_count &&
-         p.num_kb >= 8 * p.ksplit)
+  while (p.ksplit < 8 && 2ll * p.ksplit * tiles128 * p.groups <= d.sm_count && p.num_kb >= 8 * p.ksplit)
     p.ksplit *= 2;
   const long long ctas =
       static_cast<long long>(tiles) * (p.tile_rows / kTileRows) * p.groups * p.ksplit;

@@ -44,6 +44,7 @@ struct LoraExt {
 };
 // Rows of a tile that lora_gemm uses for these sizes (128 or 256).
 int lora_gemm_tile_rows(int M, int N, int K, int *rows);
+// Launched with programmatic serialization: reads `ext` behind a grid_wait.
 int lora_gemm(const __half *A, const __half *B, __half *C, int M, int N, int K, const LoraExt &ext,
               cudaStream_t stream);
 
