@@ -12,6 +12,7 @@ on the batch is read on the device, so a captured call follows its tensors at re
 call raises HgemmError (or TypeError / ValueError for tensors of the wrong type or shape).
 """
 import ctypes
+import functools
 import struct
 
 import torch
@@ -78,15 +79,20 @@ def _cuda(t):
     return dev
 
 
-def _new(shape, dtype, like, stream):
-    """A tensor of this call on the launching stream: memory from that stream's pool is free for work
-    on it."""
+def _new(shape, like, stream):
+    """A float16 tensor of this call on the launching stream: memory from that stream's pool is free for
+    work on it."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape)
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(stream, device=like.device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape)
+
+
+# What a call needs depends on its sizes alone.
+_lora_bytes = functools.lru_cache(1024)(lambda *sizes: lib.hgemm_lora_workspace_bytes(*sizes))
+_attn_bytes = functools.lru_cache(1024)(lambda *sizes: lib.hgemm_attn_prompt_workspace_bytes(*sizes))
 
 
 def _scratch(need, workspace, like, stream):
@@ -94,7 +100,7 @@ def _scratch(need, workspace, like, stream):
     if workspace is None:
         if need == 0:
             return None, 0, 0
-        workspace = _new((need,), _U8, like, stream)
+        workspace = _new(((need + 1) // 2,), like, stream)
     elif workspace.get_device() != like.get_device() or not workspace.is_contiguous():
         raise ValueError(f"workspace must be contiguous on {like.device}")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
@@ -134,10 +140,11 @@ def lora(X, W, down, up, scale, seg_start, seg_adapter, Y=None, workspace=None, 
     ss = _dense("seg_start", seg_start, _I32, (S + 1,), dev)
     sa = _dense("seg_adapter", seg_adapter, _I32, (S,), dev)
     if Y is None:
-        Y = _new((T, N), _HALF, X, stream)
-    y = _dense("Y", Y, _HALF, (T, N), dev)
-    keep, ws, nbytes = _scratch(lib.hgemm_lora_workspace_bytes(T, N, K, r, A, S), workspace, X,
-                                stream)
+        Y = _new((T, N), X, stream)
+        y = Y.data_ptr()
+    else:
+        y = _dense("Y", Y, _HALF, (T, N), dev)
+    keep, ws, nbytes = _scratch(_lora_bytes(T, N, K, r, A, S), workspace, X, stream)
     _call("hgemm_lora",
           _pack_lora(x, w, y, d, u, sc, ss, sa, ws, nbytes, T, N, K, r, A, S), dev, stream)
     return Y
@@ -166,12 +173,12 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, axis_o
     inv = _dense("inv_freq", inv_freq, _F32, (half,), dev)
     axis = _dense("axis_of", axis_of, _U8, (half,), dev) if axis_of is not None else 0
     if q_out is None:
-        q_out = _new((T, hq, d), _HALF, q, stream)
+        q_out = _new((T, hq, d), q, stream)
         qos = hq * d
     else:
         qos = _heads("q_out", q_out, dev)
     if k_out is None:
-        k_out = _new((T, hk, d), _HALF, q, stream)
+        k_out = _new((T, hk, d), q, stream)
         kos = hk * d
     else:
         kos = _heads("k_out", k_out, dev)
@@ -203,15 +210,14 @@ def attn_prompt(q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None, lse
     cq = _dense("cu_q", cu_q, _I32, (B + 1,), dev)
     ck = _dense("cu_k", cu_k, _I32, (B + 1,), dev) if cu_k is not None else 0
     if out is None:
-        out = _new((Tq, hq, d), _HALF, q, stream)
+        out = _new((Tq, hq, d), q, stream)
         os = hq * d
     elif out.shape != q.shape:
         raise ValueError("out has another shape than q")
     else:
         os = _heads("out", out, dev)
     ls = _dense("lse", lse, _F32, (Tq, hq), dev) if lse is not None else 0
-    keep, ws, nbytes = _scratch(lib.hgemm_attn_prompt_workspace_bytes(Tq, Tk, B, hq, hkv, d),
-                                workspace, q, stream)
+    keep, ws, nbytes = _scratch(_attn_bytes(Tq, Tk, B, hq, hkv, d), workspace, q, stream)
     _call("hgemm_attn_prompt",
           _pack_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ls, cq, ck, qs, ks,
                      vs, os, ws, nbytes, Tq, Tk, B, hq, hkv, d, 1 if causal else 0,
