@@ -67,6 +67,10 @@ __device__ void attn_row(const AttnParams &p, const __half *qrow, const __half *
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
     s *= p.scale2;
+    if (s != s) {  // a NaN score: so is all of the row
+      m = l = o[0] = o[1] = o[2] = o[3] = s;
+      return;
+    }
     if (s > m) {
       const float f = exp2f(m - s);
       l *= f;
@@ -212,6 +216,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(misc + 1);
   Tile *found = reinterpret_cast<Tile *>(misc + 2);
 
+  if (p.chunk > 0) ptx::grid_launch_dependents();  // attn_join_kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (base & 1023u) {  // swizzle atoms would be off (the declaration asks for this alignment)
     if (threadIdx.x == 0) atomicCAS(p.status_word, 0u, 0x100u | kSiteAttnQ);
@@ -638,7 +643,10 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
   const long long rows = static_cast<long long>(p.total_q) * p.heads_q;
   const long long row = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
-  if (row >= rows) return;
+  if (row >= rows) {
+    ptx::grid_wait();
+    return;
+  }
   const int i = static_cast<int>(row / p.heads_q), h = static_cast<int>(row % p.heads_q);
   // Ranges of the row's sequence; rows of no sequence hold nothing and are left as they were.
   int mine = 0;
@@ -649,6 +657,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
     if (i >= q0 && i < q1) mine = chunks_of(p, k1 - k0);
   }
   const int chunks = __reduce_max_sync(0xffffffffu, mine);
+  ptx::grid_wait();
   if (chunks == 0) return;
   // A lane holds the sums of ranges lane, lane + 32, .. .
   constexpr int kEach = kMaxChunks / 32;
@@ -856,8 +865,20 @@ int run(const hgemm_attn_prompt_t *a, cudaStream_t stream) {
        : pl.tiles == 1   ? launch<2, 1>(tq, tk, tv, p, d, ctas, stream)
                          : launch<2, 2>(tq, tk, tv, p, d, ctas, stream);
   if (st != HGEMM_OK || pl.chunk == 0) return st;
-  attn_join_kernel<<<static_cast<unsigned>(joins), 256, 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(joins), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, attn_join_kernel, p) != cudaSuccess) {
+    cudaGetLastError();
+    return HGEMM_ERR_LAUNCH;
+  }
+  return HGEMM_OK;
 }
 
 }  // namespace

@@ -66,6 +66,17 @@ def test_lora_sizes(cuda, T, K, N, r):
         check_lora(cuda, T, K, N, r, 3, [0, a, b, T], [2, 0, 1])
 
 
+@pytest.mark.parametrize("T,N,K", [
+    (65, 72, 512), (65, 512, 512), (65, 8, 64), (65, 512, 64), (513, 4096, 64), (257, 4104, 1024),
+    (513, 2048, 1024), (2049, 2056, 264), (1500, 4096, 264), (3000, 2056, 2048), (777, 8192, 1024),
+    (4100, 4096, 2048)])
+def test_lora_tiles(cuda, T, N, K):
+    """Every tile of the GEMM, whole in N and not, with several adapters to a tile and a rank of two
+    64-column blocks."""
+    cut = [0, T // 9, T // 5, T // 5 + 1, T // 2, T - T // 3, T - 2, T]
+    check_lora(cuda, T, K, N, 72, 6, cut, [5, 0, -1, 3, 0, 4, 1], seed=N)
+
+
 @pytest.mark.parametrize("T", [40, 64, 200, 515])
 @pytest.mark.parametrize("r", [16, 96])
 def test_lora_segments(cuda, T, r):
@@ -296,6 +307,15 @@ def test_attn_single_tokens(cuda, nk, hq, hkv, d):
     check_attn(cuda, [1], [nk], hq, hkv, d, seed=nk)
 
 
+@pytest.mark.parametrize("q,k,hq,hkv,d", [
+    ([300], [7000], 4, 1, 128), ([700, 1, 650], [7000, 12000, 6200], 16, 8, 128),
+    ([129, 65], [6200, 6300], 8, 8, 96), ([1000, 0, 40, 900], [6000, 9000, 20000, 900], 16, 8, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attn_long_keys(cuda, q, k, hq, hkv, d, causal):
+    """Prompts over many keys: two row tiles to a CTA, key ranges joined and not, one tile without rows."""
+    check_attn(cuda, q, k, hq, hkv, d, causal=causal, seed=len(q))
+
+
 def test_attn_many_sequences(cuda):
     lens = [(i * 37) % 90 for i in range(300)]
     check_attn(cuda, lens, lens, 4, 1, 64, extra=3)
@@ -317,6 +337,8 @@ def test_attn_growing_maximum(cuda):
         edit(q, k, v)
         k.copy_(k.flip(0))
     check_attn(cuda, [700], [700], 4, 2, 128, edit=fall)
+    check_attn(cuda, [300], [7000], 4, 1, 128, edit=edit)
+    check_attn(cuda, [700], [6500], 16, 8, 128, edit=edit)
 
 
 def test_attn_scale(cuda):
