@@ -97,7 +97,8 @@ constexpr int kMaxChunks = 64;   // key ranges of a sequence
 constexpr float kLag = 8.0f;
 
 // DB: 64-element blocks of head_dim in shared memory (head_dim <= 64 DB); TILES: row tiles of a CTA,
-// each with four softmax warps, a thread to a row.
+// each with four softmax warps, a thread to a row; FINE: weights go into their product as two binary16
+// numbers each, the second of what the first left over, 22 bits in all.
 //
 // Blocks of 64 keys, because a tile's scores then have two places in TMEM: the next block's scores are
 // formed while a block's softmax runs, and no tile ever waits for the way from its weights through two
@@ -194,7 +195,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return y;
 }
 
-template <int DB, int TILES>
+template <int DB, int TILES, bool FINE>
 __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES>::CTAS)
     attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const AttnParams p) {
@@ -355,6 +356,11 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
 #pragma unroll
           for (int k = 0; k < kBlock / 16; ++k)
             ptx::umma_f16_ts(tmO, tmS + place * kBlock + 8 * k, vd + 128 * k, idesc_o, !(first && k == 0));
+          if constexpr (FINE) {
+#pragma unroll
+            for (int k = 0; k < kBlock / 16; ++k)
+              ptx::umma_f16_ts(tmO, tmS + place * kBlock + kBlock / 2 + 8 * k, vd + 128 * k, idesc_o, true);
+          }
         }
       };
       // Load `item` lies in stage item % S; it is waited for and given back once by either tile's warp,
@@ -436,6 +442,8 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     const int n = i == 0 ? count0 : count1;
     const int qi = first + row / p.group;  // query of this row, inside the sequence
     const bool live = qt >= 0 && row < p.tile_q * p.group && qi < qlen;
+    // A warp whose 32 rows are no query's (single tokens fill one of the four) only keeps step.
+    const bool idle = !__any_sync(0xffffffffu, live);
     const int limit = p.causal ? max(0, min(klen, qi + 1 + klen - qlen)) : klen;
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp, lane << 16
     const uint32_t tS = tmem + lane_base + i * (2 * kBlock);
@@ -454,6 +462,10 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     for (int u = 0; u < n; ++u) {
       const uint32_t place = tS + (u & 1) * kBlock;
       if (!(ok = wait(sfull + 16 * i + 8 * (u & 1), u >> 1, kSiteAttnScores))) break;
+      if (idle) {  // whatever stands in its rows of the weights stays in its rows of the output
+        if (lane == 0) ptx::mbar_arrive(pfull + 16 * i + 8 * (u & 1));
+        continue;
+      }
       uint32_t sr[2][32];
       ptx::tmem_ld_32x32b_x32(place, sr[0]);
       ptx::tmem_ld_32x32b_x32(place + 32, sr[1]);
@@ -500,7 +512,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       const float2 neg = make_float2(neg1, neg1), scale = make_float2(p.scale2, p.scale2);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t w2[16];
+        uint32_t w2[16], rest[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float2 x = __ffma2_rn(
@@ -509,8 +521,14 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
           sum[e & 1] = __fadd2_rn(sum[e & 1], ab);
           const __half2 h2 = __float22half2_rn(ab);
           w2[e] = *reinterpret_cast<const uint32_t *>(&h2);
+          if constexpr (FINE) {
+            const float2 up = __half22float2(h2);
+            const __half2 r2 = __float22half2_rn(__fadd2_rn(ab, make_float2(-up.x, -up.y)));
+            rest[e] = *reinterpret_cast<const uint32_t *>(&r2);
+          }
         }
         ptx::tmem_st_32x32b_x16(place + 16 * c, w2);
+        if constexpr (FINE) ptx::tmem_st_32x32b_x16(place + kBlock / 2 + 16 * c, rest);
       }
       ptx::tmem_st_wait();
       ptx::tc_fence_before();
@@ -518,7 +536,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
       if (lane == 0) ptx::mbar_arrive(pfull + 16 * i + 8 * (u & 1));
     }
     if (ok && n > 0) ok = wait(ofull + 8 * i, 0, kSiteAttnOut);
-    if (ok) {
+    if (ok && !idle) {
       const int kb = b0 * kBlock;                                  // first key of this CTA
       const int ke = min(limit, kb + n * kBlock);                  // behind the last that the row sees
       const bool any = ke > kb;
@@ -714,6 +732,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
 struct AttnPlan {
   int tiles;       // row tiles of a CTA
   int tile_q;      // queries of a row tile
+  bool fine;       // weights of 22 bits
   int chunk, max_chunks;
   long long items;  // upper bound of (tile, key range) pairs of all sequences
   size_t workspace;
@@ -729,11 +748,19 @@ AttnPlan make_plan(int total_q, int total_k, int batch, int heads_q, int heads_k
   // tokens 174 and 166 us, 8192 tokens 475 and 495, 16384 tokens 1.89 and 2.06 ms), in favour of
   // one tile at head_dim 64 up to 8192.
   pl.tiles = head_dim > 64 && avg_k >= 6144 && avg_q > pl.tile_q ? 2 : 1;
+  // Weights rounded to binary16 leave as much error in an output as its own rounding does: together 1.4
+  // times the latter over many outputs, over a token's few by chance 1.5 and more (6 rows of 96, seen). There
+  // they keep 22 bits, which costs 5% (one token over 131072 keys 124 us against 118, before its key ranges
+  // were made longer); 16 tokens of 32 heads would take 106 us instead of 99, a dozen prompts 141 for 122.
+  pl.fine = static_cast<long long>(total_q) * heads_q <= 128;
   const int span = pl.tiles * pl.tile_q;
   const long long max_tiles = std::min<long long>(total_q, total_q / span + static_cast<long long>(batch));
   // Key ranges where there are few tiles: of single tokens (whose lengths set the pace) up to two
   // waves of CTAs, of prompts up to half a wave, beyond which writing and joining the parts costs more
-  // than the idle SMs. About four ranges to a CTA slot, of 1024 keys at least.
+  // than the idle SMs. As many as fill one wave at the mean length (longer sequences get more), of 256 keys
+  // at least: one token over 2000 keys 12.9 us with 256, 14.2 with 128, 20.0 with 1024; over 131072 keys 97.5
+  // us with one wave of ranges, 124 with four shorter ones to a slot, whose starts then cost more than the
+  // wave's uneven end.
   const long long slots = kSms * (pl.tiles == 1 ? 2 : 1);
   const long long est_tiles = std::max<long long>((total_q + span - 1) / span, batch);
   const long long units = est_tiles * heads_kv;
@@ -742,8 +769,8 @@ AttnPlan make_plan(int total_q, int total_k, int batch, int heads_q, int heads_k
   pl.max_chunks = 1;
   pl.items = max_tiles;
   if (avg_q <= pl.tile_q ? units < 2 * slots : 2 * units <= slots) {
-    const long long work = units * blocks / batch;
-    long long chunk = std::max<long long>(16, (work + 4 * slots - 1) / (4 * slots));
+    const long long ranges = std::max<long long>(1, slots / units);  // of a sequence, in one wave
+    long long chunk = std::max<long long>(4, (blocks / batch + ranges - 1) / ranges);
     chunk = std::max(chunk, (blocks + kMaxChunks - 1) / kMaxChunks);
     const long long chunks = (blocks + chunk - 1) / chunk;
     if (chunks > 1) {
@@ -787,14 +814,14 @@ int check(const hgemm_attn_prompt_t *a) {
   return HGEMM_OK;
 }
 
-template <int DB, int TILES>
+template <int DB, int TILES, bool FINE>
 int launch(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const AttnParams &p,
            const OpDevice &d, long long ctas, cudaStream_t stream) {
   using Cfg = AttnCfg<DB, TILES>;
   static bool done[64];
-  const int st = op_smem(reinterpret_cast<const void *>(attn_kernel<DB, TILES>), Cfg::SMEM, d.dev, done);
+  const int st = op_smem(reinterpret_cast<const void *>(attn_kernel<DB, TILES, FINE>), Cfg::SMEM, d.dev, done);
   if (st != HGEMM_OK) return st;
-  attn_kernel<DB, TILES>
+  attn_kernel<DB, TILES, FINE>
       <<<static_cast<unsigned>(ctas), Cfg::THREADS, Cfg::SMEM, stream>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? HGEMM_OK : HGEMM_ERR_LAUNCH;
 }
@@ -861,9 +888,14 @@ int run(const hgemm_attn_prompt_t *a, cudaStream_t stream) {
   const long long ctas = pl.items * a->heads_kv;
   const long long joins = (static_cast<long long>(a->total_q) * a->heads_q + 7) / 8;
   if (ctas > 0x7fffffffll || joins > 0x7fffffffll) return HGEMM_ERR_TOO_LARGE;
-  st = a->head_dim <= 64 ? launch<1, 1>(tq, tk, tv, p, d, ctas, stream)
-       : pl.tiles == 1   ? launch<2, 1>(tq, tk, tv, p, d, ctas, stream)
-                         : launch<2, 2>(tq, tk, tv, p, d, ctas, stream);
+  if (a->head_dim <= 64)
+    st = pl.fine ? launch<1, 1, true>(tq, tk, tv, p, d, ctas, stream)
+                 : launch<1, 1, false>(tq, tk, tv, p, d, ctas, stream);
+  else if (pl.tiles == 1)
+    st = pl.fine ? launch<2, 1, true>(tq, tk, tv, p, d, ctas, stream)
+                 : launch<2, 1, false>(tq, tk, tv, p, d, ctas, stream);
+  else
+    st = launch<2, 2, false>(tq, tk, tv, p, d, ctas, stream);
   if (st != HGEMM_OK || pl.chunk == 0) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(joins), 1, 1);
