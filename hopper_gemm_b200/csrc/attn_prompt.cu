@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     return (seen + kBlock - 1) / kBlock;
   };
   const int need = max(need_of(0), need_of(TILES - 1));
-  const bool whole = p.chunk == 0;
+  const bool whole = chunks_of(p, klen) == 1;  // nothing to join
   const int per = whole ? need : p.chunk;
   const int split = work.chunk, b0 = split * per;
   auto count_of = [&](int i) { return max(0, min(need_of(i) - b0, per)); };
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
     return;
   }
   const int i = static_cast<int>(row / p.heads_q), h = static_cast<int>(row % p.heads_q);
-  // Ranges of the row's sequence; rows of no sequence hold nothing and are left as they were.
+  // Ranges of the row's sequence; rows of no sequence are left as they were.
   int mine = 0;
   for (int b = lane; b < p.batch; b += 32) {
     int q0, q1, k0, k1;
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
   }
   const int chunks = __reduce_max_sync(0xffffffffu, mine);
   ptx::grid_wait();
-  if (chunks == 0) return;
+  if (chunks <= 1) return;  // written by its only CTA
   // A lane holds the sums of ranges lane, lane + 32, .. .
   constexpr int kEach = kMaxChunks / 32;
   float z[kEach], top = -INFINITY;
