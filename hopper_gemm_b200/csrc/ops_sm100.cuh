@@ -64,7 +64,6 @@ enum OpWaitSite : unsigned {
   kSiteLoraFewEmpty = 43,
   kSiteLoraFewFull = 44,
   kSiteLoraFewAcc = 45,
-  kSiteOpDrain = 63,
 };
 
 // Bounded wait of one thread; false when the CTA is unwinding or the wait ran out (recorded in
