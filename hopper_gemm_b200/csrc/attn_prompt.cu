@@ -838,6 +838,7 @@ int check(const hgemm_attn_prompt_t *a) {
   if (!a->q || !a->out || !a->cu_q) return HGEMM_ERR_INVALID_ARG;
   if (!a->cu_k && a->total_k != a->total_q) return HGEMM_ERR_INVALID_ARG;
   if (a->total_k > 0 && (!a->k || !a->v)) return HGEMM_ERR_INVALID_ARG;
+  if (a->out == a->q || a->out == a->k || a->out == a->v) return HGEMM_ERR_INVALID_ARG;
   if (!op_aligned16(a->q) || !op_aligned16(a->k) || !op_aligned16(a->v) || !op_aligned16(a->out))
     return HGEMM_ERR_INVALID_ARG;
   const long long qrow = static_cast<long long>(a->heads_q) * a->head_dim;

@@ -708,6 +708,7 @@ int check(const hgemm_lora_t *a) {
   if (a->tokens == 0 || a->N == 0) return HGEMM_OK;
   if (!a->X || !a->W || !a->Y || !op_aligned16(a->X) || !op_aligned16(a->W) || !op_aligned16(a->Y))
     return HGEMM_ERR_INVALID_ARG;
+  if (a->Y == a->X || a->Y == a->W) return HGEMM_ERR_INVALID_ARG;
   if (a->segments > 0 && (!a->seg_start || !a->seg_adapter)) return HGEMM_ERR_INVALID_ARG;
   if (a->adapters > 0 && a->segments > 0 &&
       (!a->down || !a->up || !a->scale || !op_aligned16(a->down) || !op_aligned16(a->up)))

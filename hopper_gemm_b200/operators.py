@@ -9,7 +9,8 @@ Each function checks its tensors, allocates what is not given (outputs, workspac
 on `stream` (default: the current stream of the tensors' device) through the C ABI of
 libhgemm_b200.so, whose header states the formulas and ranges. Launches are asynchronous; what depends
 on the batch is read on the device, so a captured call follows its tensors at replay. A refused
-call raises HgemmError (or TypeError / ValueError for tensors of the wrong type or shape).
+call raises HgemmError (or TypeError / ValueError for tensors of the wrong type or shape). They serve:
+no gradients are formed.
 """
 import ctypes
 import functools

@@ -289,10 +289,12 @@ int hgemm_qk_norm_rope(const hgemm_qk_norm_rope_t *args, hgemm_stream_t stream);
  * keys, or a single token); a query without any key gets zeros and an lse of -infinity. Queries
  * behind cu_q[batch] are not touched. Scores, the running maximum and sum are fp32; the
  * weights of a row, relative to its running maximum, are rounded to binary16 as an operand of the
- * second product. lse (fp32, total_q x heads_q, natural logarithm of the row's sum) may be NULL.
+ * second product (calls of up to 128 rows total_q * heads_q keep 22 bits). lse (fp32, total_q x heads_q, natural logarithm of the row's sum) may be NULL.
  * scale is finite and not negative; heads_q is a multiple of heads_kv, at most 128 times it; head_dim is a multiple of 8 up to 128.
  * Strides are halves between tokens, multiples of 8 and at least heads * head_dim; heads of a
- * token are adjacent; q, k, v and out start on 16-byte boundaries. total_q and total_k are the
+ * token are adjacent; q, k, v and out start on 16-byte boundaries; out overlaps no input (other columns
+ * of the same rows are fine). A row that sees an infinity or NaN, or whose tile holds one in a place masked
+ * for it, is formed again by itself, at about 7 keys a microsecond. total_q and total_k are the
  * rows that the tensors hold; starts that point behind them are cut off there. */
 typedef struct {
   const hgemm_half_t *q, *k, *v;

@@ -1,6 +1,9 @@
 """GPU: the attention layer's operators against plain 64-bit forms, at the sizes, masks, strides and
 values where they can go wrong."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -534,6 +537,58 @@ def test_two_graphs_do_not_share_a_workspace(cuda):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+CAPTURED_FIRST = """
+import torch, hopper_gemm_b200 as hg
+T, d = {T}, 64
+g = torch.Generator(device="cuda").manual_seed(0)
+n = lambda *s: torch.randn(s, generator=g, device="cuda").half()
+x, w, down, up, wn = n(T, 256), n(256, 384) / 16, n(2, 256, 16) / 16, n(2, 16, 384) / 4, n(d)
+i32 = lambda v: torch.tensor(v, device="cuda", dtype=torch.int32)
+scale, seg, ids, pos = torch.ones(2, device="cuda"), i32([0, 3, T]), i32([1, 0]), i32(list(range(T)))
+inv = torch.ones(d // 2, device="cuda") / 100
+def layer():
+    qkv = hg.lora(x, w, down, up, scale, seg, ids).view(T, 6, d)
+    q, k = hg.qk_norm_rope(qkv[:, :4], qkv[:, 4:5], wn, wn, pos, inv)
+    return hg.attn_prompt(q, k, qkv[:, 5:], seg)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = layer()
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(got, layer())
+"""
+
+
+@pytest.mark.parametrize("T", [20, 200])
+def test_first_call_of_a_process_is_captured(T):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", CAPTURED_FIRST.format(T=T)], cwd=root, timeout=120,
+                         capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr[-2000:]
+
+
+def test_explicit_workspace_on_another_stream(cuda):
+    """The caller's workspace, a view of its own buffer, with prompts in key ranges and single tokens."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for q, k in (([1] * 3, [900, 4000, 70]), ([40], [5000])):
+        Q, K, V = (torch.randn((n, h, 64), generator=g, device="cuda").half()
+                   for n, h in ((sum(q), 4), (sum(k), 2), (sum(k), 2)))
+        cq, ck = i32(starts(q)), i32(starts(k))
+        want = cuda.attn_prompt(Q, K, V, cq, ck)
+        need = cuda.lib.hgemm_attn_prompt_workspace_bytes(sum(q), sum(k), len(q), 4, 2, 64)
+        assert need > 0
+        ws = torch.full((need + 512,), 0x7f, device="cuda", dtype=torch.uint8)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        got = cuda.attn_prompt(Q, K, V, cq, ck, workspace=ws[256:256 + need], stream=s)
+        s.synchronize()
+        assert torch.equal(got, want)
+        assert bool((ws[:256] == 0x7f).all()) and bool((ws[256 + need:] == 0x7f).all())
+        with pytest.raises(cuda.HgemmError):
+            cuda.attn_prompt(Q, K, V, cq, ck, workspace=ws[256:255 + need])
 
 
 def test_repeated_runs_are_identical(cuda):

@@ -132,3 +132,14 @@ def test_public_functions_refuse_host_tensors():
         hg.qk_norm_rope(x[None], x[None], x[0], x[0], x[0], x[0])
     with pytest.raises(AttributeError):
         hg.no_such_operator
+
+
+def test_outputs_over_inputs_are_refused():
+    """With everything else in order (each pointer a place of its own)."""
+    far = {n: P + (i + 1) * (1 << 24) for i, n in enumerate(("X", "W", "down", "up", "q", "k", "v"))}
+    st = {k: far[k] for k in ("X", "W", "down", "up")}
+    for over in (dict(Y=far["X"]), dict(Y=far["W"])):
+        assert call(lib.hgemm_lora, lora_args(**st, **over)) == BAD
+    st = {k: far[k] for k in ("q", "k", "v")}
+    for name in ("q", "k", "v"):
+        assert call(lib.hgemm_attn_prompt, attn_args(**st, out=far[name])) == BAD
