@@ -3,11 +3,13 @@
 Produces, next to this file:
   libhgemm_b200.so       the GEMM product: tcgen05 kernel, dispatcher, C ABI, NCCL row shards,
                          host-buffer pipeline, and the operators of a served attention layer
+  _operators.so          the operators' Python binding (checks of tensors, outputs, streams), built against
+                         the installed torch; skipped with a notice when there is none
   libhgemm_cublas_ref.so the cuBLAS comparator used by bench.py and the GPU tests
   libhgemm_cutlass_ref.so the CUTLASS SM100 comparator (third grid column, cross-check tests),
                          built when CUTLASS's headers are found (the copies vendored in the
                          flashinfer or tilelang wheels); skipped with a notice otherwise
-Both are compiled with `-gencode arch=compute_100a,code=sm_100a`; nvcc cross-compiles them on
+The CUDA libraries are compiled with `-gencode arch=compute_100a,code=sm_100a`; nvcc cross-compiles them on
 a machine without a GPU.
 """
 import os
@@ -23,6 +25,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 LIB = os.path.join(HERE, "libhgemm_b200.so")
 CUBLAS_LIB = os.path.join(HERE, "libhgemm_cublas_ref.so")
 CUTLASS_LIB = os.path.join(HERE, "libhgemm_cutlass_ref.so")
+BINDING = os.path.join(HERE, "_operators.so")
 
 
 def _cutlass_include():
@@ -64,6 +67,25 @@ def _run(cmd, verbose):
     subprocess.run(cmd, check=True)
 
 
+def _build_binding(nvcc, verbose):
+    """_operators.so: host code against torch's headers, found without importing torch."""
+    import importlib.util
+    import sysconfig
+    spec = importlib.util.find_spec("torch")
+    if not spec or not spec.submodule_search_locations:
+        print("note: torch not found; _operators.so (the operators' Python binding) skipped", flush=True)
+        return
+    torch = list(spec.submodule_search_locations)[0]
+    include = [INCLUDE, sysconfig.get_paths()["include"], os.path.join(torch, "include"),
+               os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+               os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")]
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"] +
+         ["-I" + d for d in include] + ["-o", BINDING, os.path.join(CSRC, "operators_py.cpp"),
+         "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
+         "-ltorch_python"],
+         verbose)
+
+
 def build(force=False, verbose=True, extra_flags=()):
     nvcc = _nvcc()
     common = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I" + INCLUDE,
@@ -75,6 +97,9 @@ def build(force=False, verbose=True, extra_flags=()):
                    os.path.join(CSRC, "ops_sm100.cuh"), os.path.join(INCLUDE, "hgemm_b200.h")]
     if force or _stale(LIB, deps):
         _run([nvcc] + common + ["-shared", "-o", LIB] + srcs + ["-ldl"], verbose)
+    if force or _stale(BINDING, [os.path.join(CSRC, "operators_py.cpp"),
+                                 os.path.join(INCLUDE, "hgemm_b200.h")]):
+        _build_binding(nvcc, verbose)
     csrc = [os.path.join(CSRC, "cublas_ref.cu")]
     if force or _stale(CUBLAS_LIB, csrc):
         _run([nvcc] + common + ["-shared", "-o", CUBLAS_LIB] + csrc + ["-lcublas"], verbose)
