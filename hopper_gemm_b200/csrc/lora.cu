@@ -9,7 +9,7 @@
 // lands in the same fp32 accumulators and Y is written and rounded once; an adapter costs its row
 // tiles rank / K of the GEMM. H is rounded to binary16 because it is a tcgen05 operand next to Up.
 //
-// Few tokens (decoding): bound by the bytes of W and of the adapters in use. W is the M operand of the
+// Few tokens (decoding, short batches; few_plan says when): bound by the bytes of W and of the adapters in use. W is the M operand of the
 // product, 128 of its columns to a CTA, and the tokens are its N; K is split over a cluster, so that
 // every SM pulls weights, and joined through distributed shared memory. The adapters run on the CUDA
 // cores in fp32, H in a launch of its own under whose feet the main kernel already starts, and Up's part
@@ -18,6 +18,7 @@
 // No counterpart in the reference.
 
 #include <algorithm>
+#include <cmath>
 
 #include "ops_sm100.cuh"
 
@@ -25,6 +26,7 @@ namespace hgemm {
 namespace {
 
 constexpr int kMaxRank = 256;
+constexpr int kSms = 148;          // what plans (and with them workspaces) reckon with
 constexpr int kTileRows = 128;     // rows of a shrink CTA
 constexpr int kMaxTileRows = 256;  // rows of a GEMM tile
 constexpr int kSegCache = 1024;    // segment starts kept in shared memory
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(256) lora_repair_kernel(const LoraParams p) {
 }
 
 // ------------------------------------------------------------------------------ few tokens
-constexpr int kFewTokens = 64;  // at most (the accumulator's columns)
+constexpr int kFewTokens = 64;  // of a CTA, at most (the accumulator's columns)
 constexpr int kFewCols = 128;   // columns of W in a CTA
 constexpr int kAddWarps = 8;    // that form the adapters' part and join the partial sums
 constexpr int kLoadWarps = 4;   // two for W, two for X, each every other stage
@@ -391,7 +393,8 @@ struct LoraFewParams {
   float *low;  // slices x tokens x rank: partial sums of X Down
   int tokens, N, K, rank, adapters, segments;
   int slices, slice_rows;   // K ranges of the first product
-  int n16;                  // tokens rounded up to 16
+  int n16;                  // tokens of a CTA, rounded up to 16
+  int chunks;               // of kFewTokens tokens
   int ksplit, num_kb, stages, share;  // share: tokens that a CTA of the cluster joins
   int whole_blocks;  // N % 64 == 0: tmW is (64 columns, K, column blocks), one box for 128 columns
   unsigned *status_word;
@@ -476,7 +479,9 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const int x_bytes = p.n16 * 128, stage_bytes = 2 * kBBytes + x_bytes;
   float *delta = reinterpret_cast<float *>(smem + p.stages * stage_bytes);  // share x kFewCols
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x % p.ksplit, n0 = blockIdx.x / p.ksplit * kFewCols;
+  const int split = blockIdx.x % p.ksplit, item = blockIdx.x / p.ksplit;
+  // CTAs of the same columns next to each other, so that W comes from HBM once.
+  const int n0 = item / p.chunks * kFewCols, first = item % p.chunks * kFewTokens;
   const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * split / p.ksplit);
   const int kb1 = static_cast<int>(static_cast<long long>(p.num_kb) * (split + 1) / p.ksplit);
   if (threadIdx.x == 0) {
@@ -498,7 +503,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&s_tmem);
   const OpWait wc{&s_abort, p.status_word, p.timeout_ns};
   // Tokens that this CTA joins, adds the adapters' part to and writes.
-  const int t0 = min(p.tokens, split * p.share), t1 = min(p.tokens, t0 + p.share);
+  const int end = min(p.tokens, first + kFewTokens);
+  const int t0 = min(end, first + split * p.share), t1 = min(end, t0 + p.share);
 
   // Warps 0.. 7 add, 8 issues products, 9.. load. A thread is held 400 to 600 cycles by a TMA load, which
   // for one thread and stages of 16 KB would be a third of what an SM can take in.
@@ -517,7 +523,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         const uint32_t bar = ptx::smem_u32(&s_full[st]), dst = base + st * stage_bytes;
         if (loads_x) {
           // (counted on the barrier before or after the bytes are announced)
-          ptx::tma_load_2d(&tmX, dst + 2 * kBBytes, bar, kb * 64, 0);
+          ptx::tma_load_2d(&tmX, dst + 2 * kBBytes, bar, kb * 64, first);
         } else {
           ptx::mbar_arrive_expect_tx(bar, stage_bytes);
           if (p.whole_blocks) {
@@ -564,7 +570,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     // What does not hang on the first product: whose token it is, and Up's rows into L2.
     for (int t = t0 + w; t < t1; t += kAddWarps) {
       const int a = warp_token_adapter(p.seg_start, p.seg_adapter, p.segments, p.adapters, t);
-      if (lane == 0) s_adapter[t] = a;
+      if (lane == 0) s_adapter[t - first] = a;
       if (a >= 0 && n0 + c < p.N)
         for (int r = lane >> 4; r < p.rank; r += 2)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(
@@ -573,7 +579,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     ptx::grid_wait();
     for (int t = t0 + w; t < t1; t += kAddWarps) {
       __syncwarp();
-      const int a = s_adapter[t];
+      const int a = s_adapter[t - first];
       float f[8] = {};
       if (a >= 0) {
         const float sc = p.scale[a];
@@ -646,7 +652,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) {
         const int tt = min(t + x * kStep, t1 - 1);
-        const uint32_t off = part_addr + (tt * kFewPart + col) * 4;
+        const uint32_t off = part_addr + ((tt - first) * kFewPart + col) * 4;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           if (k < p.ksplit) v[x][k] = ptx::ld_shared_cluster_f(ptx::mapa(off, k));
@@ -682,6 +688,44 @@ bool sizes_ok(int tokens, int N, int K, int rank, int adapters, int segments) {
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Few tokens: K ranges of the first product, so that the CTAs of all tokens fill the SMs a few times, of
+// 64 rows at least (a workspace of `tokens` tokens holds them).
+int few_slices(int tokens, int K) {
+  return std::max(1, std::min({kMaxSlices, 592 / tokens, K / 64}));
+}
+
+struct FewPlan {
+  bool use;
+  int tiles, chunks, most, n16, num_kb, ksplit, share, stage;
+};
+// How few tokens are run, and whether: depends on the sizes alone, since the workspace does.
+FewPlan few_plan(int tokens, int N, int K, int rank) {
+  FewPlan f;
+  f.tiles = (N + kFewCols - 1) / kFewCols;
+  f.chunks = (tokens + kFewTokens - 1) / kFewTokens;
+  f.most = std::min(tokens, kFewTokens);  // of a CTA
+  f.n16 = (f.most + 15) / 16 * 16;
+  f.num_kb = (K + 63) / 64;
+  f.stage = 2 * kBBytes + f.n16 * 128;
+  // Two CTAs to an SM, and of K as many ranges as they take, a power of two, with 4 k-blocks or more each
+  // (clusters of 6 left CTAs for a second wave: 26 us against 20 us with 4 at N = 6144).
+  const long long items = static_cast<long long>(f.tiles) * f.chunks;
+  f.ksplit = 1;
+  while (f.ksplit < 8 && 2 * f.ksplit * items <= 2 * kSms && f.num_kb >= 8 * f.ksplit) f.ksplit *= 2;
+  f.share = (f.most + f.ksplit - 1) / f.ksplit;
+  // This path reads Down and Up once for every token and splits K, the other takes an adapter's
+  // tokens together and does not split. In us, fitted to what both took at T x K x N, rank (this, the
+  // other): 128 x 4096 x 4096, 16: 18.6, 29.7; 64: 29.2, 30.4; 128: 45.9, 34.0; 256 x 4096 x 4096, 16: 28.2, 41.5;
+  // 64: 54.8, 41.4; 512 x 4096 x 4096, 16: 50.1, 44.8; 128 x 5760 x 880, 16: 14.0, 37.6; 128: 39.9, 40.9;
+  // 256 x 896 x 2016, 16: 17.2, 26.3; 64: 29.0, 26.1.
+  const double waves = std::ceil(static_cast<double>(items * f.ksplit) / (2 * kSms));
+  const double here = 8.0 + static_cast<double>(items) * f.num_kb * f.stage / 1.5e7 +  // W and X into the SMs
+                      2.0 * tokens * K * rank / 7.5e6 +                               // Down
+                      0.0088 * f.share * rank * waves;                                // Up
+  f.use = tokens <= 512 && here <= 22.0 + 0.17 * f.num_kb;
+  return f;
+}
 
 // Workspace, in order: the entries' tables, the list of odd blocks, the operand blocks. Sized for
 // 128-row tiles' tables and 256-row tiles' blocks, whichever the GEMM takes.
@@ -720,12 +764,6 @@ int check(const hgemm_lora_t *a) {
   return HGEMM_OK;
 }
 
-// Few tokens: K ranges of the first product, so that the CTAs of all tokens fill the SMs a few times, of
-// 64 rows at least (a workspace of `tokens` tokens holds them).
-int few_slices(int tokens, int K) {
-  return std::max(1, std::min({kMaxSlices, 592 / tokens, K / 64}));
-}
-
 int run_few(const hgemm_lora_t *a, const OpDevice &d, cudaStream_t stream) {
   LoraFewParams p;
   p.X = a->X;
@@ -744,19 +782,17 @@ int run_few(const hgemm_lora_t *a, const OpDevice &d, cudaStream_t stream) {
   p.segments = a->segments;
   p.slices = few_slices(a->tokens, a->K);
   p.slice_rows = (a->K + p.slices - 1) / p.slices;
-  p.n16 = (a->tokens + 15) / 16 * 16;
-  p.num_kb = (a->K + 63) / 64;
+  const FewPlan f = few_plan(a->tokens, a->N, a->K, a->rank);
+  p.chunks = f.chunks;
+  p.n16 = f.n16;
+  p.num_kb = f.num_kb;
+  p.ksplit = f.ksplit;
+  p.share = f.share;
   p.status_word = d.status_word;
   p.timeout_ns = d.timeout_ns;
-  // Two CTAs to an SM, and of K as many ranges as they take, a power of two, with 4 k-blocks or more each
-  const int tiles = (a->N + kFewCols - 1) / kFewCols;
-  // (clusters of 6 left CTAs for a second wave: 26 us against 20 us with 4 at N = 6144).
-  p.ksplit = 1;
-  while (p.ksplit < 8 && 2 * p.ksplit * tiles <= 2 * d.sm_count && p.num_kb >= 8 * p.ksplit) p.ksplit *= 2;
-  p.share = (a->tokens + p.ksplit - 1) / p.ksplit;
-  const int stage = 2 * kBBytes + p.n16 * 128, delta = p.share * kFewCols * 4;
-  p.stages = std::min(8, (kFewSmem - 1024 - delta) / stage);
-  const int smem = 1024 + p.stages * stage + delta;
+  const int delta = p.share * kFewCols * 4;
+  p.stages = std::min(8, (kFewSmem - 1024 - delta) / f.stage);
+  const int smem = 1024 + p.stages * f.stage + delta;
   CUtensorMap tw, tx;
   const unsigned long long wd[2] = {static_cast<unsigned long long>(a->N),
                                     static_cast<unsigned long long>(a->K)};
@@ -780,7 +816,7 @@ int run_few(const hgemm_lora_t *a, const OpDevice &d, cudaStream_t stream) {
   lora_low_kernel<<<p.tokens * p.slices, kLowThreads, 0, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return HGEMM_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.ksplit), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(f.tiles * f.chunks * f.ksplit), 1, 1);
   cfg.blockDim = dim3(kFewThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -808,7 +844,7 @@ int run(const hgemm_lora_t *a, cudaStream_t stream) {
   OpDevice d;
   st = op_device(&d);
   if (st != HGEMM_OK) return st;
-  if (a->tokens <= kFewTokens) return run_few(a, d, stream);
+  if (few_plan(a->tokens, a->N, a->K, a->rank).use) return run_few(a, d, stream);
   LoraParams p;
   st = lora_gemm_tile_rows(a->tokens, a->N, a->K, &p.tile_rows);
   if (st != HGEMM_OK) return st;
@@ -915,7 +951,7 @@ int hgemm_lora(const hgemm_lora_t *args, hgemm_stream_t stream) {
 size_t hgemm_lora_workspace_bytes(int tokens, int N, int K, int rank, int adapters, int segments) {
   if (!hgemm::sizes_ok(tokens, N, K, rank, adapters, segments)) return 0;
   if (tokens == 0 || N == 0 || adapters == 0 || segments == 0) return 0;
-  if (tokens <= hgemm::kFewTokens)
+  if (hgemm::few_plan(tokens, N, K, rank).use)
     return static_cast<size_t>(hgemm::few_slices(tokens, K)) * tokens * rank * sizeof(float);
   return hgemm::layout(tokens, N, rank, segments).total;
 }

@@ -80,6 +80,22 @@ def test_lora_tiles(cuda, T, N, K):
     check_lora(cuda, T, K, N, 72, 6, cut, [5, 0, -1, 3, 0, 4, 1], seed=N)
 
 
+@pytest.mark.parametrize("T,N,K", [(65, 72, 512), (65, 512, 512), (65, 8, 64), (65, 512, 64),
+                                   (40, 520, 136), (9, 136, 72)])
+def test_lora_tiles_of_few_tokens_at_a_high_rank(cuda, T, N, K):
+    """Few tokens whose adapters weigh more than the projection."""
+    cut = [0, T // 9, T // 5, T // 5 + 1, T // 2, T - T // 3, T - 2, T]
+    check_lora(cuda, T, K, N, 256, 6, cut, [5, 0, -1, 3, 0, 4, 1], seed=T)
+
+
+@pytest.mark.parametrize("T", [63, 64, 65, 127, 128, 129, 300, 511, 512, 513])
+@pytest.mark.parametrize("K,N", [(1032, 264), (64, 1160), (2048, 128)])
+def test_lora_tokens_in_chunks_of_64(cuda, T, K, N):
+    """Batches that one CTA's 64 tokens do not hold, at a low rank; requests across the chunks."""
+    cut = [0, 1, T // 3, T // 3 + 1, T - 20, T - 3]
+    check_lora(cuda, T, K, N, 8, 5, cut, [2, 4, -1, 0, 3], seed=T)
+
+
 @pytest.mark.parametrize("T", [40, 64, 200, 515])
 @pytest.mark.parametrize("r", [16, 96])
 def test_lora_segments(cuda, T, r):
