@@ -394,7 +394,6 @@ struct LoraFewParams {
   int tokens, N, K, rank, adapters, segments;
   int slices, slice_rows;   // K ranges of the first product
   int n16;                  // tokens of a CTA, rounded up to 16
-  int chunks;               // of kFewTokens tokens
   int ksplit, num_kb, stages, share;  // share: tokens that a CTA of the cluster joins
   int whole_blocks;  // N % 64 == 0: tmW is (64 columns, K, column blocks), one box for 128 columns
   unsigned *status_word;
@@ -479,9 +478,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const int x_bytes = p.n16 * 128, stage_bytes = 2 * kBBytes + x_bytes;
   float *delta = reinterpret_cast<float *>(smem + p.stages * stage_bytes);  // share x kFewCols
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x % p.ksplit, item = blockIdx.x / p.ksplit;
-  // CTAs of the same columns next to each other, so that W comes from HBM once.
-  const int n0 = item / p.chunks * kFewCols, first = item % p.chunks * kFewTokens;
+  const int split = blockIdx.x % p.ksplit, n0 = blockIdx.x / p.ksplit * kFewCols;
+  const int first = blockIdx.y * kFewTokens;
   const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * split / p.ksplit);
   const int kb1 = static_cast<int>(static_cast<long long>(p.num_kb) * (split + 1) / p.ksplit);
   if (threadIdx.x == 0) {
@@ -570,7 +568,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     // What does not hang on the first product: whose token it is, and Up's rows into L2.
     for (int t = t0 + w; t < t1; t += kAddWarps) {
       const int a = warp_token_adapter(p.seg_start, p.seg_adapter, p.segments, p.adapters, t);
-      if (lane == 0) s_adapter[t - first] = a;
+      if (lane == 0) s_adapter[t - t0] = a;
       if (a >= 0 && n0 + c < p.N)
         for (int r = lane >> 4; r < p.rank; r += 2)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(
@@ -579,7 +577,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     ptx::grid_wait();
     for (int t = t0 + w; t < t1; t += kAddWarps) {
       __syncwarp();
-      const int a = s_adapter[t - first];
+      const int a = s_adapter[t - t0];
       float f[8] = {};
       if (a >= 0) {
         const float sc = p.scale[a];
@@ -646,13 +644,13 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   if (adds && ok) {
     constexpr int kAhead = 2, kStep = kAddWarps / 4;  // tokens in flight of a thread; of the CTA
     const int col = threadIdx.x & (kFewCols - 1);
-    const uint32_t part_addr = ptx::smem_u32(part);
+    const uint32_t part_addr = ptx::smem_u32(part) - first * (kFewPart * 4);
     for (int t = t0 + static_cast<int>(threadIdx.x) / kFewCols; t < t1; t += kAhead * kStep) {
       float v[kAhead][8];
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) {
         const int tt = min(t + x * kStep, t1 - 1);
-        const uint32_t off = part_addr + ((tt - first) * kFewPart + col) * 4;
+        const uint32_t off = part_addr + (tt * kFewPart + col) * 4;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           if (k < p.ksplit) v[x][k] = ptx::ld_shared_cluster_f(ptx::mapa(off, k));
@@ -783,7 +781,6 @@ int run_few(const hgemm_lora_t *a, const OpDevice &d, cudaStream_t stream) {
   p.slices = few_slices(a->tokens, a->K);
   p.slice_rows = (a->K + p.slices - 1) / p.slices;
   const FewPlan f = few_plan(a->tokens, a->N, a->K, a->rank);
-  p.chunks = f.chunks;
   p.n16 = f.n16;
   p.num_kb = f.num_kb;
   p.ksplit = f.ksplit;
@@ -816,7 +813,7 @@ int run_few(const hgemm_lora_t *a, const OpDevice &d, cudaStream_t stream) {
   lora_low_kernel<<<p.tokens * p.slices, kLowThreads, 0, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return HGEMM_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(f.tiles * f.chunks * f.ksplit), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(f.tiles * f.ksplit), static_cast<unsigned>(f.chunks), 1);
   cfg.blockDim = dim3(kFewThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
