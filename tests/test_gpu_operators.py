@@ -4,6 +4,7 @@ import math
 import os
 import subprocess
 import sys
+import threading
 
 import pytest
 import torch
@@ -605,6 +606,50 @@ def test_explicit_workspace_on_another_stream(cuda):
         assert bool((ws[:256] == 0x7f).all()) and bool((ws[256 + need:] == 0x7f).all())
         with pytest.raises(cuda.HgemmError):
             cuda.attn_prompt(Q, K, V, cq, ck, workspace=ws[256:255 + need])
+
+
+def test_calls_from_several_threads(cuda):
+    """Four threads, a stream each; one adapter for two requests; tensors that ask for gradients."""
+    T = 70
+    X, W, down, up, scale = lora_case(T, 256, 384, 16, 3)
+    seg, ids = i32([0, 30, T]), i32([1, 1])
+    want = cuda.lora(X, W, down, up, scale, seg, ids)
+    with torch.inference_mode():
+        assert torch.equal(cuda.lora(X, W, down, up, scale, seg, ids), want)
+    assert torch.equal(cuda.lora(X.clone().requires_grad_(), W, down, up, scale, seg, ids), want)
+    torch.cuda.synchronize()
+    failed = []
+
+    def work():
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(50):
+                    got = cuda.lora(X, W, down, up, scale, seg, ids)
+                s.synchronize()
+                assert torch.equal(got, want)
+        except BaseException as e:  # noqa: B036  (handed to the test's own thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
+@pytest.mark.parametrize("over", [dict(scale=float("nan")), dict(scale=1e60), dict(scale="x"),
+                                  dict(stream="s"), dict(lse=3), dict(workspace=torch.zeros(4))])
+def test_attn_refuses_through_python(cuda, over):
+    q = torch.zeros((5, 4, 64), dtype=torch.float16, device=DEV)
+    with pytest.raises((cuda.HgemmError, TypeError, ValueError, AttributeError)):
+        cuda.attn_prompt(q, q[:, :2], q[:, 2:], i32([0, 5]), **over)
+    with pytest.raises(cuda.HgemmError):
+        cuda.attn_prompt(q, q[:, :2], q[:, 2:], i32([0, 5]), out=q)
+    with pytest.raises(cuda.HgemmError):
+        cuda.attn_prompt(q, q[:, :2], q[:, 2:], i32([]))
+    status_clear(cuda)
 
 
 def test_repeated_runs_are_identical(cuda):
