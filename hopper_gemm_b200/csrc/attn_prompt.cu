@@ -133,10 +133,16 @@ constexpr int kMaxChunks = 64;   // key ranges of a sequence
 // output is rescaled only when the maximum has grown past it. 2^8 times a weight below 1 stays far
 // inside binary16, and the fp32 sums do not care.
 constexpr float kLag = 8.0f;
+// That maximum is lowered by kRaise: a row's largest weight is 2^7 when the maximum is met and below 2^15 a lag behind
+// (binary16 ends at 65504), weights down to 2^-21 of the largest keep all of binary16's 11 bits, and the grid
+// of those below it is 2^-31 of it. (With the largest at 1 that grid is 2^-24: 131071 keys 15 below one in their
+// logarithm came out 0.2 to 3% off, 17.5 below it they were gone.) Weighted values and sums scale alike.
+constexpr float kRaise = 7.0f;
 
 // DB: 64-element blocks of head_dim in shared memory (head_dim <= 64 DB); TILES: row tiles of a CTA,
 // each with four softmax warps, a thread to a row; FINE: weights go into their product as two binary16
-// numbers each, the second of what the first left over, 22 bits in all.
+// numbers each, the second of what the first left over: 22 bits in all, down to 2^-10 of the row's largest
+// (the second's own grid is kRaise's 2^-31 of it).
 //
 // Blocks of 64 keys, because a tile's scores then have two places in TMEM: the next block's scores are
 // formed while a block's softmax runs, and no tile ever waits for the way from its weights through two
@@ -486,7 +492,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp, lane << 16
     const uint32_t tS = tmem + lane_base + i * (2 * kBlock);
     const uint32_t tO = tmem + lane_base + Cfg::O_COL + i * (DB * 64);
-    float m = -INFINITY;  // maximum that the weights are relative to (scaled)
+    float m = -INFINITY;  // what the weights are relative to (scaled): a maximum less kRaise
     float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};  // of the weights, in four parts
     bool ok = true;
     auto wait = [&](uint32_t bar, int phase, unsigned site) {
@@ -523,9 +529,9 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
         for (int e = 0; e < 32; e += 2)
           mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2;
-      const bool grow = top > m + kLag;  // true of the first key, from -infinity
+      const bool grow = top > m + (kRaise + kLag);  // true of the first key, from -infinity
       const float m_old = m;
-      if (grow) m = top;
+      if (grow) m = top - kRaise;
       if (u > 0 && __any_sync(0xffffffffu, grow)) {
         // O comes to rest with the block before: the scores behind this block's are formed after it.
         if (!(ok = u + 1 < n ? wait(sfull + 16 * i + 8 * ((u + 1) & 1), (u + 1) >> 1, kSiteAttnScores)

@@ -41,3 +41,29 @@ def test_norm_of_a_head_with_an_infinity(cuda, d, rot, interleaved):
     for x, y, name in ((q, got[0], "q"), (k, got[1], "k")):
         want, tol = ref.qk_norm_rope(x, w, pos, inv, axis, 1e-6, interleaved)
         ref.close(y, want, tol, f"{name} d{d} rot{rot}")
+
+
+# ------------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("gap", [8.0, 15.0, 17.5, 19.0])
+@pytest.mark.parametrize("rows,keys,hq,hkv", [(1, 131072, 8, 2), (1, 131072, 2, 2), (300, 131072, 2, 2), (17, 30000, 16, 1), (3000, 3000, 8, 2)])
+def test_attn_one_key_above_many_small_ones(cuda, gap, rows, keys, hq, hkv):
+    """Key 0 has the value 0 and scores `gap` above all others, whose values are 1: out = n e^-gap / (1 + n e^-gap).
+
+    A weight's rounding to binary16 is U16 of it, and 2^-32 of the maximum at least (2^-25 under an exponent raised by 7);
+    its exponential is 8 U32 off, the score itself exact; sums of n terms n U32; one rounding of the output."""
+    d, n = 128, keys - 1
+    q = torch.zeros((rows, hq, d), dtype=torch.float16, device=DEV)
+    k = torch.zeros((keys, hkv, d), dtype=torch.float16, device=DEV)
+    v = torch.ones((keys, hkv, d), dtype=torch.float16, device=DEV)
+    q[..., 3] = 1
+    k[0, :, 3] = gap
+    v[0] = 0
+    lse = torch.empty((rows, hq), device=DEV)
+    out = cuda.attn_prompt(q, k, v, i32([0, rows]), i32([0, keys]), scale=1.0, causal=False, lse=lse)
+    w = math.exp(-gap)
+    want = n * w / (1 + n * w)
+    tol = n * (w * (U16 + 8 * U32) + 2.0 ** -32) / (1 + n * w) + (n + 16) * U32 * want + U16 * want + ref.TINY
+    err = (out.double() - want).abs().max().item()
+    assert err <= tol, (err, tol, want)
+    z = math.log1p(n * w)
+    assert (lse.double() - (gap + z)).abs().max().item() <= (n + 16) * U32 + 8 * U32 * gap
