@@ -176,6 +176,10 @@ struct AttnCfg {
   static_assert(8 * (2 * STAGES + 1 + 6 * TILES) + 32 <= HEAD, "barriers");
 };
 
+// log2 of the sum of a key range whose scores are all -infinity: no missing keys, which have -infinity here.
+// Beside other ranges it weighs 0 (0 times an infinite value is NaN); a row of nothing else is 0 / 0.
+constexpr float kAllMinusInf = -3.402823466e38f;
+
 // Key ranges of a sequence with klen keys.
 __device__ __forceinline__ int chunks_of(const AttnParams &p, int klen) {
   if (p.chunk == 0) return 1;
@@ -667,7 +671,8 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
                      p.k + k0 * p.k_stride + static_cast<long long>(h) * p.head_dim,
                      p.v + k0 * p.v_stride + static_cast<long long>(h) * p.head_dim, p.k_stride, p.v_stride,
                      p.head_dim, p.scale2, kb, end);
-        const float ir = 1.0f / sum1.l;
+        // (a range of -infinity alone is handed over as it stands: zeros, or NaN of an infinite value)
+        const float ir = !whole && sum1.l == 0.0f ? 1.0f : 1.0f / sum1.l;
         if (4 * lane < p.head_dim) {
           const float4 f = make_float4(sum1.o.x * ir, sum1.o.y * ir, sum1.o.z * ir, sum1.o.w * ir);
           if (whole) {
@@ -683,7 +688,7 @@ __global__ void __launch_bounds__(AttnCfg<DB, TILES>::THREADS, AttnCfg<DB, TILES
             *reinterpret_cast<float4 *>(dst + 4 * lane) = f;
           }
         }
-        if (lane == src) lse2 = sum1.m + log2f(sum1.l);
+        if (lane == src) lse2 = !whole && sum1.l == 0.0f ? kAllMinusInf : sum1.m + log2f(sum1.l);
       }
       if (live) {
         if (!whole)
@@ -761,7 +766,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
       }
     }
   }
-  const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+  const bool none = top == kAllMinusInf;
+  const float inv = none ? __int_as_float(0x7fffffff) : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
   if (4 * lane < p.head_dim) {
     const __half2 a = __floats2half2_rn(o[0] * inv, o[1] * inv);
     const __half2 b = __floats2half2_rn(o[2] * inv, o[3] * inv);
@@ -769,7 +775,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p) {
                                4 * lane) = make_uint2(*reinterpret_cast<const uint32_t *>(&a),
                                                       *reinterpret_cast<const uint32_t *>(&b));
   }
-  if (lane == 0 && p.lse) p.lse[row] = (top + log2f(l)) * 0.69314718055994530942f;
+  if (lane == 0 && p.lse) p.lse[row] = none ? -INFINITY : (top + log2f(l)) * 0.69314718055994530942f;
 }
 
 // ------------------------------------------------------------------------------ host side

@@ -67,3 +67,41 @@ def test_attn_one_key_above_many_small_ones(cuda, gap, rows, keys, hq, hkv):
     assert err <= tol, (err, tol, want)
     z = math.log1p(n * w)
     assert (lse.double() - (gap + z)).abs().max().item() <= (n + 16) * U32 + 8 * U32 * gap
+
+
+@pytest.mark.parametrize("q_lens,k_lens,hq,hkv,d", [([70, 5], [70, 5], 4, 2, 64), ([1, 1], [9000, 40], 8, 2, 128), ([1], [700], 4, 4, 64),
+                                                    ([40], [5000], 4, 1, 128), ([2], [20000], 8, 2, 64)])
+def test_attn_rows_whose_scores_are_all_minus_infinity(cuda, q_lens, k_lens, hq, hkv, d):
+    """Seen keys of score -infinity are no missing keys: softmax is 0 / 0, so NaN, and the sum's logarithm -infinity,
+    whether the keys are split into ranges or not."""
+    tq, tk = sum(q_lens), sum(k_lens)
+    q, k, v = rand(1, (tq, hq, d)), rand(2, (tk, hkv, d)), rand(3, (tk, hkv, d))
+    q[..., 0] = q[..., 0].abs() + 1
+    k[:k_lens[0], 0, 0] = -math.inf
+    lse = torch.full((tq, hq), 7.0, device=DEV)
+    cq, ck = i32([0] + list(torch.tensor(q_lens).cumsum(0))), i32([0] + list(torch.tensor(k_lens).cumsum(0)))
+    out = cuda.attn_prompt(q, k, v, cq, ck, lse=lse)
+    g, n = hq // hkv, q_lens[0]
+    assert out[:n, :g].isnan().all()
+    assert (lse[:n, :g] == -math.inf).all()
+    assert out[:n, g:].isfinite().all() and out[n:].isfinite().all()
+
+
+@pytest.mark.parametrize("q_len,keys", [(1, 9000), (1, 700), (40, 5000), (200, 900)])
+def test_attn_some_ranges_of_minus_infinity(cuda, q_len, keys):
+    """Weights of exactly 0 in whole key ranges: they count for nothing, but 0 * infinity is NaN in the one column
+    where a value among them is infinite."""
+    hq, hkv, d = 4, 2, 64
+    q, k, v = rand(4, (q_len, hq, d)), rand(5, (keys, hkv, d)), rand(6, (keys, hkv, d))
+    q[..., 0] = q[..., 0].abs() + 1
+    dead = slice(0, keys * 3 // 4)
+    k[dead, :, 0] = -math.inf
+    want, tol, wl, tl = ref.attn(q, k[dead.stop:], v[dead.stop:], [q_len], [keys - dead.stop], d ** -0.5, True)
+    lse = torch.empty((q_len, hq), device=DEV)
+    out = cuda.attn_prompt(q, k, v, i32([0, q_len]), i32([0, keys]), lse=lse)
+    ref.close(out, want, tol, "dead keys")
+    ref.close(lse, wl, tl, "lse")
+    v[keys // 3, 1, 7] = math.inf
+    out = cuda.attn_prompt(q, k, v, i32([0, q_len]), i32([0, keys]))
+    want[:, 2:, 7] = math.nan
+    ref.close(out, want, tol, "an infinite value among them")
