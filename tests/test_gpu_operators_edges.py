@@ -105,3 +105,21 @@ def test_attn_some_ranges_of_minus_infinity(cuda, q_len, keys):
     out = cuda.attn_prompt(q, k, v, i32([0, q_len]), i32([0, keys]))
     want[:, 2:, 7] = math.nan
     ref.close(out, want, tol, "an infinite value among them")
+
+
+@pytest.mark.parametrize("rows,hq", [(1, 1), (1, 32), (16, 8)])
+def test_attn_few_rows_keep_22_bits_of_a_weight(cuda, rows, hq):
+    """Two keys whose weights differ by 2^-13, values 1 and -1: 1 - (1 - 2^-13) is lost where weights have 11 bits.
+    With 22 they are off by 2^-23, their exponentials by 8 U32 and the scores' product by 132 U32 of 2^-13."""
+    d, eps = 128, 2.0 ** -13
+    q = torch.zeros((rows, hq, d), dtype=torch.float16, device=DEV)
+    k = torch.zeros((2, hq, d), dtype=torch.float16, device=DEV)
+    v = torch.ones((2, hq, d), dtype=torch.float16, device=DEV)
+    q[..., 5] = 1
+    k[1, :, 5] = -eps
+    v[1] = -1
+    out = cuda.attn_prompt(q, k, v, i32([0, rows]), i32([0, 2]), scale=1.0, causal=False)
+    w = math.exp(-eps)
+    want = (1 - w) / (1 + w)
+    tol = (2.0 ** -23 + 8 * U32 + 132 * U32 * eps) + U16 * want + ref.TINY
+    assert (out.double() - want).abs().max().item() <= tol
