@@ -793,7 +793,7 @@ AttnPlan make_plan(int total_q, int total_k, int batch, int heads_q, int heads_k
   AttnPlan pl;
   const int group = heads_q / heads_kv;
   pl.tile_q = kRows / group;
-  const long long avg_q = (total_q + batch - 1) / batch, avg_k = (total_k + batch - 1) / batch;
+  const long long avg_q = (total_q + batch - 1ll) / batch, avg_k = (total_k + batch - 1ll) / batch;
   // Two row tiles to a CTA share the loaded keys, one tile each to two CTAs of an SM lets one's start
   // and end lie under the other's work: measured equal near 6000 keys a sequence at head_dim 128 (4 x 2048
   // tokens 174 and 166 us, 8192 tokens 475 and 495, 16384 tokens 1.89 and 2.06 ms), in favour of
@@ -846,6 +846,8 @@ int check(const hgemm_attn_prompt_t *a) {
   if (a->head_dim < 8 || a->head_dim > kMaxDim || a->head_dim % 8 != 0)
     return HGEMM_ERR_INVALID_ARG;
   if (!(a->scale >= 0.0f) || a->scale - a->scale != 0.0f) return HGEMM_ERR_INVALID_ARG;
+  if (a->total_q > kOpMaxRows || a->total_k > kOpMaxRows || a->batch > kOpMaxRows)
+    return HGEMM_ERR_TOO_LARGE;
   if (a->total_q == 0 || a->batch == 0) return HGEMM_OK;
   if (!a->q || !a->out || !a->cu_q) return HGEMM_ERR_INVALID_ARG;
   if (!a->cu_k && a->total_k != a->total_q) return HGEMM_ERR_INVALID_ARG;
@@ -978,7 +980,8 @@ size_t hgemm_attn_prompt_workspace_bytes(int total_q, int total_k, int batch, in
                                          int heads_kv, int head_dim) {
   if (total_q <= 0 || total_k < 0 || batch <= 0 || heads_kv < 1 || heads_q < heads_kv ||
       heads_q % heads_kv != 0 || heads_q / heads_kv > hgemm::kRows || head_dim < 8 ||
-      head_dim > hgemm::kMaxDim || head_dim % 8 != 0)
+      head_dim > hgemm::kMaxDim || head_dim % 8 != 0 || total_q > hgemm::kOpMaxRows ||
+      total_k > hgemm::kOpMaxRows || batch > hgemm::kOpMaxRows)
     return 0;
   return hgemm::make_plan(total_q, total_k, batch, heads_q, heads_kv, head_dim).workspace;
 }

@@ -690,6 +690,9 @@ bool sizes_ok(int tokens, int N, int K, int rank, int adapters, int segments) {
   return tokens >= 0 && N >= 0 && K >= 8 && N % 8 == 0 && K % 8 == 0 && rank >= 8 &&
          rank <= kMaxRank && rank % 8 == 0 && adapters >= 0 && segments >= 0;
 }
+bool too_large(int tokens, int N, int K, int segments) {
+  return tokens > kOpMaxRows || N > kOpMaxRows || K > kOpMaxRows || segments > kOpMaxSegments;
+}
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -753,6 +756,7 @@ Layout layout(int tokens, int N, int rank, int segments) {
 int check(const hgemm_lora_t *a) {
   if (!a || !sizes_ok(a->tokens, a->N, a->K, a->rank, a->adapters, a->segments))
     return HGEMM_ERR_INVALID_ARG;
+  if (too_large(a->tokens, a->N, a->K, a->segments)) return HGEMM_ERR_TOO_LARGE;
   if (a->tokens == 0 || a->N == 0) return HGEMM_OK;
   if (!a->X || !a->W || !a->Y || !op_aligned16(a->X) || !op_aligned16(a->W) || !op_aligned16(a->Y))
     return HGEMM_ERR_INVALID_ARG;
@@ -952,7 +956,9 @@ int hgemm_lora(const hgemm_lora_t *args, hgemm_stream_t stream) {
 }
 
 size_t hgemm_lora_workspace_bytes(int tokens, int N, int K, int rank, int adapters, int segments) {
-  if (!hgemm::sizes_ok(tokens, N, K, rank, adapters, segments)) return 0;
+  if (!hgemm::sizes_ok(tokens, N, K, rank, adapters, segments) ||
+      hgemm::too_large(tokens, N, K, segments))
+    return 0;
   if (tokens == 0 || N == 0 || adapters == 0 || segments == 0) return 0;
   if (hgemm::few_plan(tokens, N, K, rank).use)
     return static_cast<size_t>(hgemm::few_slices(tokens, K)) * tokens * rank * sizeof(float);

@@ -48,6 +48,11 @@ int lora_gemm_tile_rows(int M, int N, int K, int *rows);
 int lora_gemm(const __half *A, const __half *B, __half *C, int M, int N, int K, const LoraExt &ext,
               cudaStream_t stream);
 
+// The most rows, columns, sequences or segments of a call: the kernels reckon with them in 32 bits, up to a
+// grid's step or a tile behind the last one (a binary search adds two segment numbers).
+constexpr int kOpMaxRows = 0x7fffffff - 0xffff;
+constexpr int kOpMaxSegments = 1 << 30;
+
 inline bool op_aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Wait sites of the operators' kernels in the device status word (the GEMM uses 1..12).

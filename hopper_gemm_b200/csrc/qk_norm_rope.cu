@@ -238,7 +238,8 @@ int check(const hgemm_qk_norm_rope_t *a) {
     return HGEMM_ERR_INVALID_ARG;
   if (a->axes < 1 || (a->axes > 1 && a->rot_dim > 0 && !a->axis_of)) return HGEMM_ERR_INVALID_ARG;
   if (!(a->eps >= 0.0f)) return HGEMM_ERR_INVALID_ARG;
-  if (a->heads_q > kMaxHeads || a->heads_kv > kMaxHeads) return HGEMM_ERR_TOO_LARGE;
+  if (a->heads_q > kMaxHeads || a->heads_kv > kMaxHeads || a->tokens > kOpMaxRows)
+    return HGEMM_ERR_TOO_LARGE;
   if (a->tokens == 0 || a->heads_q + a->heads_kv == 0) return HGEMM_OK;
   if (a->rot_dim > 0 && (!a->positions || !a->inv_freq)) return HGEMM_ERR_INVALID_ARG;
   auto operand = [&](const void *in, const void *out, const void *w, long long is, long long os,

@@ -1,0 +1,65 @@
+"""CPU: sizes, workspaces and outputs that the attention layer's operators refuse, with every other argument in
+order and a place of its own for each pointer; no GPU calls (a refused call returns before the first)."""
+import ctypes
+
+import pytest
+
+import hopper_gemm_b200 as hg
+from hopper_gemm_b200 import lib
+from hopper_gemm_b200._native import HgemmAttnPrompt, HgemmLora, HgemmQkNormRope
+
+BAD, TOO_LARGE = hg.HGEMM_ERR_INVALID_ARG, 9
+LIMIT = 2 ** 31 - 2 ** 16  # the most rows of a call: 0x7fffffff - 0xffff
+
+
+def filled(cls, **values):
+    st = cls()
+    for i, (name, kind) in enumerate(cls._fields_):
+        if kind is ctypes.c_void_p:
+            setattr(st, name, (i + 1) << 44)  # never touched
+    for name, v in values.items():
+        setattr(st, name, v)
+    return st
+
+
+def lora_args(**over):
+    return filled(HgemmLora, **{**dict(workspace_bytes=1 << 43, tokens=16, N=64, K=64, rank=16, adapters=4,
+                                       segments=2), **over})
+
+
+def norm_args(**over):
+    return filled(HgemmQkNormRope, **{**dict(q_stride=1024, k_stride=256, q_out_stride=1024, k_out_stride=256,
+                                             tokens=16, heads_q=8, heads_kv=2, head_dim=128, rot_dim=128,
+                                             axes=1, eps=1e-6), **over})
+
+
+def attn_args(**over):
+    return filled(HgemmAttnPrompt, **{**dict(q_stride=1024, k_stride=256, v_stride=256, out_stride=1024,
+                                             workspace_bytes=1 << 43, total_q=16, total_k=16, batch=2, heads_q=8,
+                                             heads_kv=2, head_dim=128, causal=1, scale=0.1), **over})
+
+
+def status(st):
+    fn = {HgemmLora: lib.hgemm_lora, HgemmQkNormRope: lib.hgemm_qk_norm_rope,
+          HgemmAttnPrompt: lib.hgemm_attn_prompt}[type(st)]
+    return fn(ctypes.byref(st), None)
+
+
+@pytest.mark.parametrize("st", [
+    lora_args(tokens=LIMIT + 1), lora_args(tokens=2 ** 31 - 1), lora_args(N=2 ** 31 - 8), lora_args(K=2 ** 31 - 8),
+    lora_args(segments=2 ** 30 + 1), norm_args(tokens=LIMIT + 1), norm_args(tokens=2 ** 31 - 1),
+    norm_args(heads_q=(1 << 20) + 1, q_stride=1 << 32, q_out_stride=1 << 32),
+    attn_args(total_q=LIMIT + 1), attn_args(total_q=2 ** 31 - 1, total_k=2 ** 31 - 1), attn_args(total_k=2 ** 31 - 1),
+    attn_args(batch=2 ** 31 - 1)])
+def test_sizes_that_32_bits_would_not_hold_are_refused(st):
+    assert status(st) == TOO_LARGE
+    assert hg.last_status() == TOO_LARGE
+
+
+def test_workspaces_of_refused_and_of_the_largest_sizes():
+    lora, attn = lib.hgemm_lora_workspace_bytes, lib.hgemm_attn_prompt_workspace_bytes
+    assert lora(2 ** 31 - 1, 64, 64, 16, 4, 2) == 0 and lora(16, 64, 64, 16, 4, 2 ** 30 + 1) == 0
+    assert attn(2 ** 31 - 1, 2 ** 31 - 1, 2, 1, 1, 64) == 0 and attn(1, 2 ** 31 - 1, 1, 1, 1, 64) == 0
+    assert lora(LIMIT, 64, 64, 16, 4, 2) > 0
+    assert 0 < attn(1, LIMIT, 1, 8, 1, 64) < 1 << 20
+    assert 0 <= attn(LIMIT, LIMIT, 2 ** 20, 8, 1, 64) < 1 << 62
