@@ -31,6 +31,7 @@ namespace hgemm {
 namespace {
 
 constexpr int kMaxDim = 128;
+constexpr float kLog2e = 1.44269504088896340736f;
 
 struct AttnParams {
   const __half *q, *k, *v;
@@ -845,7 +846,8 @@ int check(const hgemm_attn_prompt_t *a) {
     return HGEMM_ERR_INVALID_ARG;
   if (a->head_dim < 8 || a->head_dim > kMaxDim || a->head_dim % 8 != 0)
     return HGEMM_ERR_INVALID_ARG;
-  if (!(a->scale >= 0.0f) || a->scale - a->scale != 0.0f) return HGEMM_ERR_INVALID_ARG;
+  const float scale2 = a->scale * kLog2e;
+  if (!(a->scale >= 0.0f) || scale2 - scale2 != 0.0f) return HGEMM_ERR_INVALID_ARG;
   if (a->total_q > kOpMaxRows || a->total_k > kOpMaxRows || a->batch > kOpMaxRows)
     return HGEMM_ERR_TOO_LARGE;
   if (a->total_q == 0 || a->batch == 0) return HGEMM_OK;
@@ -907,7 +909,7 @@ int run(const hgemm_attn_prompt_t *a, cudaStream_t stream) {
   p.head_dim = a->head_dim;
   p.causal = a->causal != 0;
   // scale 0 is a plain mean: any tiny factor gives it without 0 times the masked -infinity.
-  p.scale2 = std::max(a->scale * 1.44269504088896340736f, 1e-37f);
+  p.scale2 = std::max(a->scale * kLog2e, 1e-37f);
   p.dim16 = (a->head_dim + 15) / 16 * 16;
   p.status_word = d.status_word;
   p.timeout_ns = d.timeout_ns;

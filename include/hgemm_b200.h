@@ -289,10 +289,13 @@ int hgemm_qk_norm_rope(const hgemm_qk_norm_rope_t *args, hgemm_stream_t stream);
  * keys, the one before it all but the last, and so on (a whole prompt, one appended to earlier
  * keys, or a single token); a query without any key gets zeros and an lse of -infinity. Queries
  * behind cu_q[batch] are not touched. Scores, the running maximum and sum are fp32; the
- * weights of a row are rounded to binary16 as an operand of the second product: by at most 2^-11 of
- * themselves, or 2^-32 of the row's largest where that is more (calls of up to 128 rows total_q *
- * heads_q: 2^-22 of themselves, or 2^-32 of the largest). lse (fp32, total_q x heads_q, natural logarithm of the row's sum) may be NULL.
- * scale is finite and not negative; heads_q is a multiple of heads_kv, at most 128 times it; head_dim is a multiple of 8 up to 128.
+ * weights of a row are rounded to binary16 as an operand of the second product: by at most 2^-11
+ * of themselves, or 2^-32 of the row's largest where that is more (calls of up to 128 rows
+ * total_q * heads_q: 2^-22 of themselves, or 2^-32 of the largest). lse (fp32, total_q x heads_q,
+ * natural logarithm of the row's sum) may be NULL.
+ * scale is not negative; scale and log2(e) * scale are finite, and so have to be scores in these
+ * units in fp32. heads_q is a multiple of heads_kv, at most 128 times it; head_dim is a multiple
+ * of 8 up to 128.
  * Strides are halves between tokens, multiples of 8 and at least heads * head_dim; heads of a
  * token are adjacent; q, k, v and out start on 16-byte boundaries; out overlaps no input (other columns
  * of the same rows are fine). A row that sees an infinity or NaN, or whose tile holds one in a place masked

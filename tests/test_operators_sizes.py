@@ -63,3 +63,9 @@ def test_workspaces_of_refused_and_of_the_largest_sizes():
     assert lora(LIMIT, 64, 64, 16, 4, 2) > 0
     assert 0 < attn(1, LIMIT, 1, 8, 1, 64) < 1 << 20
     assert 0 <= attn(LIMIT, LIMIT, 2 ** 20, 8, 1, 64) < 1 << 62
+
+
+def test_a_scale_that_overflows_in_log2_units_is_refused():
+    """A masked score of -infinity, and a score of 0, would become NaN."""
+    for scale in (2.4e38, 3.4e38):
+        assert status(attn_args(scale=scale)) == BAD
