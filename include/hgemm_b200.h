@@ -239,7 +239,10 @@ int hgemm_plan(int M, int N, int K, float beta, int aligned16, int force_bm, int
  * one whose adapter is outside [0, adapters), gets X W alone. X W is summed in fp32 and the
  * adapter's part is added before the one rounding to binary16; X Down is rounded to binary16
  * (after the scale), as an operand of the second product, so |scale * X Down| must stay below
- * 65504. K, N and rank are multiples of 8, 8 <= rank <= 256; matrices are row-major, contiguous
+ * 65504. An infinity or NaN stays with the tokens that it belongs to. In an adapter's Up it makes
+ * the call slower: other tokens next to that adapter's are formed again in these columns (1200
+ * tokens of 4096 x 4096 beside an adapter of nothing else: 0.71 ms instead of 0.07).
+ * K, N and rank are multiples of 8, 8 <= rank <= 256; matrices are row-major, contiguous
  * and start on 16-byte boundaries. Y must not overlap the inputs. */
 typedef struct {
   const hgemm_half_t *X;    /* tokens x K */

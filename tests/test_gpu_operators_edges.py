@@ -123,3 +123,61 @@ def test_attn_few_rows_keep_22_bits_of_a_weight(cuda, rows, hq):
     want = (1 - w) / (1 + w)
     tol = (2.0 ** -23 + 8 * U32 + 132 * U32 * eps) + U16 * want + ref.TINY
     assert (out.double() - want).abs().max().item() <= tol
+
+
+# ------------------------------------------------------------------------------- lora
+def pass_us(fn):
+    best = math.inf
+    for _ in range(3):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        fn()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b) * 1e3)
+    return best
+
+
+def test_lora_a_request_of_nan_does_not_stall_the_others(cuda):
+    """Half of 1200 tokens are NaN: their rows are NaN and cost no more than a few calls' time."""
+    T, K, N, r, A = 1200, 4096, 4096, 16, 6
+    X, W = rand(1, (T, K)), rand(2, (K, N), K ** -0.5)
+    down, up = rand(3, (A, K, r), K ** -0.5), rand(4, (A, r, N), r ** -0.5)
+    scale = torch.ones(A, device=DEV)
+    seg, ids = i32([0, 200, 800, 1000, T]), i32([1, 4, 2, 0])
+    args = (W, down, up, scale, seg, ids)
+    want = cuda.lora(X, *args)
+    bad = X.clone()
+    bad[200:800] = math.nan
+    got = cuda.lora(bad, *args)
+    assert got[200:800].isnan().all()
+    assert torch.equal(got[:200], want[:200]) and torch.equal(got[800:], want[800:])
+    clean, stalled = pass_us(lambda: cuda.lora(X, *args)), pass_us(lambda: cuda.lora(bad, *args))
+    assert stalled < 10 * clean + 500, (clean, stalled)
+
+
+@pytest.mark.parametrize("what", [math.inf, math.nan])
+def test_lora_an_adapter_of_infinities_costs_the_others_little(cuda, what):
+    """One adapter's Up is not finite in some columns: its own tokens show it there, the other tokens of its
+    row tiles are formed again, in a few calls' time."""
+    T, K, N, r, A = 1200, 4096, 4096, 24, 6
+    X, W = rand(1, (T, K)), rand(2, (K, N), K ** -0.5)
+    down, up = rand(3, (A, K, r), K ** -0.5), rand(4, (A, r, N), r ** -0.5)
+    scale = torch.ones(A, device=DEV)
+    starts, ids = [0, 200, 210, 800, 1000, T], [1, 4, 2, -1, 0]
+    broken = [5, 64, 1000, 1001, N - 1]
+    want, tol = ref.lora(X, W, down, up, scale, ref.token_adapters(T, starts, ids, A))
+    up[4, :, broken] = what
+    call = lambda: cuda.lora(X, W, down, up, scale, i32(starts), i32(ids))  # noqa: E731
+    got = call()
+    assert not got[200:210][:, broken].isfinite().any()
+    want[200:210, broken] = got[200:210, broken].double()
+    ref.close(got, want, tol, "other tokens")
+    up[4] = what
+    got = call()
+    assert not got[200:210].isfinite().any()
+    want[200:210] = got[200:210].double()
+    ref.close(got, want, tol, "all columns")
+    us = pass_us(call)
+    print("one adapter of infinities:", us, "us")
+    assert us < 20000, us
