@@ -59,7 +59,7 @@ struct LoraParams {
   int tile_rows, chunks;    // rows of a GEMM tile; 64-column blocks of H
   int groups, per_group;    // adapters of a tile are taken `per_group` at a time by `groups` CTAs
   int ksplit, num_kb;
-  int entries;
+  int entries, per_tile;    // of all tiles; of each, or 0: as its segments say
   int *base, *count, *adapter;
   __half *low;
   unsigned *odd_count;
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                        : -1;
   if (threadIdx.x == 0) {
     // Tiles before this one have at most one entry each more than the segments that begin in them.
-    s_base = tile + starts_upto(starts, p.segments, tile0 - 1);
+    s_base = p.per_tile ? tile * p.per_tile : tile + starts_upto(starts, p.segments, tile0 - 1);
   }
   __syncthreads();
   if (cached) {
@@ -802,21 +802,34 @@ FewPlan few_plan(int tokens, int N, int K, int rank) {
   return f;
 }
 
+// Entries of a call (an adapter of a row tile each): a tile has at most as many as adapters, and all have
+// at most one each more than segments that begin in them. The fewer of the two decides (4096 requests of one token over
+// 8 adapters at rank 64: 4 MB of operand blocks instead of 135).
+struct Entries {
+  int per_tile;  // 0: as the segments say
+  long long all;
+};
+Entries entries_of(int tokens, int tile_rows, int adapters, int segments) {
+  const long long tiles = (tokens + tile_rows - 1) / tile_rows;
+  const int most = std::min(tile_rows, adapters);
+  if (tiles * most <= tiles + segments) return {most, tiles * most};
+  return {0, tiles + segments};
+}
+
 // Workspace, in order: the entries' tables, the list of odd blocks, the operand blocks. Sized for
 // 128-row tiles' tables and 256-row tiles' blocks, whichever the GEMM takes.
 struct Layout {
   size_t tables, list, low, total;
-  long long entries128, entries256;
 };
-Layout layout(int tokens, int N, int rank, int segments) {
+Layout layout(int tokens, int N, int rank, int adapters, int segments) {
   Layout l;
-  const long long t128 = (tokens + 127) / 128, t256 = (tokens + 255) / 256;
-  l.entries128 = t128 + segments;
-  l.entries256 = t256 + segments;
-  l.tables = up256(static_cast<size_t>(2 * t128 + l.entries128 + 1) * sizeof(int));
+  const long long t128 = (tokens + 127) / 128;
+  const long long e128 = entries_of(tokens, 128, adapters, segments).all;
+  const long long e256 = entries_of(tokens, 256, adapters, segments).all;
+  l.tables = up256(static_cast<size_t>(2 * t128 + std::max(e128, e256) + 1) * sizeof(int));
   l.list = up256(static_cast<size_t>((tokens + 31) / 32) * ((N + 63) / 64) * 8);
   const size_t row = static_cast<size_t>((rank + 63) / 64) * 64 * sizeof(__half);
-  l.low = static_cast<size_t>(std::max(l.entries128 * 128, l.entries256 * 256)) * row;
+  l.low = static_cast<size_t>(std::max(e128 * 128, e256 * 256)) * row;
   l.total = l.tables + l.list + l.low;
   return l;
 }
@@ -940,10 +953,11 @@ int run(const hgemm_lora_t *a, cudaStream_t stream) {
   p.chunks = (a->rank + 63) / 64;
   p.num_kb = (a->K + 63) / 64;
   const int tiles = (a->tokens + p.tile_rows - 1) / p.tile_rows;
-  const Layout l = layout(a->tokens, a->N, a->rank, a->segments);
-  const long long entries = p.tile_rows == 128 ? l.entries128 : l.entries256;
-  if (entries * p.chunks * p.tile_rows > 0x7fffffffll) return HGEMM_ERR_TOO_LARGE;
-  p.entries = static_cast<int>(entries);
+  const Layout l = layout(a->tokens, a->N, a->rank, a->adapters, a->segments);
+  const Entries e = entries_of(a->tokens, p.tile_rows, a->adapters, a->segments);
+  if (e.all * p.chunks * p.tile_rows > 0x7fffffffll) return HGEMM_ERR_TOO_LARGE;
+  p.per_tile = e.per_tile;
+  p.entries = static_cast<int>(e.all);
   char *ws = static_cast<char *>(a->workspace);
   p.odd_count = reinterpret_cast<unsigned *>(ws);
   p.base = reinterpret_cast<int *>(ws) + 1;
@@ -1030,7 +1044,7 @@ size_t hgemm_lora_workspace_bytes(int tokens, int N, int K, int rank, int adapte
   if (tokens == 0 || N == 0 || adapters == 0 || segments == 0) return 0;
   if (hgemm::few_plan(tokens, N, K, rank).use)
     return static_cast<size_t>(hgemm::few_slices(tokens, K)) * tokens * rank * sizeof(float);
-  return hgemm::layout(tokens, N, rank, segments).total;
+  return hgemm::layout(tokens, N, rank, adapters, segments).total;
 }
 
 }  // extern "C"

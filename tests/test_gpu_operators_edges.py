@@ -181,3 +181,50 @@ def test_lora_an_adapter_of_infinities_costs_the_others_little(cuda, what):
     us = pass_us(call)
     print("one adapter of infinities:", us, "us")
     assert us < 20000, us
+
+
+# ------------------------------------------------------------------------------- lora: tables and tiles
+@pytest.mark.parametrize("T,A,segs,K,N", [
+    (1500, 5, 1500, 256, 512), (1500, 1100, 1500, 256, 512), (1500, 1100, 9, 256, 512),
+    (4100, 3, 4100, 512, 4096), (4100, 40, 70, 512, 4096), (1025, 2, 1024, 64, 264), (700, 300, 1023, 128, 136)])
+def test_lora_tables_of_many_segments_and_adapters(cuda, T, A, segs, K, N):
+    """More segments and adapters than the tables in shared memory hold, entries by tiles and by segments, several
+    adapters to a tile, empty segments."""
+    r = 24
+    X, W = rand(T, (T, K)), rand(A, (K, N), K ** -0.5)
+    down, up = rand(segs, (A, K, r), K ** -0.5), rand(K, (A, r, N), r ** -0.5)
+    scale = torch.rand(A, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)) + 0.5
+    cut = [min(T, s * T // segs + (s % 3 == 1 and segs < T)) for s in range(segs)] + [T]
+    ids = [(s * 7919) % (A + 1) - 1 for s in range(segs)]
+    got = cuda.lora(X, W, down, up, scale, i32(cut), i32(ids))
+    want, tol = ref.lora(X, W, down, up, scale, ref.token_adapters(T, cut, ids, A))
+    ref.close(got, want, tol, "lora")
+    assert cuda.device_status(clear=True) == (0, 0)
+
+
+TILES = {(1, 64): (700, 520, 1024), (1, 128): (700, 520, 264), (1, 256): (700, 4104, 512),
+         (2, 128): (777, 2056, 2048), (2, 256): (700, 6144, 1024), (2, 512): (1037, 6144, 1024)}
+
+
+@pytest.mark.parametrize("tile", sorted(TILES))
+def test_lora_infinities_do_not_leak_in_any_tile(cuda, tile):
+    """Columns of one adapter's Up are infinite: in every tile of the GEMM its blocks are listed and the other
+    requests' rows formed again."""
+    T, N, K = TILES[tile]
+    r, A = 72, 4
+    plan = cuda.plan(T, N, K)
+    assert (plan["pair"], plan["tile_n"]) == tile and plan["ksplit"] == 1
+    X, W = rand(T, (T, K)), rand(N, (K, N), K ** -0.5)
+    down, up = rand(3, (A, K, r), K ** -0.5), rand(4, (A, r, N), r ** -0.5)
+    scale = torch.ones(A, device=DEV)
+    cut, ids = [0, T // 3, T // 3 + 5, T - 70, T - 1, T], [0, 2, 1, -1, 3]
+    want, tol = ref.lora(X, W, down, up, scale, ref.token_adapters(T, cut, ids, A))
+    broken = [0, 9, N // 2, N // 2 + 1, N - 1]
+    up[2, :, broken] = math.inf
+    up[3, 5, broken] = -math.inf
+    got = cuda.lora(X, W, down, up, scale, i32(cut), i32(ids))
+    for own in (slice(T // 3, T // 3 + 5), slice(T - 1, T)):
+        assert not got[own][:, broken].isfinite().any()
+        want[own, broken] = got[own, broken].double()
+    ref.close(got, want, tol, f"tile {tile}")
+    assert cuda.device_status(clear=True) == (0, 0)

@@ -69,3 +69,12 @@ def test_a_scale_that_overflows_in_log2_units_is_refused():
     """A masked score of -infinity, and a score of 0, would become NaN."""
     for scale in (2.4e38, 3.4e38):
         assert status(attn_args(scale=scale)) == BAD
+
+
+@pytest.mark.parametrize("T,N,K,r,A,S,most", [
+    (4096, 4096, 4096, 64, 8, 4096, 8 << 20), (8192, 4096, 4096, 128, 32, 8192, 80 << 20),
+    (4096, 4096, 4096, 64, 1 << 20, 1, 8 << 20), (1 << 20, 4096, 4096, 16, 1 << 20, 3, 256 << 20)])
+def test_lora_workspace_goes_by_the_adapters_too(T, N, K, r, A, S, most):
+    """Operand blocks of 128 or 256 rows of 64 columns for each adapter of each row tile: min(adapters, one more than
+    the segments) of them at most, not one for every segment."""
+    assert lib.hgemm_lora_workspace_bytes(T, N, K, r, A, S) <= most
