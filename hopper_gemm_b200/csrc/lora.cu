@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // shared memory and W read in whole rows. With nothing listed this returns at once.
 constexpr int kRepairThreads = 256;
 constexpr int kRepairK = 64;  // of X at a time
-__global__ void __launch_bounds__(kRepairThreads) lora_repair_kernel(const LoraParams p) {
+__global__ void __launch_bounds__(kRepairThreads, 2) lora_repair_kernel(const LoraParams p) {
   __shared__ int s_least[64], s_most[64];  // adapters with an infinity or NaN in a column of Up
   __shared__ int s_own[32], s_entry[32];   // a row's adapter, and its place among the tile's
   __shared__ float s_x[32][kRepairK];
