@@ -775,7 +775,7 @@ struct FewPlan {
   int tiles, chunks, most, n16, num_kb, ksplit, share, stage;
 };
 // How few tokens are run, and whether: depends on the sizes alone, since the workspace does.
-FewPlan few_plan(int tokens, int N, int K, int rank) {
+FewPlan few_plan(int tokens, int N, int K, int rank, int adapters, int segments) {
   FewPlan f;
   f.tiles = (N + kFewCols - 1) / kFewCols;
   f.chunks = (tokens + kFewTokens - 1) / kFewTokens;
@@ -789,16 +789,38 @@ FewPlan few_plan(int tokens, int N, int K, int rank) {
   f.ksplit = 1;
   while (f.ksplit < 8 && 2 * f.ksplit * items <= 2 * kSms && f.num_kb >= 8 * f.ksplit) f.ksplit *= 2;
   f.share = (f.most + f.ksplit - 1) / f.ksplit;
-  // This path reads Down and Up once for every token and splits K, the other takes an adapter's
-  // tokens together and does not split. In us, fitted to what both took at T x K x N, rank (this, the
-  // other): 128 x 4096 x 4096, 16: 18.6, 29.7; 64: 29.2, 30.4; 128: 45.9, 34.0; 256 x 4096 x 4096, 16: 28.2, 41.5;
-  // 64: 54.8, 41.4; 512 x 4096 x 4096, 16: 50.1, 44.8; 128 x 5760 x 880, 16: 14.0, 37.6; 128: 39.9, 40.9;
-  // 256 x 896 x 2016, 16: 17.2, 26.3; 64: 29.0, 26.1.
+  // This path reads Down and Up once for every token, W once for every 64, and splits K; the other takes an
+  // adapter's tokens together, in row tiles, and does not split. Both in us, fitted to eager calls of 1 to 512 tokens, ranks
+  // of 8 to 128, one to 200 adapters at 36 sizes of K x N from 536 x 1440 to 19192 x 33352 and 4096 x 128256, each in
+  // both paths: at 95% of 2774 points the rule takes the faster one or one within 5% of it, on average 0.8% is lost,
+  // at worst 55% (200 tokens of as many adapters, rank 8, 5088 x 17840). This path and the other, in us:
+  //    K x N          tokens, rank, adapters: us, us
+  //    4096 x 4096    1, 16, 1: 13.6, 32.8    128, 16, 1: 21.1, 32.6   256, 64, 32: 70.6, 57.4   512, 16, 1: 57.4, 44.7
+  //    4096 x 28672   1, 16, 1: 39.4, 57.7    48, 16, 1: 52.0, 48.9    48, 64, 32: 107, 82       128, 16, 1: 125, 51
+  //    14336 x 4096   1, 16, 1: 28.2, 103     48, 64, 32: 53.4, 95.6   192, 64, 32: 131, 116
+  //    8192 x 57344   1, 16, 1: 139, 192      48, 16, 1: 191, 166
+  const int rows = (tokens + kTileRows - 1) / kTileRows, chunks = (rank + 63) / 64;
+  const int distinct = std::min({tokens, adapters, segments});  // adapters, at most
+  const double w_mb = 2e-6 * K * N, adapter_mb = 2e-6 * distinct * rank * (static_cast<double>(K) + N);
   const double waves = std::ceil(static_cast<double>(items * f.ksplit) / (2 * kSms));
-  const double here = 8.0 + static_cast<double>(items) * f.num_kb * f.stage / 1.5e7 +  // W and X into the SMs
-                      2.0 * tokens * K * rank / 7.5e6 +                               // Down
-                      0.0088 * f.share * rank * waves;                                // Up
-  f.use = tokens <= 512 && here <= 22.0 + 0.17 * f.num_kb;
+  const int slices = few_slices(tokens, K);
+  const double here = 4.6 + 6.3 * waves +                                    // launches; a CTA's start and end
+                      0.10 * waves * f.num_kb / f.ksplit * f.stage / 16384 +  // W and X into an SM
+                      0.123 * f.chunks * w_mb + 0.183 * adapter_mb +          // out of memory or L2
+                      9.3e-5 * K / slices * rank * std::ceil(tokens * slices / (8.0 * kSms)) +  // Down for each token
+                      7.5e-8 * tokens * N * rank + 0.0066 * f.share * rank * waves;             // Up, its sums
+  const int of_tile = std::min(distinct, kTileRows);  // adapters of a row tile, at most
+  const int per_group = std::max(1, kBlocks / chunks);
+  const double shrinks = static_cast<double>((of_tile + per_group - 1) / per_group) * rows;  // products X Down
+  double ksplit = 1.0;
+  while (ksplit < 8.0 && 2.0 * ksplit * shrinks <= kSms && f.num_kb >= 8.0 * ksplit) ksplit *= 2.0;
+  const double tiles = static_cast<double>(rows) * ((N + 255) / 256) / kSms;  // of an SM
+  const double other = 6.7 + 9.9 * std::ceil(tiles) +
+                       std::max(1.0, tiles) * (0.166 * f.num_kb + 0.60 * chunks * of_tile) +
+                       0.122 * w_mb + 0.088 * adapter_mb +
+                       0.234 * std::ceil(shrinks * ksplit / kSms) * f.num_kb / ksplit +  // H, the longest
+                       0.23 * shrinks * f.num_kb / kSms;                                 // and all of it
+  f.use = tokens <= 512 && here <= other;
   return f;
 }
 
@@ -871,7 +893,7 @@ int run_few(const hgemm_lora_t *a, const OpDevice &d, cudaStream_t stream) {
   p.segments = a->segments;
   p.slices = few_slices(a->tokens, a->K);
   p.slice_rows = (a->K + p.slices - 1) / p.slices;
-  const FewPlan f = few_plan(a->tokens, a->N, a->K, a->rank);
+  const FewPlan f = few_plan(a->tokens, a->N, a->K, a->rank, a->adapters, a->segments);
   p.n16 = f.n16;
   p.num_kb = f.num_kb;
   p.ksplit = f.ksplit;
@@ -932,7 +954,7 @@ int run(const hgemm_lora_t *a, cudaStream_t stream) {
   OpDevice d;
   st = op_device(&d);
   if (st != HGEMM_OK) return st;
-  if (few_plan(a->tokens, a->N, a->K, a->rank).use) return run_few(a, d, stream);
+  if (few_plan(a->tokens, a->N, a->K, a->rank, a->adapters, a->segments).use) return run_few(a, d, stream);
   LoraParams p;
   st = lora_gemm_tile_rows(a->tokens, a->N, a->K, &p.tile_rows);
   if (st != HGEMM_OK) return st;
@@ -1042,7 +1064,7 @@ size_t hgemm_lora_workspace_bytes(int tokens, int N, int K, int rank, int adapte
       hgemm::too_large(tokens, N, K, segments))
     return 0;
   if (tokens == 0 || N == 0 || adapters == 0 || segments == 0) return 0;
-  if (hgemm::few_plan(tokens, N, K, rank).use)
+  if (hgemm::few_plan(tokens, N, K, rank, adapters, segments).use)
     return static_cast<size_t>(hgemm::few_slices(tokens, K)) * tokens * rank * sizeof(float);
   return hgemm::layout(tokens, N, rank, adapters, segments).total;
 }

@@ -228,3 +228,18 @@ def test_lora_infinities_do_not_leak_in_any_tile(cuda, tile):
         want[own, broken] = got[own, broken].double()
     ref.close(got, want, tol, f"tile {tile}")
     assert cuda.device_status(clear=True) == (0, 0)
+
+
+@pytest.mark.parametrize("T,K,N,r", [(1, 264, 28672, 16), (1, 64, 128256, 8), (48, 1024, 14336, 32), (70, 520, 33352, 16),
+                                     (16, 14336, 136, 64), (200, 14336, 264, 16), (130, 512, 28672, 64)])
+def test_lora_wide_and_long_projections(cuda, T, K, N, r):
+    A = 6
+    X, W = rand(T, (T, K)), rand(N, (K, N), K ** -0.5)
+    down, up = rand(K, (A, K, r), K ** -0.5), rand(r, (A, r, N), r ** -0.5)
+    scale = torch.rand(A, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)) + 0.5
+    cut, ids = list(range(T + 1)), [(5 * t) % (A + 1) - 1 for t in range(T)]
+    for cut, ids in ((cut, ids), ([0, T // 2, T], [3, 1])):
+        got = cuda.lora(X, W, down, up, scale, i32(cut), i32(ids))
+        want, tol = ref.lora(X, W, down, up, scale, ref.token_adapters(T, cut, ids, A))
+        ref.close(got, want, tol, f"lora {T}x{K}x{N}")
+    assert cuda.device_status(clear=True) == (0, 0)

@@ -78,3 +78,29 @@ def test_lora_workspace_goes_by_the_adapters_too(T, N, K, r, A, S, most):
     """Operand blocks of 128 or 256 rows of 64 columns for each adapter of each row tile: min(adapters, one more than
     the segments) of them at most, not one for every segment."""
     assert lib.hgemm_lora_workspace_bytes(T, N, K, r, A, S) <= most
+
+
+def few_tokens(T, N, K, r, A, S):
+    """Whether these sizes take the path of few tokens, whose workspace is its partial sums of X Down."""
+    slices = max(1, min(16, 592 // T, K // 64))
+    return lib.hgemm_lora_workspace_bytes(T, N, K, r, A, S) == slices * T * r * 4
+
+
+@pytest.mark.parametrize("K,N", [(4096, 4096), (4096, 14336), (4096, 28672), (14336, 4096), (28672, 8192),
+                                 (8192, 57344), (4096, 128256)])
+def test_lora_path_goes_by_the_width_of_the_projection(K, N):
+    """One token is W's bytes, which the path that splits K streams at any width (4096 x 28672: 39 us against 58, 8192 x
+    57344: 139 against 192); 128 tokens of a wide projection are read twice there (4096 x 28672: 125 us against 51)."""
+    assert few_tokens(1, N, K, 16, 1, 1)
+    assert few_tokens(1, N, K, 64, 32, 1)
+    if N >= 14336:
+        assert not few_tokens(128, N, K, 16, 1, 1)
+        assert not few_tokens(256, N, K, 64, 32, 256)
+
+
+def test_lora_path_goes_by_the_adapters():
+    """Every adapter of a row tile is more k-blocks there (64 tokens x 4096 x 4096 of 32 adapters, rank 64: 45 us against
+    25 here), of one adapter's tokens it takes all at once (512 tokens, rank 16: 45 against 57)."""
+    assert few_tokens(64, 4096, 4096, 64, 32, 64)
+    assert not few_tokens(512, 4096, 4096, 16, 1, 1)
+    assert few_tokens(256, 880, 5760, 64, 32, 256)
