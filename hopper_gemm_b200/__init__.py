@@ -17,6 +17,7 @@ launch. Next to the projections of an attention layer (no counterpart in the ref
 Everything goes through the C ABI of libhgemm_b200.so; there is no fallback path.
 """
 import ctypes
+import importlib.util
 
 from . import _native
 from ._native import (HGEMM_ERR_DEVICE_TIMEOUT, HGEMM_ERR_INVALID_ARG, HGEMM_OK,  # noqa: F401
@@ -25,15 +26,32 @@ from ._native import (HGEMM_ERR_DEVICE_TIMEOUT, HGEMM_ERR_INVALID_ARG, HGEMM_OK,
 __all__ = ["solve", "launch", "launch_tuned", "launch_host", "gemm", "plan", "last_status",
            "status_string",
            "device_status", "release", "HgemmError", "set_wait_timeout_ns",
-           "selftest_wait_timeout", "shard_rows", "lora", "qk_norm_rope", "attn_prompt"]
+           "selftest_wait_timeout", "shard_rows"]
 
 _OPERATORS = ("lora", "qk_norm_rope", "attn_prompt")
+
+
+def _have_operators():
+    """Whether torch and the operators' binding are installed (imports neither)."""
+    def there(name):
+        try:
+            return importlib.util.find_spec(name) is not None
+        except (ImportError, ValueError):
+            return False
+    return there("torch") and there(__name__ + "._operators")
+
+
+if _have_operators():  # `from hopper_gemm_b200 import *` works without them too
+    __all__ += _OPERATORS
 
 
 def __getattr__(name):
     # The operators take torch tensors; torch is imported with the first of them.
     if name in _OPERATORS:
-        from . import operators
+        try:
+            from . import operators
+        except ImportError as e:
+            raise AttributeError(f"module {__name__!r} has no attribute {name!r} here: {e}") from e
         for n in _OPERATORS:
             globals()[n] = getattr(operators, n)
         return globals()[name]

@@ -1,6 +1,9 @@
 """CPU: sizes, workspaces and outputs that the attention layer's operators refuse, with every other argument in
 order and a place of its own for each pointer; no GPU calls (a refused call returns before the first)."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -104,3 +107,38 @@ def test_lora_path_goes_by_the_adapters():
     assert few_tokens(64, 4096, 4096, 64, 32, 64)
     assert not few_tokens(512, 4096, 4096, 16, 1, 1)
     assert few_tokens(256, 880, 5760, 64, 32, 256)
+
+
+WITHOUT = """
+import importlib.abc, sys
+class Gone(importlib.abc.MetaPathFinder):
+    def find_spec(self, name, path=None, target=None):
+        if name in {names}:
+            raise ModuleNotFoundError("No module named " + repr(name), name=name)
+if {blank}:
+    sys.modules.update(dict.fromkeys({names}))
+else:
+    sys.meta_path.insert(0, Gone())
+from hopper_gemm_b200 import *
+import hopper_gemm_b200 as hg
+assert callable(launch) and hg.plan(64, 64, 64)["path"] == 1
+assert not hasattr(hg, "lora") and "lora" not in globals() and "torch" not in [m for m in sys.modules if sys.modules[m]]
+"""
+
+
+@pytest.mark.parametrize("names", [["torch"], ["hopper_gemm_b200._operators"]])
+@pytest.mark.parametrize("blank", [False, True])
+def test_the_package_works_without_torch_or_the_binding(names, blank):
+    """Star import and everything but the operators, which are no attributes then."""
+    code = WITHOUT.format(names=names, blank=blank)
+    if names != ["torch"]:
+        code = code.replace(' and "torch" not in [m for m in sys.modules if sys.modules[m]]', "")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0, run.stderr[-2000:]
+
+
+def test_star_import_brings_the_operators():
+    names = {}
+    exec("from hopper_gemm_b200 import *", names)
+    assert callable(names["lora"]) and callable(names["qk_norm_rope"]) and callable(names["attn_prompt"])
