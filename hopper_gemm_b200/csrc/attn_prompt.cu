@@ -854,20 +854,29 @@ int check(const hgemm_attn_prompt_t *a) {
   if (!a->q || !a->out || !a->cu_q) return HGEMM_ERR_INVALID_ARG;
   if (!a->cu_k && a->total_k != a->total_q) return HGEMM_ERR_INVALID_ARG;
   if (a->total_k > 0 && (!a->k || !a->v)) return HGEMM_ERR_INVALID_ARG;
-  if (a->out == a->q || a->out == a->k || a->out == a->v) return HGEMM_ERR_INVALID_ARG;
   if (!op_aligned16(a->q) || !op_aligned16(a->k) || !op_aligned16(a->v) || !op_aligned16(a->out))
     return HGEMM_ERR_INVALID_ARG;
   const long long qrow = static_cast<long long>(a->heads_q) * a->head_dim;
   const long long krow = static_cast<long long>(a->heads_kv) * a->head_dim;
   if (a->q_stride < qrow || a->out_stride < qrow || a->k_stride < krow || a->v_stride < krow)
     return HGEMM_ERR_INVALID_ARG;
-  if (a->q_stride % 8 || a->out_stride % 8 || a->k_stride % 8 || a->v_stride % 8)
-    return HGEMM_ERR_INVALID_ARG;
+  for (const long long stride : {a->q_stride, a->out_stride, a->k_stride, a->v_stride})
+    if (stride % 8 || stride > kOpMaxStride) return HGEMM_ERR_INVALID_ARG;
   const size_t need = hgemm_attn_prompt_workspace_bytes(a->total_q, a->total_k, a->batch, a->heads_q,
                                                         a->heads_kv, a->head_dim);
   if (need > 0 && (!a->workspace || !op_aligned16(a->workspace) || a->workspace_bytes < need))
     return HGEMM_ERR_INVALID_ARG;
-  return HGEMM_OK;
+  const OpRows in[] = {op_heads(a->q, a->heads_q, a->head_dim, a->q_stride, a->total_q),
+                       op_heads(a->k, a->heads_kv, a->head_dim, a->k_stride, a->total_k),
+                       op_heads(a->v, a->heads_kv, a->head_dim, a->v_stride, a->total_k),
+                       op_dense(a->cu_q, 4ll * a->batch + 4), op_dense(a->cu_k, 4ll * a->batch + 4)};
+  const OpRows out[] = {op_heads(a->out, a->heads_q, a->head_dim, a->out_stride, a->total_q),
+                        op_dense(a->lse, 4ll * a->total_q * a->heads_q),
+                        op_dense(a->workspace, static_cast<long long>(need))};
+  bool over = op_overlap(out[0], out[1]) || op_overlap(out[0], out[2]) || op_overlap(out[1], out[2]);
+  for (const OpRows &o : out)
+    for (const OpRows &i : in) over |= op_overlap(o, i);
+  return over ? HGEMM_ERR_INVALID_ARG : HGEMM_OK;
 }
 
 template <int DB, int TILES, bool FINE>

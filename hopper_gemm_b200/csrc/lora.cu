@@ -863,7 +863,6 @@ int check(const hgemm_lora_t *a) {
   if (a->tokens == 0 || a->N == 0) return HGEMM_OK;
   if (!a->X || !a->W || !a->Y || !op_aligned16(a->X) || !op_aligned16(a->W) || !op_aligned16(a->Y))
     return HGEMM_ERR_INVALID_ARG;
-  if (a->Y == a->X || a->Y == a->W) return HGEMM_ERR_INVALID_ARG;
   if (a->segments > 0 && (!a->seg_start || !a->seg_adapter)) return HGEMM_ERR_INVALID_ARG;
   if (a->adapters > 0 && a->segments > 0 &&
       (!a->down || !a->up || !a->scale || !op_aligned16(a->down) || !op_aligned16(a->up)))
@@ -872,7 +871,15 @@ int check(const hgemm_lora_t *a) {
                                                  a->segments);
   if (need > 0 && (!a->workspace || !op_aligned16(a->workspace) || a->workspace_bytes < need))
     return HGEMM_ERR_INVALID_ARG;
-  return HGEMM_OK;
+  const long long T = a->tokens, N = a->N, K = a->K, A = a->segments > 0 ? a->adapters : 0;
+  const OpRows in[] = {op_dense(a->X, 2 * T * K), op_dense(a->W, 2 * K * N), op_dense(a->down, 2 * A * K * a->rank),
+                       op_dense(a->up, 2 * A * a->rank * N), op_dense(a->scale, 4 * A),
+                       op_dense(a->seg_start, A > 0 ? 4ll * a->segments + 4 : 0),
+                       op_dense(a->seg_adapter, A > 0 ? 4ll * a->segments : 0)};
+  const OpRows Y = op_dense(a->Y, 2 * T * N), ws = op_dense(a->workspace, static_cast<long long>(need));
+  bool over = op_overlap(Y, ws);
+  for (const OpRows &x : in) over |= op_overlap(Y, x) || op_overlap(ws, x);
+  return over ? HGEMM_ERR_INVALID_ARG : HGEMM_OK;
 }
 
 int run_few(const hgemm_lora_t *a, const OpDevice &d, cudaStream_t stream) {

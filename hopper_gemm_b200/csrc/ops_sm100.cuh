@@ -52,8 +52,37 @@ int lora_gemm(const __half *A, const __half *B, __half *C, int M, int N, int K, 
 // grid's step or a tile behind the last one (a binary search adds two segment numbers).
 constexpr int kOpMaxRows = 0x7fffffff - 0xffff;
 constexpr int kOpMaxSegments = 1 << 30;
+constexpr long long kOpMaxStride = 1ll << 38;  // halves (a tensor map ends at 2^40 bytes)
 
 inline bool op_aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// An operand as rows of bytes; rows of one length next to each other may be one long row.
+struct OpRows {
+  const void *at;
+  long long width, stride, rows;
+};
+inline OpRows op_dense(const void *at, long long bytes) { return {at, bytes, bytes, 1}; }
+// Halves of `heads` heads for each token.
+inline OpRows op_heads(const void *at, long long heads, int head_dim, long long stride, long long tokens) {
+  return {at, 2 * heads * head_dim, 2 * stride, tokens};
+}
+// Whether two operands share a byte. (Rows of two different strides, both with gaps, are taken to
+// lie in each other's.)
+inline bool op_overlap(OpRows a, OpRows b) {
+  if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  for (OpRows *r : {&a, &b}) r->rows = r->rows < (1ll << 60) / r->stride ? r->rows : (1ll << 60) / r->stride + 1;
+  for (OpRows *r : {&a, &b})
+    if (r->rows == 1 || r->width == r->stride) *r = op_dense(r->at, r->width + (r->rows - 1) * r->stride);
+  if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) return false;
+  // Row i of a and row j of b meet where k = i - j has d - a.width < k * stride < d + b.width.
+  const long long stride = a.rows > 1 ? a.stride : b.stride;
+  const long long d = static_cast<long long>(reinterpret_cast<uintptr_t>(b.at)) -
+                      static_cast<long long>(reinterpret_cast<uintptr_t>(a.at));
+  const long long low = d - a.width;
+  long long k = low >= 0 ? low / stride + 1 : -((-low - 1) / stride);  // the first above low
+  k = k < 1 - b.rows ? 1 - b.rows : k;
+  return k <= a.rows - 1 && k * stride < d + b.width;
+}
 
 // Wait sites of the operators' kernels in the device status word (the GEMM uses 1..12).
 enum OpWaitSite : unsigned {

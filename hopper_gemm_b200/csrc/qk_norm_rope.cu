@@ -247,12 +247,25 @@ int check(const hgemm_qk_norm_rope_t *a) {
     if (heads == 0) return true;
     const long long row = static_cast<long long>(heads) * a->head_dim;
     return in && out && w && op_aligned16(in) && op_aligned16(out) && op_aligned16(w) &&
-           is % 8 == 0 && os % 8 == 0 && is >= row && os >= row && (in != out || is == os);
+           is % 8 == 0 && os % 8 == 0 && is >= row && os >= row && is <= kOpMaxStride && os <= kOpMaxStride && (in != out || is == os);
   };
   if (!operand(a->q, a->q_out, a->q_weight, a->q_stride, a->q_out_stride, a->heads_q) ||
       !operand(a->k, a->k_out, a->k_weight, a->k_stride, a->k_out_stride, a->heads_kv))
     return HGEMM_ERR_INVALID_ARG;
-  return HGEMM_OK;
+  const OpRows in[] = {op_heads(a->q, a->heads_q, a->head_dim, a->q_stride, a->tokens),
+                       op_heads(a->k, a->heads_kv, a->head_dim, a->k_stride, a->tokens),
+                       op_dense(a->q_weight, a->heads_q ? 2 * a->head_dim : 0),
+                       op_dense(a->k_weight, a->heads_kv ? 2 * a->head_dim : 0),
+                       op_dense(a->positions, a->rot_dim ? 4ll * a->axes * a->tokens : 0),
+                       op_dense(a->inv_freq, 2ll * a->rot_dim),
+                       op_dense(a->axis_of, a->axes > 1 ? a->rot_dim / 2 : 0)};
+  const OpRows out[] = {op_heads(a->q_out, a->heads_q, a->head_dim, a->q_out_stride, a->tokens),
+                        op_heads(a->k_out, a->heads_kv, a->head_dim, a->k_out_stride, a->tokens)};
+  bool over = op_overlap(out[0], out[1]);
+  for (int o = 0; o < 2; ++o)
+    for (int i = 0; i < 7; ++i)
+      over |= !(i == o && out[o].at == in[i].at) && op_overlap(out[o], in[i]);  // in place, or apart
+  return over ? HGEMM_ERR_INVALID_ARG : HGEMM_OK;
 }
 
 int run(const hgemm_qk_norm_rope_t *a, cudaStream_t stream) {

@@ -229,8 +229,9 @@ int hgemm_plan(int M, int N, int K, float beta, int aligned16, int force_bm, int
  * comes from the caller's `workspace` (16-byte aligned, at least the number of bytes that the
  * matching _workspace_bytes function returns; two calls that can overlap on the GPU need one
  * each). A NULL args pointer, a size or alignment outside the stated ranges, a NULL pointer to
- * an operand that is read or written, or a workspace that is too small returns
- * HGEMM_ERR_INVALID_ARG before any work; more than 2^31 - 65536 tokens, columns, queries, keys or
+ * an operand that is read or written, a workspace that is too small, or an output or workspace
+ * that shares memory with another operand (but for what is stated below; not looked for in rows of
+ * two different strides that both have gaps) returns HGEMM_ERR_INVALID_ARG before any work; more than 2^31 - 65536 tokens, columns, queries, keys or
  * sequences, or 2^30 segments, HGEMM_ERR_TOO_LARGE. No counterpart in the reference. */
 
 /* Shared projection with low-rank adapters:

@@ -6,6 +6,7 @@ import subprocess
 import sys
 
 import pytest
+import torch
 
 import hopper_gemm_b200 as hg
 from hopper_gemm_b200 import lib
@@ -142,3 +143,88 @@ def test_star_import_brings_the_operators():
     names = {}
     exec("from hopper_gemm_b200 import *", names)
     assert callable(names["lora"]) and callable(names["qk_norm_rope"]) and callable(names["attn_prompt"])
+
+
+def order(st):
+    """Nothing is refused: the call gets as far as the device, of which there is none."""
+    return status(st) != BAD
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="an accepted call would run on made-up addresses")
+@pytest.mark.parametrize("st", [lora_args(), norm_args(), attn_args(), attn_args(cu_k=None), norm_args(axes=3),
+                                lora_args(adapters=0, down=None, up=None, scale=None), attn_args(lse=None)])
+def test_arguments_in_order_are_not_refused(st):
+    assert order(st)
+
+
+@pytest.mark.parametrize("out", ["Y", "workspace"])
+@pytest.mark.parametrize("name,last", [("X", 16 * 64 * 2), ("W", 64 * 64 * 2), ("down", 4 * 64 * 16 * 2),
+                                       ("up", 4 * 64 * 16 * 2), ("scale", 16), ("seg_start", 12), ("seg_adapter", 8)])
+def test_lora_outputs_over_inputs(out, name, last):
+    """At an input's first byte, and at the 16 bytes that hold its last one."""
+    at = getattr(lora_args(), name)
+    for where in (at, at + (last - 1) // 16 * 16):
+        assert status(lora_args(**{out: where})) == BAD
+
+
+def test_lora_output_over_the_workspace():
+    need = lib.hgemm_lora_workspace_bytes(16, 64, 64, 16, 4, 2)
+    ws = lora_args().workspace
+    for where in (ws, ws + (need - 1) // 16 * 16, ws - 16 * 64 * 2 + 16):
+        assert status(lora_args(Y=where)) == BAD
+
+
+@pytest.mark.parametrize("out,ins", [("q_out", "k"), ("k_out", "q"), ("q_out", "k_out"), ("q_out", "q_weight"),
+                                     ("k_out", "k_weight"), ("k_out", "positions"), ("q_out", "inv_freq")])
+def test_norm_outputs_over_other_operands(out, ins):
+    assert status(norm_args(**{out: getattr(norm_args(), ins)})) == BAD
+
+
+@pytest.mark.parametrize("over", [
+    dict(q_out=16), dict(q_out=-16), dict(q_out=1024 * 2 * 15), dict(q_out=2048 - 16)])
+def test_norm_output_over_a_part_of_its_input(over):
+    """Shifted against the input, by less than a row or by whole rows."""
+    base = norm_args().q
+    assert status(norm_args(q_out=base + over["q_out"])) == BAD
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "cu_q", "cu_k"])
+@pytest.mark.parametrize("out", ["out", "lse"])
+def test_attn_outputs_over_inputs(out, name):
+    st = attn_args()
+    assert status(attn_args(**{out: getattr(st, name)})) == BAD
+
+
+def test_attn_outputs_over_each_other_and_the_workspace():
+    st = attn_args(total_q=2, total_k=20000)
+    assert lib.hgemm_attn_prompt_workspace_bytes(2, 20000, 2, 8, 2, 128) > 0
+    for a, b in (("out", "lse"), ("out", "workspace"), ("lse", "workspace"), ("workspace", "q"), ("workspace", "v")):
+        assert status(attn_args(total_q=2, total_k=20000, **{a: getattr(st, b)})) == BAD
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="an accepted call would run on made-up addresses")
+def test_other_columns_of_the_same_rows_are_no_overlap():
+    """Queries, keys, values and outputs as columns of one buffer, rows of 8 + 2 + 2 + 8 heads; the norm in place and
+    into the columns behind."""
+    wide, at = 20 * 128, 1 << 50
+    cols = dict(q=at, k=at + 2 * 8 * 128, v=at + 2 * 10 * 128, out=at + 2 * 12 * 128, q_stride=wide, k_stride=wide,
+                v_stride=wide, out_stride=wide)
+    assert order(attn_args(**cols))
+    for shift in (-16, 16):
+        assert not order(attn_args(**{**cols, "out": cols["out"] + shift}))
+    norm = dict(q=at, k=at + 2 * 8 * 128, q_out=at, k_out=at + 2 * 8 * 128, q_stride=wide, k_stride=wide,
+                q_out_stride=wide, k_out_stride=wide)
+    assert order(norm_args(**norm))
+    assert order(norm_args(**{**norm, "q_out": at + 2 * 10 * 128}))
+    assert not order(norm_args(**{**norm, "q_out": at + 2 * 9 * 128}))
+    assert not order(norm_args(**{**norm, "k_out": at + 2 * 7 * 128}))
+    # one token: its row ends where the row does
+    assert order(norm_args(tokens=1, q=at, q_out=at + 2 * 1024)) and not order(norm_args(tokens=1, q=at, q_out=at + 16))
+
+
+@pytest.mark.parametrize("st", [norm_args(q_stride=1 << 39), norm_args(k_out_stride=1 << 62), attn_args(v_stride=1 << 40),
+                                attn_args(out_stride=1 << 60), attn_args(total_q=LIMIT, total_k=LIMIT, cu_k=None,
+                                                                         q_stride=1 << 38, out_stride=1 << 38)])
+def test_strides_beyond_any_memory_are_refused(st):
+    """The last: rows of 2^31 times 2^39 bytes reach over every other operand."""
+    assert status(st) == BAD
