@@ -883,7 +883,7 @@ template <int DB, int TILES, bool FINE>
 int launch(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const AttnParams &p,
            const OpDevice &d, long long ctas, cudaStream_t stream) {
   using Cfg = AttnCfg<DB, TILES>;
-  static bool done[64];
+  static unsigned done[64];
   const int st = op_smem(reinterpret_cast<const void *>(attn_kernel<DB, TILES, FINE>), Cfg::SMEM, d.dev, done);
   if (st != HGEMM_OK) return st;
   attn_kernel<DB, TILES, FINE>

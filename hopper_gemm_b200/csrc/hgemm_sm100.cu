@@ -1821,6 +1821,7 @@ struct DevState {
 };
 std::mutex g_mu;
 DevState g_dev[64];
+unsigned g_contexts = 1;  // counts hgemm_release(), behind which kernels' attributes may be gone
 
 int current_device(int *dev) {
   if (cudaGetDevice(dev) != cudaSuccess || *dev < 0 || *dev >= 64) return HGEMM_ERR_CUDA;
@@ -2516,15 +2517,15 @@ int lora_gemm(const __half *A, const __half *B, __half *C, int M, int N, int K, 
   return HGEMM_OK;
 }
 
-int op_smem(const void *kernel, int smem, int dev, bool *done) {
+int op_smem(const void *kernel, int smem, int dev, unsigned *done) {
   std::lock_guard<std::mutex> lock(g_mu);
-  if (done[dev]) return HGEMM_OK;
+  if (done[dev] == g_contexts) return HGEMM_OK;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
       cudaSuccess) {
     cudaGetLastError();
     return HGEMM_ERR_CUDA;
   }
-  done[dev] = true;
+  done[dev] = g_contexts;
   return HGEMM_OK;
 }
 
@@ -2872,8 +2873,13 @@ void hgemm_release(void) {
       g_dev[i].scratch_bytes = 0;
     }
     g_dev[i].status_word = nullptr;
+    for (auto &tile : g_dev[i].attr_done)
+      for (bool &done : tile) done = false;
+    for (bool &done : g_dev[i].ext_attr_done) done = false;
   }
+  ++g_contexts;
   cudaSetDevice(cur);
+  cudaGetLastError();  // a reset device's scratch is gone already
   g_tune.clear();
   noalloc_forget_addresses();
 }

@@ -927,7 +927,7 @@ int run_few(const hgemm_lora_t *a, const OpDevice &d, cudaStream_t stream) {
   if (!(p.whole_blocks ? op_encode(&tw, a->W, 3, wd3, ws3, wb3) : op_encode(&tw, a->W, 2, wd, ws, wb)) ||
       !op_encode(&tx, a->X, 2, xd, xs, xb))
     return HGEMM_ERR_TENSOR_MAP;
-  static bool done[64];
+  static unsigned done[64];
   const int st = op_smem(reinterpret_cast<const void *>(lora_few_kernel), kFewSmem, d.dev, done);
   if (st != HGEMM_OK) return st;
   lora_low_kernel<<<p.tokens * p.slices, kLowThreads, 0, stream>>>(p);
@@ -1020,7 +1020,7 @@ int run(const hgemm_lora_t *a, cudaStream_t stream) {
   const unsigned db[3] = {64, 64, 1};
   if (!op_encode(&tx, a->X, 2, xd, xs, xb) || !op_encode(&td, a->down, 3, dd, ds, db))
     return HGEMM_ERR_TENSOR_MAP;
-  static bool done[64];
+  static unsigned done[64];
   st = op_smem(reinterpret_cast<const void *>(lora_shrink_kernel), kSmem, d.dev, done);
   if (st != HGEMM_OK) return st;
   cudaLaunchConfig_t cfg = {};

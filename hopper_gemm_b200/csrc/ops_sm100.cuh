@@ -26,9 +26,9 @@ int op_status(int status);
 // innermost first, byte strides of dimensions 1.. .
 bool op_encode(CUtensorMap *map, const void *ptr, int rank, const unsigned long long *dims,
                const unsigned long long *strides, const unsigned *box);
-// Opts `kernel` in to `smem` bytes of dynamic shared memory on device `dev`, once per process
-// and device (`done` is the caller's per-kernel array of 64 flags).
-int op_smem(const void *kernel, int smem, int dev, bool *done);
+// Opts `kernel` in to `smem` bytes of dynamic shared memory on device `dev`, once until hgemm_release()
+// (`done` is the caller's per-kernel array of 64 zeros).
+int op_smem(const void *kernel, int smem, int dev, unsigned *done);
 
 // The GEMM with additional k-blocks (the second product of low-rank adapters): row tile i of C gets,
 // after the k-blocks of A and B, count[i] entries e = base[i].. of `chunks` k-blocks each, whose A

@@ -1,6 +1,9 @@
 """GPU: the attention layer's operators at the values, masks and sizes where a rounding, a mask or a
 repair shows. References and tolerances are plain 64-bit forms derived beside each test."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -243,3 +246,49 @@ def test_lora_wide_and_long_projections(cuda, T, K, N, r):
         want, tol = ref.lora(X, W, down, up, scale, ref.token_adapters(T, cut, ids, A))
         ref.close(got, want, tol, f"lora {T}x{K}x{N}")
     assert cuda.device_status(clear=True) == (0, 0)
+
+
+# ------------------------------------------------------------------------------- after a device reset
+RESET = """
+import ctypes, glob, os, sys
+import hopper_gemm_b200 as hg
+from hopper_gemm_b200._native import HgemmAttnPrompt, HgemmLora, HgemmQkNormRope
+cudart = ctypes.CDLL("libcudart.so.12")
+
+def once():
+    def mem(n):
+        p = ctypes.c_void_p()
+        assert cudart.cudaMalloc(ctypes.byref(p), ctypes.c_size_t(n)) == 0
+        assert cudart.cudaMemset(p, 0, ctypes.c_size_t(n)) == 0
+        return p.value
+    a = HgemmLora()
+    for n in ("X", "W", "Y", "down", "up", "scale", "seg_start", "seg_adapter", "workspace"):
+        setattr(a, n, mem(1 << 22))
+    a.workspace_bytes, a.N, a.K, a.rank, a.adapters, a.segments = 1 << 22, 512, 512, 16, 2, 2
+    out = []
+    for a.tokens in (3, 700):
+        out.append(hg.lib.hgemm_lora(ctypes.byref(a), None))
+    b = HgemmAttnPrompt()
+    for n in ("q", "k", "v", "out", "cu_q", "workspace"):
+        setattr(b, n, mem(1 << 22))
+    b.q_stride = b.k_stride = b.v_stride = b.out_stride = 512
+    b.workspace_bytes, b.total_q, b.total_k, b.batch = 1 << 22, 300, 300, 2
+    b.heads_q, b.heads_kv, b.head_dim, b.causal, b.scale = 4, 4, 128, 1, 0.1
+    out.append(hg.lib.hgemm_attn_prompt(ctypes.byref(b), None))
+    out.append(hg.lib.hgemm_launch(a.X, a.W, a.Y, 512, 512, 512, 1.0, 0.0, None))
+    return out + [cudart.cudaDeviceSynchronize()] + list(hg.device_status(clear=True))
+
+assert once() == [0] * 7
+assert cudart.cudaDeviceReset() == 0
+hg.release()
+got = once()
+assert got == [0] * 7, got
+"""
+
+
+def test_calls_after_a_device_reset(cuda):
+    """hgemm_release() forgets what a reset of the device took: the calls of a new context set it up again."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, LD_LIBRARY_PATH="/usr/local/cuda/lib64:" + os.environ.get("LD_LIBRARY_PATH", ""))
+    run = subprocess.run([sys.executable, "-c", RESET], cwd=root, env=env, timeout=120, capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr[-2000:]
