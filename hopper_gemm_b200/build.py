@@ -67,19 +67,39 @@ def _run(cmd, verbose):
     subprocess.run(cmd, check=True)
 
 
-def _build_binding(nvcc, verbose):
-    """_operators.so: host code against torch's headers, found without importing torch."""
+def _torch():
+    """(directory, version) of the installed torch, found without importing it; (None, None) without one."""
     import importlib.util
-    import sysconfig
+    import re
     spec = importlib.util.find_spec("torch")
     if not spec or not spec.submodule_search_locations:
-        print("note: torch not found; _operators.so (the operators' Python binding) skipped", flush=True)
-        return
+        return None, None
     torch = list(spec.submodule_search_locations)[0]
+    with open(os.path.join(torch, "version.py")) as f:
+        return torch, re.search(r"__version__ = ['\"]([^'\"]+)['\"]", f.read()).group(1)
+
+
+def _built_for(version):
+    """What the binding holds of the torch that it was built against."""
+    return f"hopper_gemm_b200 operators for torch {version}"
+
+
+def _binding_stale(version):
+    """Whether _operators.so is absent, older than its sources or built against another torch."""
+    if _stale(BINDING, [os.path.join(CSRC, "operators_py.cpp"), os.path.join(INCLUDE, "hgemm_b200.h")]):
+        return True
+    with open(BINDING, "rb") as f:
+        return _built_for(version).encode() + b"\0" not in f.read()
+
+
+def _build_binding(nvcc, torch, version, verbose):
+    """_operators.so: host code against torch's headers."""
+    import sysconfig
     include = [INCLUDE, sysconfig.get_paths()["include"], os.path.join(torch, "include"),
                os.path.join(torch, "include", "torch", "csrc", "api", "include"),
                os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")]
-    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"] +
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+          f'-DOPERATORS_BUILT_FOR="{_built_for(version)}"'] +
          ["-I" + d for d in include] + ["-o", BINDING, os.path.join(CSRC, "operators_py.cpp"),
          "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
          "-ltorch_python"],
@@ -97,9 +117,11 @@ def build(force=False, verbose=True, extra_flags=()):
                    os.path.join(CSRC, "ops_sm100.cuh"), os.path.join(INCLUDE, "hgemm_b200.h")]
     if force or _stale(LIB, deps):
         _run([nvcc] + common + ["-shared", "-o", LIB] + srcs + ["-ldl"], verbose)
-    if force or _stale(BINDING, [os.path.join(CSRC, "operators_py.cpp"),
-                                 os.path.join(INCLUDE, "hgemm_b200.h")]):
-        _build_binding(nvcc, verbose)
+    torch, version = _torch()
+    if torch is None:
+        print("note: torch not found; _operators.so (the operators' Python binding) skipped", flush=True)
+    elif force or _binding_stale(version):
+        _build_binding(nvcc, torch, version, verbose)
     csrc = [os.path.join(CSRC, "cublas_ref.cu")]
     if force or _stale(CUBLAS_LIB, csrc):
         _run([nvcc] + common + ["-shared", "-o", CUBLAS_LIB] + csrc + ["-lcublas"], verbose)

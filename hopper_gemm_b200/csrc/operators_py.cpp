@@ -329,4 +329,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__operators() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__operators() {
+  PyObject *m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", OPERATORS_BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -14,7 +14,7 @@ no gradients are formed.
 """
 import ctypes
 
-import torch  # noqa: F401  (the library's tensors and allocator, which _operators is linked to)
+import torch  # (the library's tensors and allocator, which _operators is linked to)
 
 from . import HgemmError
 from ._native import lib
@@ -24,6 +24,9 @@ try:
 except ImportError as e:
     raise ImportError(f"hopper_gemm_b200/_operators.so: {e}; build it with "
                       "`python hopper_gemm_b200/build.py`") from e
+if _operators.built_for.split()[-1] != torch.__version__:  # the layout of its tensors is that torch's
+    raise ImportError(f"hopper_gemm_b200/_operators.so is built for torch {_operators.built_for.split()[-1]}, this is "
+                      f"{torch.__version__}; build it with `python hopper_gemm_b200/build.py`")
 
 _operators.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
     "hgemm_lora", "hgemm_lora_workspace_bytes", "hgemm_qk_norm_rope", "hgemm_attn_prompt",

@@ -228,3 +228,16 @@ def test_other_columns_of_the_same_rows_are_no_overlap():
 def test_strides_beyond_any_memory_are_refused(st):
     """The last: rows of 2^31 times 2^39 bytes reach over every other operand."""
     assert status(st) == BAD
+
+
+def test_the_binding_is_built_for_the_installed_torch(tmp_path, monkeypatch):
+    """Another torch, an older binding, or none: it is built again."""
+    from hopper_gemm_b200 import _operators, build
+    where, version = build._torch()
+    assert version == torch.__version__ and os.path.samefile(where, os.path.dirname(torch.__file__))
+    assert _operators.built_for == build._built_for(version)
+    assert not build._binding_stale(version)
+    for other in ("1.0.0", version + "1", version[:-1]):
+        assert build._binding_stale(other)
+    monkeypatch.setattr(build, "BINDING", str(tmp_path / "_operators.so"))
+    assert build._binding_stale(version)
