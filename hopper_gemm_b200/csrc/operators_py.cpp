@@ -146,6 +146,13 @@ void call(const char *name, Entry entry, const Args &args, hgemm_stream_t stream
   throw Refused();
 }
 
+// A tensor of the caller's that was written: what autograd has saved of it is no longer that, and it says so.
+void written(PyObject *o) {
+  if (o == Py_None) return;
+  const at::Tensor &t = THPVariable_Unpack(o);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 template <class F>
 PyObject *guarded(Py_ssize_t got, Py_ssize_t want, F &&f) {
   HANDLE_TH_ERRORS
@@ -196,6 +203,7 @@ PyObject *lora(PyObject *, PyObject *const *p, Py_ssize_t n) {
     }
     scratch(a, g_lora_bytes(a.tokens, a.N, a.K, a.rank, a.adapters, a.segments), p[8], dev, keep);
     call("hgemm_lora", g_lora, a, launch.stream);
+    written(p[7]);
     return p[7] == Py_None ? THPVariable_Wrap(Y) : Py_NewRef(p[7]);
   });
 }
@@ -249,6 +257,8 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *p, Py_ssize_t n) {
       a.k_out_stride = hk * d;
     }
     call("hgemm_qk_norm_rope", g_norm, a, launch.stream);
+    written(p[9]);
+    written(p[10]);
     PyObject *y0 = p[9] == Py_None ? THPVariable_Wrap(q_out) : Py_NewRef(p[9]);
     PyObject *y1 = p[10] == Py_None ? THPVariable_Wrap(k_out) : Py_NewRef(p[10]);
     PyObject *both = y0 && y1 ? PyTuple_Pack(2, y0, y1) : nullptr;
@@ -299,6 +309,8 @@ PyObject *attn_prompt(PyObject *, PyObject *const *p, Py_ssize_t n) {
     }
     scratch(a, g_attn_bytes(a.total_q, a.total_k, a.batch, a.heads_q, a.heads_kv, a.head_dim), p[9], dev, keep);
     call("hgemm_attn_prompt", g_attn, a, launch.stream);
+    written(p[7]);
+    written(p[8]);
     return p[7] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(p[7]);
   });
 }

@@ -292,3 +292,49 @@ def test_calls_after_a_device_reset(cuda):
     env = dict(os.environ, LD_LIBRARY_PATH="/usr/local/cuda/lib64:" + os.environ.get("LD_LIBRARY_PATH", ""))
     run = subprocess.run([sys.executable, "-c", RESET], cwd=root, env=env, timeout=120, capture_output=True, text=True)
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+# ------------------------------------------------------------------------------- outputs that autograd has saved
+def test_outputs_of_the_caller_are_known_as_written(cuda):
+    """A tensor that another operation keeps for its gradient, written by an operator: backward says so instead of going on
+    with other values. Inference tensors have no such count."""
+    w = rand(1, (64,))
+    pos, inv = i32(list(range(6))), torch.ones(32, device=DEV)
+    x = rand(2, (6, 4, 64)).requires_grad_()
+
+    def kept():
+        y = x * 2
+        return y, (y * y).sum()
+
+    y, z = kept()
+    cuda.qk_norm_rope(y[:, :3], y[:, 3:], w, w, pos, inv, q_out=y[:, :3])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    y, z = kept()
+    cuda.qk_norm_rope(y[:, :3], y[:, 3:], w, w, pos, inv, k_out=y[:, 3:])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    y, z = kept()
+    q = rand(3, (6, 4, 64))
+    cuda.attn_prompt(q, q, q, i32([0, 6]), out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    lse = torch.ones((6, 4), device=DEV, requires_grad=True) * 2
+    z = (lse * lse).sum()
+    cuda.attn_prompt(q, q, q, i32([0, 6]), lse=lse)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    y, z = kept()
+    down, up = rand(4, (1, 64, 8)), rand(5, (1, 8, 64))
+    cuda.lora(rand(6, (24, 64)), rand(7, (64, 64)), down, up, torch.ones(1, device=DEV), i32([0, 24]), i32([0]),
+              Y=y.view(24, 64))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    y, z = kept()
+    cuda.attn_prompt(q, q, q, i32([0, 6]))
+    z.backward()
+    with torch.inference_mode():
+        out = torch.empty_like(q)
+        cuda.attn_prompt(q, q, q, i32([0, 6]), out=out)
+    assert torch.equal(out, cuda.attn_prompt(q, q, q, i32([0, 6])))
+    cuda.attn_prompt(q, q, q, i32([0, 6]), out=out)
