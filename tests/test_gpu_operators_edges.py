@@ -338,3 +338,47 @@ def test_outputs_of_the_caller_are_known_as_written(cuda):
         cuda.attn_prompt(q, q, q, i32([0, 6]), out=out)
     assert torch.equal(out, cuda.attn_prompt(q, q, q, i32([0, 6])))
     cuda.attn_prompt(q, q, q, i32([0, 6]), out=out)
+
+
+# ------------------------------------------------------------------------------- a cache with room to grow
+@pytest.mark.parametrize("behind", [0.0, 7.0, math.nan])
+def test_attn_cache_of_slots_with_room(cuda, behind):
+    """Single tokens over slots that are not full: a sequence without queries stands for the rest of each. A captured step
+    follows the starts as the sequences grow."""
+    slots, size, hq, hkv, d = 5, 700, 8, 2, 128
+    fill = [1, 64, 130, 699, 317]
+    k, v, q = rand(1, (slots * size, hkv, d)), rand(2, (slots * size, hkv, d)), rand(3, (slots, hq, d))
+    store = [k.clone(), v.clone()]
+
+    def cu_k():
+        return [0] + [x for s in range(slots) for x in (s * size + fill[s], (s + 1) * size)]
+
+    def blank():
+        for t, full in zip((k, v), store):
+            for s in range(slots):
+                t[s * size:(s + 1) * size] = full[s * size:(s + 1) * size]
+                t[s * size + fill[s]:(s + 1) * size] = behind
+
+    cq, ck = i32([0] + [x for s in range(slots) for x in (s + 1, s + 1)]), i32(cu_k())
+    out = torch.empty_like(q)
+
+    def check():
+        for s in range(slots):
+            rows = slice(s * size, s * size + fill[s])
+            want, tol, _, _ = ref.attn(q[s:s + 1], k[rows], v[rows], [1], [fill[s]], d ** -0.5, True)
+            ref.close(out[s:s + 1], want, tol, f"slot {s} of {fill[s]}")
+
+    blank()
+    cuda.attn_prompt(q, k, v, cq, ck, out=out)
+    check()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        cuda.attn_prompt(q, k, v, cq, ck, out=out)
+    for _ in range(2):
+        fill = [min(size, n + 1) for n in fill]
+        blank()
+        ck.copy_(i32(cu_k()))
+        graph.replay()
+        check()
+    assert cuda.device_status(clear=True) == (0, 0)
