@@ -17,9 +17,10 @@
 // row's limit are masked; the tiles with most keys start first.
 //
 // Long prompts: bound by the exponentials (64 a row and block, 4 lanes a cycle) beside the products; 16384 tokens
-// of 32 heads over 8, head_dim 128, causal: 1.89 to 2.1 ms, 1050 to 1160 TFLOP/s (the GPU's power moves it). 4096 x 1: 985
-// TFLOP/s. Prompts of some 700 tokens (12 of 8192 in all) 122 us, where starts and ends of 2100 short CTAs count.
-// Single tokens: bound by HBM; 16 over 131072 keys of 8 heads 99 us with the join, 5.4 TB/s.
+// of 32 heads over 8, head_dim 128, causal: 2.12 ms, 1040 TFLOP/s (1.88 ms in a replayed graph; the GPU's power
+// moves both). Prompts of some 700 tokens (12 of 8192 in all) 137 us, where starts and ends of 2100 short CTAs
+// count. Single tokens: bound by HBM; 16 over 131072 keys of 8 heads 112 us with the join, 4.8 TB/s. (Eager calls
+// over changing inputs; the figures at the choices below compare variants in replayed graphs over one input.)
 //
 // No counterpart in the reference.
 
@@ -800,10 +801,10 @@ AttnPlan make_plan(int total_q, int total_k, int batch, int heads_q, int heads_k
   // tokens 174 and 166 us, 8192 tokens 475 and 495, 16384 tokens 1.89 and 2.06 ms), in favour of
   // one tile at head_dim 64 up to 8192.
   pl.tiles = head_dim > 64 && avg_k >= 6144 && avg_q > pl.tile_q ? 2 : 1;
-  // Weights rounded to binary16 leave as much error in an output as its own rounding does: together 1.4
-  // times the latter over many outputs, over a token's few by chance 1.5 and more (6 rows of 96, seen). There
-  // they keep 22 bits, which costs 5% (one token over 131072 keys 124 us against 118, before its key ranges
-  // were made longer); 16 tokens of 32 heads would take 106 us instead of 99, a dozen prompts 141 for 122.
+  // Weights rounded to binary16 leave as much error in an output as its own rounding does, together 1.4 times the
+  // latter; with 22 bits the output's own is left. A choice between that and time: small calls, whose few outputs do
+  // not average their errors either (1.53 times, 6 rows of 96 seen), take it at 5% (one token over 131072
+  // keys 124 us against 118); larger ones do not (16 tokens of 32 heads 106 us instead of 99, a dozen prompts 141 for 122).
   pl.fine = static_cast<long long>(total_q) * heads_q <= 128;
   const int span = pl.tiles * pl.tile_q;
   const long long max_tiles = std::min<long long>(total_q, total_q / span + static_cast<long long>(batch));

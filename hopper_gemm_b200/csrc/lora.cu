@@ -7,19 +7,20 @@
 // which the rows of other adapters are zero. The projection's own GEMM kernel (hgemm_sm100.cu) then
 // walks those blocks as additional k-blocks behind the k-blocks of X and W, so that Up's product
 // lands in the same fp32 accumulators and Y is written and rounded once; an adapter costs its row
-// tiles rank / K of the GEMM. H is rounded to binary16 because it is a tcgen05 operand next to Up.
+// tiles rank / K of the GEMM. H is rounded to binary16 because it is a tcgen05 operand next to Up (the path of few
+// tokens keeps it in fp32).
 //
-// Few tokens (decoding, short batches; few_plan says when): bound by the bytes of W and of the adapters in use. W is the M operand of the
-// product, 128 of its columns to a CTA, and the tokens are its N; K is split over a cluster, so that
-// every SM pulls weights, and joined through distributed shared memory. The adapters run on the CUDA
+// Few tokens (decoding, short batches; few_plan says when): bound by the bytes of W and of the adapters in
+// use. W is the M operand of the product, 128 of its columns to a CTA, and the tokens are its N; K is split
+// over a cluster, so that every SM pulls weights, and joined through distributed shared memory. The adapters run on the CUDA
 // cores in fp32, H in a launch of its own under whose feet the main kernel already starts, and Up's part
 // in warps that would otherwise wait for the main loop.
 //
-// Measured (one B200): 1 token x 4096 x 4096, rank 16: 9.4 us, of which W's 33.6 MB are 5.2; 48 tokens of as many
-// adapters x 4096 x 6144, rank 32: 20.0 us (H 7.5, under which W streams; then every token's rows of
-// Up from L2). 1037 tokens x 4096 x 4096 of many adapters: 51 us, the GEMM alone 33.9 and H 20, part of it
-// hidden: both take whole SMs' shared memory. 8192 tokens x 4096 x 6144: 309 to 350 us, the GEMM alone 291 to
-// 333, H 29: bound by the products and the power limit.
+// Measured (one B200, eager calls over changing inputs): 1 token x 4096 x 4096, rank 16: 12.3 us, of which W's 33.6 MB
+// are 5.2; 48 tokens of as many requests x 4096 x 6144, rank 32: 24.6 us (H 7.5, under which W streams; then every
+// token's rows of Up from L2). 1037 tokens x 4096 x 4096 of many adapters: 58 us, the GEMM alone 33.9 and H 20,
+// part of it hidden: both take whole SMs' shared memory. 8192 tokens x 4096 x 6144: 381 us (323 in a replayed
+// graph), the GEMM alone 291 to 333, H 29: bound by the products and the power limit.
 //
 // No counterpart in the reference.
 

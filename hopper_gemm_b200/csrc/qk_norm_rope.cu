@@ -2,7 +2,7 @@
 //
 //   n = x * rsqrt(mean(x^2) + eps) * w;   (n1, n2) -> (n1 cos a - n2 sin a, n2 cos a + n1 sin a)
 //
-// Bound: HBM. Every half is read once and written once (4 bytes of traffic an element), against
+// Bound: loads in flight to HBM (ncu: DRAM and issue at 45% each). Every half is read once and written once (4 bytes of traffic an element), against
 // about ten fp32 operations, so what matters is loads in flight and few instructions beside them.
 // Norm weight and rotation are one: element e becomes r (x_e A_e + x_partner B_e), with A and B (weight
 // times cos, weight times sin) formed once for a token and side, and two elements go into an
@@ -11,12 +11,12 @@
 // next to them when pairs are adjacent), so that the rotation needs no other lane, the mean square is
 // the only exchange, and A and B stay in registers over all heads of a side. The heads of the next two
 // passes are on their way while one is worked on.
-// The angles: one lane for each pair forms position * inv_freq in fp64 (exact: 31 + 24 bits), reduces it
-// to a turn there and takes sincospi in fp32, while the token's first heads are loaded.
+// The angles: one lane for each pair forms position * inv_freq / pi in fp64 (three roundings: at a position of 2^31 off by
+// 2^-22 of half a turn), reduces it to a turn there and takes sincospi in fp32, while the token's first heads are loaded.
 // Forms in which a CTA's warps shared a token (through registers, or a ring of bulk copies) took 37 us
 // for 8191 tokens of 40 heads of 128: A and B came from shared memory for every head, whose bandwidth
 // was then the bound. Measured: 36 us, 4.6 TB/s (a contiguous copy of the same bytes takes 30 to 31); 2500 tokens
-// of 32 heads of 80, where one wave of warps has a token each and latency counts, 12.3 us; 48 tokens 4.3.
+// of 32 heads of 80, where one wave of warps has a token each and latency counts, 12.3 us; a call of 48 tokens 5.4.
 //
 // No counterpart in the reference.
 

@@ -238,11 +238,13 @@ int hgemm_plan(int M, int N, int K, float beta, int aligned16, int force_bm, int
  *   Y[t,:] = X[t,:] W + scale[a] * (X[t,:] Down[a]) Up[a],   a = seg_adapter[s], t in segment s
  * Segment s holds the tokens seg_start[s] <= t < seg_start[s+1]; a token of no segment, or of
  * one whose adapter is outside [0, adapters), gets X W alone. X W is summed in fp32 and the
- * adapter's part is added before the one rounding to binary16; X Down is rounded to binary16
- * (after the scale), as an operand of the second product, so |scale * X Down| must stay below
- * 65504. An infinity or NaN stays with the tokens that it belongs to. In an adapter's Up it makes
+ * adapter's part is added before the one rounding to binary16. scale * X Down is rounded to
+ * binary16, as an operand of the second product, or, in the path that small calls take, kept in
+ * fp32: a token's result may differ by that rounding (2^-11 of each element) between calls of
+ * other sizes, and |scale * X Down| must stay below 65504, which the small ones do not enforce. An
+ * infinity or NaN stays with the tokens that it belongs to. In an adapter's Up it makes
  * the call slower: other tokens next to that adapter's are formed again in these columns (1200
- * tokens of 4096 x 4096 beside an adapter of nothing else: 0.71 ms instead of 0.07).
+ * tokens of 4096 x 4096 beside an adapter of nothing else: 0.69 ms instead of 0.07).
  * K, N and rank are multiples of 8, 8 <= rank <= 256; matrices are row-major, contiguous
  * and start on 16-byte boundaries. Y must not overlap the inputs. */
 typedef struct {
@@ -267,7 +269,7 @@ size_t hgemm_lora_workspace_bytes(int tokens, int N, int K, int rank, int adapte
  *   pair (n1, n2) i of the first rot_dim elements turns by positions[axis_of[i]][t]*inv_freq[i]:
  *     (n1 cos - n2 sin, n2 cos + n1 sin); elements from rot_dim on are the norm alone.
  * Pairs are (i, i + rot_dim/2), or (2i, 2i+1) when interleaved != 0. Angles are formed and
- * reduced in fp64, so any int32 position is exact to fp32. axes > 1 gives every pair the position of one
+ * reduced in fp64: with inv_freq up to 1 any int32 position is off by less than 2^-21 of half a turn. axes > 1 gives every pair the position of one
  * axis (time, height, width); axis_of may be NULL when axes == 1, and values above axes - 1
  * count as axes - 1. head_dim is a multiple of 8 up to 256, rot_dim a multiple of 16 up to
  * head_dim (0: the norm alone), at most 2^20 heads on a side (HGEMM_ERR_TOO_LARGE). Strides are halves between tokens, multiples of 8 and at least
