@@ -2,8 +2,9 @@
 //
 //   n = x * rsqrt(mean(x^2) + eps) * w;   (n1, n2) -> (n1 cos a - n2 sin a, n2 cos a + n1 sin a)
 //
-// Bound: loads in flight to HBM (ncu: DRAM and issue at 45% each). Every half is read once and written once (4 bytes of traffic an element), against
-// about ten fp32 operations, so what matters is loads in flight and few instructions beside them.
+// Bound: loads in flight to HBM (ncu: DRAM and issue at 45% each). Every half is read once and written once (4
+// bytes of traffic an element), against about ten fp32 operations, so what matters is loads in flight and few
+// instructions beside them.
 // Norm weight and rotation are one: element e becomes r (x_e A_e + x_partner B_e), with A and B (weight
 // times cos, weight times sin) formed once for a token and side, and two elements go into an
 // instruction (fma.rn.f32x2). A warp takes a token: its lane groups of a few lanes hold a head each, 16
