@@ -870,10 +870,10 @@ int check(const hgemm_attn_prompt_t *a) {
   const OpRows in[] = {op_heads(a->q, a->heads_q, a->head_dim, a->q_stride, a->total_q),
                        op_heads(a->k, a->heads_kv, a->head_dim, a->k_stride, a->total_k),
                        op_heads(a->v, a->heads_kv, a->head_dim, a->v_stride, a->total_k),
-                       op_dense(a->cu_q, 4ll * a->batch + 4), op_dense(a->cu_k, 4ll * a->batch + 4)};
+                       op_dense(a->cu_q, 4, a->batch + 1), op_dense(a->cu_k, 4, a->batch + 1)};
   const OpRows out[] = {op_heads(a->out, a->heads_q, a->head_dim, a->out_stride, a->total_q),
-                        op_dense(a->lse, 4ll * a->total_q * a->heads_q),
-                        op_dense(a->workspace, static_cast<long long>(need))};
+                        op_dense(a->lse, 4, a->total_q, a->heads_q),
+                        op_dense(a->workspace, 1, static_cast<double>(need))};
   bool over = op_overlap(out[0], out[1]) || op_overlap(out[0], out[2]) || op_overlap(out[1], out[2]);
   for (const OpRows &o : out)
     for (const OpRows &i : in) over |= op_overlap(o, i);

@@ -872,12 +872,12 @@ int check(const hgemm_lora_t *a) {
                                                  a->segments);
   if (need > 0 && (!a->workspace || !op_aligned16(a->workspace) || a->workspace_bytes < need))
     return HGEMM_ERR_INVALID_ARG;
-  const long long T = a->tokens, N = a->N, K = a->K, A = a->segments > 0 ? a->adapters : 0;
-  const OpRows in[] = {op_dense(a->X, 2 * T * K), op_dense(a->W, 2 * K * N), op_dense(a->down, 2 * A * K * a->rank),
-                       op_dense(a->up, 2 * A * a->rank * N), op_dense(a->scale, 4 * A),
-                       op_dense(a->seg_start, A > 0 ? 4ll * a->segments + 4 : 0),
-                       op_dense(a->seg_adapter, A > 0 ? 4ll * a->segments : 0)};
-  const OpRows Y = op_dense(a->Y, 2 * T * N), ws = op_dense(a->workspace, static_cast<long long>(need));
+  const int A = a->segments > 0 ? a->adapters : 0;
+  const OpRows in[] = {op_dense(a->X, 2, a->tokens, a->K), op_dense(a->W, 2, a->K, a->N),
+                       op_dense(a->down, 2, A, a->K, a->rank), op_dense(a->up, 2, A, a->rank, a->N),
+                       op_dense(a->scale, 4, A), op_dense(a->seg_start, 4, A > 0 ? a->segments + 1 : 0),
+                       op_dense(a->seg_adapter, 4, A > 0 ? a->segments : 0)};
+  const OpRows Y = op_dense(a->Y, 2, a->tokens, a->N), ws = op_dense(a->workspace, 1, static_cast<double>(need));
   bool over = op_overlap(Y, ws);
   for (const OpRows &x : in) over |= op_overlap(Y, x) || op_overlap(ws, x);
   return over ? HGEMM_ERR_INVALID_ARG : HGEMM_OK;

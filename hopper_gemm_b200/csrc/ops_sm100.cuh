@@ -62,6 +62,11 @@ struct OpRows {
   long long width, stride, rows;
 };
 inline OpRows op_dense(const void *at, long long bytes) { return {at, bytes, bytes, 1}; }
+// The same of a x b x c elements (sizes that no memory holds end at 2^60 bytes).
+inline OpRows op_dense(const void *at, int size, double a, double b = 1.0, double c = 1.0) {
+  const double bytes = size * a * b * c, most = 1152921504606846976.0;
+  return op_dense(at, static_cast<long long>(bytes < most ? bytes : most));
+}
 // Halves of `heads` heads for each token.
 inline OpRows op_heads(const void *at, long long heads, int head_dim, long long stride, long long tokens) {
   return {at, 2 * heads * head_dim, 2 * stride, tokens};

@@ -255,11 +255,11 @@ int check(const hgemm_qk_norm_rope_t *a) {
     return HGEMM_ERR_INVALID_ARG;
   const OpRows in[] = {op_heads(a->q, a->heads_q, a->head_dim, a->q_stride, a->tokens),
                        op_heads(a->k, a->heads_kv, a->head_dim, a->k_stride, a->tokens),
-                       op_dense(a->q_weight, a->heads_q ? 2 * a->head_dim : 0),
-                       op_dense(a->k_weight, a->heads_kv ? 2 * a->head_dim : 0),
-                       op_dense(a->positions, a->rot_dim ? 4ll * a->axes * a->tokens : 0),
-                       op_dense(a->inv_freq, 2ll * a->rot_dim),
-                       op_dense(a->axis_of, a->axes > 1 ? a->rot_dim / 2 : 0)};
+                       op_dense(a->q_weight, 2, a->heads_q ? a->head_dim : 0),
+                       op_dense(a->k_weight, 2, a->heads_kv ? a->head_dim : 0),
+                       op_dense(a->positions, 4, a->rot_dim ? a->axes : 0, a->tokens),
+                       op_dense(a->inv_freq, 4, a->rot_dim / 2),
+                       op_dense(a->axis_of, 1, a->axes > 1 ? a->rot_dim / 2 : 0)};
   const OpRows out[] = {op_heads(a->q_out, a->heads_q, a->head_dim, a->q_out_stride, a->tokens),
                         op_heads(a->k_out, a->heads_kv, a->head_dim, a->k_out_stride, a->tokens)};
   bool over = op_overlap(out[0], out[1]);

@@ -241,3 +241,13 @@ def test_the_binding_is_built_for_the_installed_torch(tmp_path, monkeypatch):
         assert build._binding_stale(other)
     monkeypatch.setattr(build, "BINDING", str(tmp_path / "_operators.so"))
     assert build._binding_stale(version)
+
+
+def test_products_of_the_largest_sizes_are_no_overlap_by_wrapping():
+    """W of 2^31 x 2^31 halves is more than 64 bits count: it ends somewhere behind every other operand here, and a place
+    inside it is refused."""
+    most = LIMIT - LIMIT % 8
+    st = lora_args(N=most, K=most)
+    assert status(lora_args(N=most, K=most, Y=st.W + (1 << 30))) == BAD
+    assert status(attn_args(total_q=LIMIT, total_k=LIMIT, cu_k=None, heads_q=1 << 20, heads_kv=1 << 20, head_dim=8,
+                            q_stride=1 << 23, k_stride=1 << 23, v_stride=1 << 23, out_stride=1 << 23)) == BAD
